@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/ek.h"
+#include "ek_host.h"
 #include "ek_launch.h"
 
 using ek::KParams;
@@ -34,9 +35,9 @@ struct EkContext {
   long long off_recv_o = 0, off_recv_d = 0, off_cnt_o = 0, off_cnt_d = 0, off_cnt_lm = 0, off_logits = 0;
 };
 
-namespace {
+namespace ek {
 
-thread_local std::string g_err;
+static thread_local std::string g_err;
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -52,11 +53,6 @@ int cuda_fail(cudaError_t e, const char* what) {
   return fail(EK_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 EncodeTiledFn get_encoder() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -70,6 +66,17 @@ EncodeTiledFn get_encoder() {
   });
   return fn;
 }
+
+}  // namespace ek
+
+using ek::aligned16;
+using ek::cuda_fail;
+using ek::DeviceGuard;
+using ek::EncodeTiledFn;
+using ek::fail;
+using ek::get_encoder;
+
+namespace {
 
 // bf16 tensor map of a KV cache [L*T, Hkv, D], box D x 1 head x tk tokens.
 int encode_kv(CUtensorMap* m, const void* base, long long rows, int hkv, int d, int tk,
@@ -86,8 +93,6 @@ int encode_kv(CUtensorMap* m, const void* base, long long rows, int hkv, int d, 
   if (r != CUDA_SUCCESS) return fail(EK_E_INVALID, "tensor map for %s failed (CUresult %d)", name, (int)r);
   return EK_SUCCESS;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int grow(EkContext* ctx, size_t counters, size_t partials) {
   cudaError_t e;
@@ -112,26 +117,13 @@ int grow(EkContext* ctx, size_t counters, size_t partials) {
   return EK_SUCCESS;
 }
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
-
 }  // namespace
 
 extern "C" {
 
 int ek_abi_version(void) { return EK_ABI_VERSION; }
 
-const char* ek_last_error(void) { return g_err.c_str(); }
+const char* ek_last_error(void) { return ek::g_err.c_str(); }
 
 int ek_context_create(int device, EkContext** out) {
   if (!out) return fail(EK_E_INVALID, "out is NULL");

@@ -1,0 +1,155 @@
+// 8-bit KV cache: rows are quantised as they are written and read back as bf16.
+//
+// Per (token, KV head), with D values x: s = bf16_up(max|x| / 127), at least
+// 2^-126; code = round_half_away(x / s); value = code * s. Rounding s up keeps
+// |x| / s <= 127. s has 8 significant bits, as x has, so x / s is either
+// exactly half an integer or at least 1/1020 away from one: 2|x| = (2k + 1) s
+// compares two integers below 2^9 * 2^8 over a common exponent. Adding 2^-12
+// to |x| * (1 / s) (fp32, error below 2^-16) and truncating after + 1/2
+// therefore gives the exact half-away-from-zero code without a division per
+// element.
+//
+// Bound: bytes (2 B in and 1 B out per element for a write, the reverse for a
+// read, plus 2 B of scale per head). A thread moves 16 elements (two 16-byte
+// loads, one 16-byte store), so 4 (D = 64) or 8 (D = 128) lanes share a head
+// and one maximum needs 2 or 3 shuffles.
+#include <cuda_bf16.h>
+
+#include "ek_host.h"
+
+namespace {
+
+struct CopyParams {
+  EkKvTensor values[2], cache[2];  // K, V
+  const int32_t* start;
+  long long start_all;
+  int length, capacity, heads;
+};
+
+constexpr int kThreads = 256;
+
+// Rows of one sequence: blockIdx.x over (row, head), blockIdx.y the sequence, blockIdx.z K or V.
+template <int D, bool WRITE>
+__global__ void __launch_bounds__(kThreads) kv_copy(const CopyParams p) {
+  constexpr int LANES = D / 16;
+  const int b = blockIdx.y, kv = blockIdx.z;
+  const long long at = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES;
+  const bool live = at < (long long)p.length * p.heads;
+  const int i = live ? (int)(at / p.heads) : 0, h = live ? (int)(at % p.heads) : 0;
+  const long long row = (p.start ? (long long)p.start[b] : p.start_all) + i;
+  const bool inside = live && row >= 0 && row < p.capacity;
+  const EkKvTensor& x = p.values[kv];
+  const EkKvTensor& c = p.cache[kv];
+  __nv_bfloat16* value = static_cast<__nv_bfloat16*>(x.data) + b * x.stride_batch + i * x.stride_row +
+                         h * x.stride_head + lane * 16;
+  int8_t* code = static_cast<int8_t*>(c.data) + b * c.stride_batch + row * c.stride_row + h * c.stride_head + lane * 16;
+  __nv_bfloat16* scale = static_cast<__nv_bfloat16*>(c.scales) + b * c.scale_stride_batch +
+                         row * c.scale_stride_row + h * c.scale_stride_head;
+  if (WRITE) {
+    uint32_t w[8] = {};
+    if (inside) {
+      const uint4 lo = __ldg(reinterpret_cast<const uint4*>(value));
+      const uint4 hi = __ldg(reinterpret_cast<const uint4*>(value) + 1);
+      w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
+    }
+    // |x| as integers: NaN > inf > finite
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, max(w[j] << 16 & 0x7fff0000u, w[j] & 0x7fff0000u));
+#pragma unroll
+    for (int m = LANES / 2; m; m >>= 1) top = max(top, __shfl_xor_sync(~0u, top, m));
+    const bool finite = top < 0x7f800000u;
+    unsigned s = (__float_as_uint(__uint_as_float(top) / 127.f) + 0xffffu) & 0xffff0000u;
+    s = finite ? max(s, 0x00800000u) : 0x7fff0000u;
+    const float inv = finite ? 1.f / __uint_as_float(s) : 0.f;
+    if (!inside) return;
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t packed = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t u = e & 1 ? w[2 * j + e / 2] & 0xffff0000u : w[2 * j + e / 2] << 16;
+        const float a = __uint_as_float(u & 0x7fffffffu);
+        int q = finite ? (int)(a * inv + (0.5f + 0x1p-12f)) : 0;
+        q = u & 0x80000000u ? -q : q;
+        packed |= (uint32_t)(q & 0xff) << (8 * e);
+      }
+      out[j] = packed;
+    }
+    *reinterpret_cast<uint4*>(code) = make_uint4(out[0], out[1], out[2], out[3]);
+    if (lane == 0) *scale = __ushort_as_bfloat16((unsigned short)(s >> 16));
+  } else {
+    if (!live) return;
+    uint4 c16 = make_uint4(0, 0, 0, 0);
+    float s = 0.f;
+    if (inside) {
+      c16 = __ldg(reinterpret_cast<const uint4*>(code));
+      s = __bfloat162float(*scale);
+    }
+    const uint32_t w[4] = {c16.x, c16.y, c16.z, c16.w};
+    uint32_t out[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t u = w[j / 2] >> (16 * (j & 1));
+      const __nv_bfloat162 r = __floats2bfloat162_rn((float)(int8_t)(u & 0xff) * s, (float)(int8_t)(u >> 8 & 0xff) * s);
+      out[j] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    reinterpret_cast<uint4*>(value)[0] = make_uint4(out[0], out[1], out[2], out[3]);
+    reinterpret_cast<uint4*>(value)[1] = make_uint4(out[4], out[5], out[6], out[7]);
+  }
+}
+
+bool strides16(const EkKvTensor& t, int elements) {
+  return t.stride_batch % elements == 0 && t.stride_row % elements == 0 && t.stride_head % elements == 0;
+}
+
+int copy(const EkKvCopyArgs* a, void* stream, bool write) {
+  using ek::fail;
+  if (!a) return fail(EK_E_INVALID, "NULL arguments");
+  if (a->batch < 0 || a->length < 0 || a->capacity < 0 || a->kv_heads < 1)
+    return fail(EK_E_INVALID, "bad sizes batch=%d length=%d capacity=%d kv_heads=%d", a->batch, a->length,
+                a->capacity, a->kv_heads);
+  if (a->head_dim != 64 && a->head_dim != 128)
+    return fail(EK_E_UNSUPPORTED, "head_dim %d (supported: 64, 128)", a->head_dim);
+  if (a->batch == 0 || a->length == 0) return EK_SUCCESS;
+  if (a->batch > 65535) return fail(EK_E_UNSUPPORTED, "batch %d (at most 65535)", a->batch);
+  const EkKvTensor* values[2] = {&a->k_values, &a->v_values};
+  const EkKvTensor* cache[2] = {&a->k_cache, &a->v_cache};
+  CopyParams p;
+  for (int i = 0; i < 2; ++i) {
+    if (!values[i]->data || !ek::aligned16(values[i]->data) || !strides16(*values[i], 8))
+      return fail(EK_E_INVALID, "bf16 rows must be 16-byte aligned with strides of 16 bytes");
+    if (a->capacity > 0 && (!cache[i]->data || !cache[i]->scales || !ek::aligned16(cache[i]->data) ||
+                            !strides16(*cache[i], 16)))
+      return fail(EK_E_INVALID, "cache codes must be 16-byte aligned with strides of 16 bytes, with scales");
+    p.values[i] = *values[i];
+    p.cache[i] = *cache[i];
+  }
+  p.start = a->start;
+  p.start_all = a->start_all;
+  p.length = a->length;
+  p.capacity = a->capacity;
+  p.heads = a->kv_heads;
+  const int per_block = kThreads / (a->head_dim / 16);
+  const long long blocks = ((long long)a->length * a->kv_heads + per_block - 1) / per_block;
+  if (blocks > 0x7fffffffll) return fail(EK_E_UNSUPPORTED, "too many rows");
+  ek::DeviceGuard g(a->device);
+  const dim3 grid((unsigned)blocks, a->batch, 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->head_dim == 64) {
+    if (write) kv_copy<64, true><<<grid, kThreads, 0, st>>>(p);
+    else kv_copy<64, false><<<grid, kThreads, 0, st>>>(p);
+  } else {
+    if (write) kv_copy<128, true><<<grid, kThreads, 0, st>>>(p);
+    else kv_copy<128, false><<<grid, kThreads, 0, st>>>(p);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? EK_SUCCESS : ek::cuda_fail(e, write ? "ek_kv_write launch" : "ek_kv_read launch");
+}
+
+}  // namespace
+
+extern "C" int ek_kv_write(const EkKvCopyArgs* a, void* stream) { return copy(a, stream, true); }
+extern "C" int ek_kv_read(const EkKvCopyArgs* a, void* stream) { return copy(a, stream, false); }

@@ -23,6 +23,8 @@ VARIANTS = [
     ("mixtral", {"EK_MODEL": 1, "EK_PF": 0}),
     ("mixtral_pf", {"EK_MODEL": 1, "EK_PF": 1}),
 ]
+# translation units compiled once
+SOURCES = ["ek_capi", "ek_kvcache", "ek_prefix_attn", "ek_sample"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMPILE_FLAGS = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
 LINK_FLAGS = [*ARCH, "-shared", "-cudart", "static"]
@@ -57,7 +59,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         defs = [f"-D{k}={v}" for k, v in macros.items()] + [f"-DEK_NS={name}"]
         jobs.append([nvcc, *COMPILE_FLAGS, *defs, "-c", "-o", str(objdir / f"ek_decode_{name}.o"),
                      str(CSRC / "ek_decode.cu")])
-    jobs.append([nvcc, *COMPILE_FLAGS, "-c", "-o", str(objdir / "ek_capi.o"), str(CSRC / "ek_capi.cu")])
+    for name in SOURCES:
+        jobs.append([nvcc, *COMPILE_FLAGS, "-c", "-o", str(objdir / f"{name}.o"), str(CSRC / f"{name}.cu")])
 
     def run(cmd):
         if verbose:
@@ -67,7 +70,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=len(jobs)) as ex:
         list(ex.map(run, jobs))
     tmp = OUT.with_suffix(".so.tmp")
-    objs = [str(objdir / f"ek_decode_{n}.o") for n, _ in VARIANTS] + [str(objdir / "ek_capi.o")]
+    objs = [str(objdir / f"ek_decode_{n}.o") for n, _ in VARIANTS] + [str(objdir / f"{n}.o") for n in SOURCES]
     run([nvcc, *LINK_FLAGS, "-o", str(tmp), *objs])
     tmp.replace(OUT)
     return OUT

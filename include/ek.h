@@ -271,6 +271,103 @@ int ek_tp_setup(EkContext* ctx, int rank, int world, int num_layers, int hidden,
                 int full_vocab, void* ipc_handle_out, void** logits_out);
 int ek_tp_connect(EkContext* ctx, const void* ipc_handles);
 
+/*
+ * Operators for several sampled continuations of one prompt. They have no
+ * counterpart in the reference. All take plain device pointers on `device`,
+ * run asynchronously on `stream`, allocate nothing and keep nothing between
+ * calls: calls on different streams, threads or captured graphs are
+ * independent as long as their output buffers and workspaces are.
+ */
+
+/* K or V rows of a cache or of a batch of new rows, indexed [batch][row][head][D].
+ * The D elements of a head are contiguous; strides count elements. */
+typedef struct EkKvTensor {
+  void* data;   /* bf16 values, or int8 codes where `scales` is given */
+  void* scales; /* bf16, one scale per (batch, row, head); NULL for bf16 values */
+  int64_t stride_batch, stride_row, stride_head; /* multiples of 16 bytes */
+  int64_t scale_stride_batch, scale_stride_row, scale_stride_head;
+} EkKvTensor;
+
+/* Arguments of ek_kv_write / ek_kv_read: row i of sequence b of the bf16 rows
+ * is cache row start[b] + i of the 8-bit cache. */
+typedef struct EkKvCopyArgs {
+  EkKvTensor k_values, v_values; /* bf16 [batch, length, kv_heads, head_dim] */
+  EkKvTensor k_cache, v_cache;   /* int8 + scales [batch, capacity, kv_heads, head_dim] */
+  const int32_t* start;          /* device int32 [batch], or NULL: start_all for every sequence */
+  int64_t start_all;
+  int32_t batch, length, capacity, kv_heads, head_dim;
+  int32_t device;
+} EkKvCopyArgs;
+
+/* Quantise rows into an 8-bit KV cache. A head's D values share one scale s:
+ * max|x| / 127 rounded up to bf16, at least 2^-126; the codes are x / s rounded
+ * to the nearest integer, halves away from zero. A head that holds a NaN or an
+ * infinity gets the scale NaN (and reads back as NaN). Rows that fall outside
+ * [0, capacity) are not written. head_dim: 64 or 128. */
+int ek_kv_write(const EkKvCopyArgs* args, void* stream);
+
+/* Read rows back: code * scale rounded to bf16. Rows outside [0, capacity) read
+ * as zeros. */
+int ek_kv_read(const EkKvCopyArgs* args, void* stream);
+
+/* Arguments of ek_prefix_attention. */
+typedef struct EkPrefixAttnArgs {
+  const void* q;                          /* bf16 [batch, q_heads, head_dim] */
+  int64_t q_stride_batch, q_stride_head;  /* elements, multiples of 8 */
+  EkKvTensor prefix_k, prefix_v;          /* [1, prefix_len, kv_heads, head_dim] */
+  EkKvTensor own_k, own_v;                /* [batch, own_capacity, kv_heads, head_dim] */
+  const int32_t* own_lens;                /* device int32 [batch]; clamped to [0, max_own_len] */
+  void* out;                              /* bf16 [batch, q_heads, head_dim] */
+  int64_t out_stride_batch, out_stride_head;
+  float* lse;                             /* f32 [batch, q_heads] natural log of the softmax sum, or NULL */
+  void* workspace;                        /* ek_prefix_attention_workspace() bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int32_t batch, q_heads, kv_heads, head_dim;
+  int32_t prefix_len, own_capacity, max_own_len;
+  float scale;
+  int32_t device;
+} EkPrefixAttnArgs;
+
+/* Bytes of workspace that this call needs (contents need not be initialised),
+ * or -1 with ek_last_error() set. Reads only the sizes, `device` and whether
+ * the tensors have scales. */
+int64_t ek_prefix_attention_workspace(const EkPrefixAttnArgs* args);
+
+/* Decode attention of a batch of sequences, one query token each, over a prefix
+ * that all of them share (read once for all) followed by each sequence's own
+ * rows. Prefix and own rows are both bf16 or both 8-bit. A row without any key
+ * gives zeros and lse -inf. */
+int ek_prefix_attention(const EkPrefixAttnArgs* args, void* stream);
+
+/* Arguments of ek_sample. */
+typedef struct EkSampleArgs {
+  const void* logits;   /* bf16 or f32 [batch, vocab] */
+  int64_t row_stride;   /* elements */
+  const float* uniforms; /* f32 [batch], in [0, 1) */
+  /* settings per row (device arrays [batch]), or NULL: the *_all value for every row */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* tokens; /* int64 [batch] */
+  float temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all;
+  int32_t logits_f32; /* 1: logits are f32, 0: bf16 */
+  int32_t batch, vocab;
+  int32_t device;
+} EkSampleArgs;
+
+/* Draw one token per row. With w_i = exp((l_i - max l) / temperature) and the
+ * order (l descending, i ascending): keep the first top_k tokens (<= 0: all),
+ * of those the tokens before which less than top_p of their weight lies
+ * (>= 1: all; the first token always stays), of those the ones with
+ * w_i >= min_p; the token is the first kept i, by index, whose running weight
+ * exceeds uniform * (kept weight). Weights are summed in fixed point
+ * (2^-42 of the largest or finer), so the result does not depend on the
+ * order of the additions. temperature <= 0: the largest logit. NaN logits
+ * count as -inf; a row without any logit above -inf gives 0. */
+int ek_sample(const EkSampleArgs* args, void* stream);
+
 /* Copy the device status record to `out` (synchronises with all work queued
  * on the context's device). With `clear`, reset it to EK_STATUS_OK. */
 int ek_read_status(EkContext* ctx, EkStatus* out, int clear);
