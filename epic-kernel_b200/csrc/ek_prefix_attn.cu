@@ -20,7 +20,10 @@
 // Bound: bytes (4 flops per byte and query row).
 #include <cuda_bf16.h>
 
+#include <cstring>
+
 #include "ek_host.h"
+#include "ek_tcgen05.cuh"
 
 namespace {
 
@@ -49,7 +52,8 @@ struct AttnParams {
   int batch, q_heads, kv_heads, group;
   int prefix_len, max_own;
   int prefix_chunk, own_chunk;    // keys per item
-  int prefix_slots, own_slots;    // items per row
+  int prefix_slots, own_slots;    // items per row, at most
+  int wide_rows, wide_slots, narrow_slots;  // prefix items of the rows of a KV head below wide_rows, and of the others
   int prefix_tiles, group_tiles;  // tiles of 8 rows: of batch * group, of group
   float scale_log2;
 };
@@ -312,6 +316,380 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows(const AttnParams p) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// `many_rows`: the prefix for many query rows, on tcgen05.
+//
+// One block takes one KV head, up to 256 query rows and a range of keys, in
+// tiles of 128 keys. S = Q K^T (128 x 128 fp32) and O += P V (128 x D) stay in
+// tensor memory; P goes back over S as bf16 and is read from there as the A
+// operand. Two softmax warpgroups work in turn with the tensor core: while one
+// takes exponentials, the products of the other run. With more than 128 rows
+// the warpgroups hold two row tiles and share every K and V tile ("wide");
+// with fewer they hold the same rows and take alternate key tiles, each with a
+// running maximum, sum and O of its own ("narrow"). A thread owns one row, so
+// the row maximum and sum need no shuffles. O is rescaled only when a maximum
+// grows by more than 2^8; until then the old one stays in use, which changes
+// no ratio.
+//
+// K and V tiles come by TMA (128-byte swizzle) into a ring, in the order in
+// which the products use them. 8-bit tiles land in a raw ring and four warps
+// widen them to bf16 in the swizzled layout; the scales of keys multiply
+// scores and probabilities, as in few_rows.
+//
+// Bound: 256 rows take 4 * 256 * 128 * D flops a tile, 2048 tensor cycles at
+// D = 128, and 2 * 128 * 128 exponentials, 2048 cycles at 16 a cycle.
+template <int D, bool I8>
+struct Many {
+  static constexpr int BLOCKS = D / 64;               // 64-element column blocks of a tile
+  static constexpr int TILE = 128 * D * 2;            // bytes of a bf16 tile
+  static constexpr int RAW = 128 * D;                 // bytes of an 8-bit tile
+  static constexpr int STAGES = I8 ? (D == 128 ? 3 : 4) : (D == 128 ? 5 : 8);
+  static constexpr int RAW_STAGES = I8 ? (D == 128 ? 3 : 6) : 0;
+  static constexpr int WARPS = I8 ? 14 : 10;          // 8 softmax, [4 widening,] loads, products
+  static constexpr int LOADER = WARPS - 2, MMA = WARPS - 1;
+  static constexpr int OFF_STAGE = 2 * TILE;          // after two Q tiles
+  static constexpr int OFF_RAW = OFF_STAGE + STAGES * TILE;
+  static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;
+  static constexpr int SCALE_BYTES = I8 ? 2 * 2 * 2 * 128 * 4 : 0;  // warpgroup, parity, k / v, key
+  static constexpr int OFF_BAR = OFF_SCALE + SCALE_BYTES;
+  static constexpr int BARS = 2 * STAGES + 2 * RAW_STAGES + 6 + 1;
+  static constexpr int SMEM = OFF_BAR + BARS * 8 + 16 + 1024;  // + alignment
+};
+
+struct ManyParams {
+  CUtensorMap k, v;
+  AttnParams a;
+  int k_keys_first, v_keys_first;  // map dimensions: (D, key, head) instead of (D, head, key)
+  int rows, wide_blocks, narrow_rows;  // rows of a KV head; blocks of 256; rows left for a narrow block
+  int wide_splits, wide_tiles, narrow_splits, narrow_tiles;  // splits of the keys and 128-key tiles of each
+  int negate;                   // scale < 0: q is negated and |scale| used
+};
+
+__device__ int g_attention_status;
+
+// Columns from `keys` on of 32 scores become -inf.
+__device__ __forceinline__ void mask_tail(uint32_t (&x)[32], int keys) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (e >= keys) x[e] = 0xff800000u;
+}
+
+template <int D, bool I8>
+__global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __grid_constant__ ManyParams p) {
+  using C = Many<D, I8>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (ek::smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* raw_full = empty + C::STAGES;
+  uint64_t* raw_empty = raw_full + C::RAW_STAGES;
+  uint64_t* s_full = raw_empty + C::RAW_STAGES;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* drained = o_full + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_at + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  // the item
+  int id = blockIdx.x;
+  const int wide_items = p.wide_blocks * p.wide_splits * p.a.kv_heads;
+  const bool wide = id < wide_items;
+  if (!wide) id -= wide_items;
+  const int splits = wide ? p.wide_splits : p.narrow_splits, per = wide ? p.wide_tiles : p.narrow_tiles;
+  const int split = id % splits;
+  id /= splits;
+  const int head = id % p.a.kv_heads;
+  const int row0 = wide ? id / p.a.kv_heads * 256 : p.wide_blocks * 256;
+  const int row1 = wide ? min(p.rows, row0 + 256) : p.rows;
+  const int tile0 = split * per;
+  const int tiles = min(per, (p.a.prefix_len + 127) / 128 - tile0);
+  const int lead = wide ? 1 : 2;  // K tiles in use before the first V tile
+
+  if (warp == C::MMA) ek::tmem_alloc(tmem_at, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) ek::mbar_init(full + i, I8 ? 128 : 1), ek::mbar_init(empty + i, 1);
+    for (int i = 0; i < C::RAW_STAGES; ++i) ek::mbar_init(raw_full + i, 1), ek::mbar_init(raw_empty + i, 128);
+    for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 128), ek::mbar_init(o_full + i, 1);
+    ek::mbar_init(drained, 1);
+    *abort = 0;
+    ek::fence_mbar_init();
+  }
+  // Q rows, zeros past the last
+  for (int i = threadIdx.x; i < (wide ? 256 : 128) * (D / 8); i += C::WARPS * 32) {
+    const int r = i / (D / 8), piece = i % (D / 8), at = row0 + r;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (at < row1) {
+      const int b = at / p.a.group, h = head * p.a.group + at % p.a.group;
+      x = __ldg(reinterpret_cast<const uint4*>(p.a.q + b * p.a.q_batch + h * p.a.q_head) + piece);
+      if (p.negate) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
+    }
+    const int t = r % 128;
+    *reinterpret_cast<uint4*>(smem + r / 128 * C::TILE + piece / 8 * 16384 + t * 128 + ((piece % 8 ^ (t & 7)) << 4)) = x;
+  }
+  ek::fence_proxy_async_smem();
+  ek::tcgen05_before_sync();
+  __syncthreads();
+  ek::tcgen05_after_sync();
+  const uint32_t tmem = *tmem_at;
+
+  // Ring order of the tiles: K_0 .. K_{lead-1}, then V_i, K_{i+lead} in turn, then the last V.
+  const int items = 2 * tiles;
+  const int lead_now = min(lead, tiles);
+
+  if (warp == C::LOADER) {
+    if (lane == 0) {
+      constexpr int N = I8 ? C::RAW_STAGES : C::STAGES;
+      uint64_t* f = I8 ? raw_full : full;
+      uint64_t* e = I8 ? raw_empty : empty;
+      uint8_t* base = smem + (I8 ? C::OFF_RAW : C::OFF_STAGE);
+      constexpr int BYTES = I8 ? C::RAW : C::TILE;
+      int n = 0;
+      for (; n < items; ++n) {
+        const int s = n % N;
+        if (n >= N && !ek::mbar_wait_bounded(e + s, (n / N - 1) & 1, abort)) break;
+        bool is_v;
+        int tile;
+        if (n < lead_now) is_v = false, tile = n;
+        else {
+          const int m = n - lead_now, both = 2 * (tiles - lead_now);
+          is_v = m >= both || m % 2 == 0;
+          tile = m >= both ? m - (tiles - lead_now) : m / 2 + (is_v ? 0 : lead_now);
+        }
+        const int key = (tile0 + tile) * 128;
+        const CUtensorMap* map = is_v ? &p.v : &p.k;
+        const bool keys_first = is_v ? p.v_keys_first : p.k_keys_first;
+        ek::mbar_arrive_expect_tx(f + s, BYTES);
+        for (int blk = 0; blk < (I8 ? 1 : C::BLOCKS); ++blk)
+          ek::tma_load_3d(base + s * BYTES + blk * 16384, map, blk * 64, keys_first ? key : head,
+                          keys_first ? head : key, f + s);
+      }
+      if (n < items) {  // gave up: let the copies in flight land
+        int quiet = 0;
+        for (int i = max(0, n - N); i < n; ++i) ek::mbar_wait_bounded(f + i % N, (i / N) & 1, &quiet);
+      }
+    }
+  } else if (warp == C::MMA) {
+    if (lane == 0) {
+      constexpr uint32_t SD = ek::mma_desc(128, 128, false), OD = ek::mma_desc(128, D, true);
+      const uint32_t stage = ek::smem_u32(smem + C::OFF_STAGE);
+      int n = 0;  // ring position
+      auto scores = [&](int w, uint32_t k) {
+        const uint32_t q = ek::smem_u32(smem) + (wide ? w * C::TILE : 0);
+#pragma unroll
+        for (int kt = 0; kt < D / 16; ++kt) {
+          const uint32_t off = kt / 4 * 16384 + kt % 4 * 32;
+          ek::mma_ss(tmem + w * 128, ek::smem_desc(q + off, 16), ek::smem_desc(k + off, 16), SD, kt > 0);
+        }
+        ek::mma_commit(s_full + w);
+      };
+      auto values = [&](int w, uint32_t v, bool add) {
+#pragma unroll
+        for (int kt = 0; kt < 8; ++kt)
+          ek::mma_ts(tmem + 256 + w * D, tmem + w * 128 + kt * 8, ek::smem_desc(v + kt * 2048, 16384), OD, add || kt > 0);
+      };
+      auto wait_stage = [&](int i) { return ek::mbar_wait_bounded(full + i % C::STAGES, (i / C::STAGES) & 1, abort); };
+      bool ok = true;
+      for (int i = 0; ok && i < lead_now; ++i) {  // first scores
+        if (!(ok = wait_stage(n))) break;
+        ek::tcgen05_after_sync();
+        const uint32_t k = stage + n % C::STAGES * C::TILE;
+        if (wide) scores(0, k), scores(1, k);
+        else scores(i, k);
+        ek::mma_commit(empty + n % C::STAGES);
+        ++n;
+      }
+      for (int i = 0; ok && i < tiles; ++i) {
+        const bool more = i + lead_now < tiles;
+        const int nv = n, nk = n + 1;
+        n += more ? 2 : 1;
+        for (int turn = 0; turn < (wide ? 2 : 1); ++turn) {
+          const int w = wide ? turn : i % 2, use = wide ? i : i / 2;
+          if (turn == 0 && !(ok = wait_stage(nv))) break;
+          if (!(ok = ek::mbar_wait_bounded(p_full + w, use & 1, abort))) break;
+          ek::tcgen05_after_sync();
+          values(w, stage + nv % C::STAGES * C::TILE, use > 0);
+          const bool last_turn = !wide || turn == 1;
+          if (last_turn) ek::mma_commit(empty + nv % C::STAGES);
+          if (more) {
+            if (turn == 0 && !(ok = wait_stage(nk))) break;
+            ek::tcgen05_after_sync();
+            scores(w, stage + nk % C::STAGES * C::TILE);
+            if (last_turn) ek::mma_commit(empty + nk % C::STAGES);
+          }
+          if (i + (wide ? 1 : 2) >= tiles) ek::mma_commit(o_full + w);
+        }
+      }
+      // tensor memory is freed below: nothing may be in flight
+      int quiet = 0;
+      ek::mma_commit(drained);
+      ek::mbar_wait_bounded(drained, 0, &quiet);
+    }
+  } else if (I8 && warp >= 8) {
+    const int t = threadIdx.x - 256;
+    for (int n = 0; n < items; ++n) {
+      const int rs = n % (I8 ? C::RAW_STAGES : 1), cs = n % C::STAGES;
+      if (!ek::mbar_wait_bounded(raw_full + rs, (n / (I8 ? C::RAW_STAGES : 1)) & 1, abort)) break;
+      if (n >= C::STAGES && !ek::mbar_wait_bounded(empty + cs, (n / C::STAGES - 1) & 1, abort)) break;
+      const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW;
+      uint8_t* to = smem + C::OFF_STAGE + cs * C::TILE;
+#pragma unroll 4
+      for (int i = t; i < 128 * D / 16; i += 128) {
+        const int r = i / (D / 16), piece = i % (D / 16);
+        const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 16);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = codes_to_bf16(__byte_perm(w[e], w[e], 0x1100));
+          y[2 * e + 1] = codes_to_bf16(__byte_perm(w[e], w[e], 0x3322));
+        }
+        // two 16-byte pieces of the 128-byte row; the second block writes them in the other order, so
+        // that the eight lanes of a row hit different banks
+        uint8_t* row = to + piece / 4 * 16384 + r * 128;
+        const int c0 = piece % 4 * 2, flip = D == 128 ? piece / 4 : 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool hi = (e ^ flip) & 1;
+          *reinterpret_cast<uint4*>(row + (((c0 + (hi ? 1 : 0)) ^ (r & 7)) << 4)) =
+              hi ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+      ek::fence_proxy_async_smem();
+      ek::mbar_arrive(full + cs);
+      ek::mbar_arrive(raw_empty + rs);
+    }
+  } else if (warp < 8) {
+    const int w = warp / 4, t = threadIdx.x % 128;
+    const int row = row0 + (wide ? w * 128 : 0) + t;
+    const bool idle = row0 + (wide ? w * 128 : 0) + (warp % 4) * 32 >= row1;  // no row in this warp
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+    const uint32_t ts = lanes + w * 128, to = lanes + 256 + w * D;
+    const int mine = wide ? tiles : (tiles - w + 1) / 2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    const float scale = p.a.scale_log2;
+    auto key_scale = [&](int use, int kv) {
+      const int key = (tile0 + (wide ? use : 2 * use + w)) * 128 + t;
+      if (use >= mine || key >= p.a.prefix_len) return kv ? 0.f : 1.f;  // masked scores stay -inf
+      const Store& s = p.a.prefix;
+      return __bfloat162float(kv ? s.vs[key * s.vs_row + head * s.vs_head] : s.ks[key * s.ks_row + head * s.ks_head]);
+    };
+    float next_ks = 0.f, next_vs = 0.f;
+    if (I8) next_ks = key_scale(0, 0), next_vs = key_scale(0, 1);
+    for (int use = 0; use < mine; ++use) {
+      const int tile = tile0 + (wide ? use : 2 * use + w);
+      const int keys = min(128, p.a.prefix_len - tile * 128);
+      const float* ks = nullptr;
+      const float* vs = nullptr;
+      if (I8) {
+        float* sc = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (w * 2 + (use & 1)) * 256;
+        sc[t] = next_ks * scale, sc[128 + t] = next_vs;
+        if (w == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+        else asm volatile("bar.sync 2, 128;" ::: "memory");
+        ks = sc, vs = sc + 128;
+        next_ks = key_scale(use + 1, 0), next_vs = key_scale(use + 1, 1);
+      }
+      if (!(ok = ek::mbar_wait_bounded(s_full + w, use & 1, abort))) break;
+      ek::tcgen05_after_sync();
+      if (!idle) {
+        // row maximum, in units of scale (base 2)
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t r[2][32];
+        ek::tmem_ld32(r[0], ts);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&x)[32] = r[c & 1];
+          ek::tmem_wait_ld(x);
+          if (c < 3) ek::tmem_ld32(r[(c + 1) & 1], ts + (c + 1) * 32);
+          if (keys < 128) mask_tail(x, keys - c * 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float v = __uint_as_float(x[e]);
+            top[e & 3] = fmaxf(top[e & 3], I8 ? v * ks[c * 32 + e] : v);
+          }
+        }
+        float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (!I8) high *= scale;
+        ek::tmem_ld32(r[0], ts);
+        const float grown = fmaxf(m, high);
+        if (use == 0) m = grown;
+        const float fix = grown - m > 8.f ? exp2_approx(m - grown) : 1.f;  // false for NaN
+        if (__any_sync(~0u, fix != 1.f)) {
+          ek::tmem_wait_ld(r[0]);
+          if (fix != 1.f) m = grown, l *= fix;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            ek::tmem_ld32(r[1], to + c * 32);
+            ek::tmem_wait_ld(r[1]);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[1][e] = __float_as_uint(__uint_as_float(r[1][e]) * fix);
+            ek::tmem_st32(to + c * 32, r[1]);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&x)[32] = r[c & 1];
+          ek::tmem_wait_ld(x);
+          if (c < 3) ek::tmem_ld32(r[(c + 1) & 1], ts + (c + 1) * 32);
+          if (keys < 128) mask_tail(x, keys - c * 32);
+          uint32_t out[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float pr[2];
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const float v = __uint_as_float(x[e + f]);
+              pr[f] = exp2_approx(fmaf(v, I8 ? ks[c * 32 + e + f] : scale, -base));
+              sum[(e + f) & 3] += pr[f];
+              if (I8) pr[f] *= vs[c * 32 + e + f];
+            }
+            out[e / 2] = pack_bf16(pr[0], pr[1]);
+          }
+          ek::tmem_st16(ts + c * 16, out);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        ek::tmem_wait_st();
+      }
+      ek::tcgen05_before_sync();
+      ek::mbar_arrive(p_full + w);
+    }
+    if (ok && mine > 0) ok = ek::mbar_wait_bounded(o_full + w, 0, abort);
+    ek::tcgen05_after_sync();
+    if (!ok) m = NAN, l = NAN;  // a wait ran out: the result is NaN and the status is set
+    if (!idle) {
+      const int b = row / p.a.group, h = head * p.a.group + row % p.a.group;
+      const long long total_rows = (long long)p.a.batch * p.a.q_heads;
+      const long long at = (wide ? split : 2 * split + w) * total_rows + (long long)b * p.a.q_heads + h;
+      if (row < row1) p.a.part_ml[at] = make_float2(m, l);
+      if (mine > 0) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          ek::tmem_ld32(r, to + c * 32);
+          ek::tmem_wait_ld(r);
+          if (row < row1) {
+            uint4* out = reinterpret_cast<uint4*>(p.a.part_o + at * D + c * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+          }
+        }
+      }
+    }
+    ek::tcgen05_before_sync();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort) g_attention_status = 1;
+  if (warp == C::MMA) {
+    ek::tcgen05_after_sync();
+    ek::tmem_free(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // One warp per (sequence, query head) joins its items.
 template <int D>
 __global__ void __launch_bounds__(128) join(const AttnParams p) {
@@ -320,19 +698,23 @@ __global__ void __launch_bounds__(128) join(const AttnParams p) {
   if (row >= rows) return;
   const int b = (int)(row / p.q_heads), h = (int)(row % p.q_heads);
   const int len = min(max(p.own_lens[b], 0), p.max_own);
-  const int parts = p.prefix_slots + (len + p.own_chunk - 1) / p.own_chunk;
+  const int shared = b * p.group + h % p.group < p.wide_rows ? p.wide_slots : p.narrow_slots;
+  const int parts = shared + (len + p.own_chunk - 1) / p.own_chunk;
+  auto place = [&](int i) { return (long long)(i < shared ? i : i - shared + p.prefix_slots) * rows + row; };
   float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[i * rows + row].x);
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
 #pragma unroll
   for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
   const float base = top == -INFINITY ? 0.f : top;
   float o[D / 32] = {}, l = 0.f;
   for (int i = 0; i < parts; ++i) {
-    const float2 ml = p.part_ml[i * rows + row];
+    const long long at = place(i);
+    const float2 ml = p.part_ml[at];
+    if (ml.y == 0.f) continue;  // an item without keys has no o
     const float f = exp2_approx(ml.x - base);
     l += ml.y * f;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[e] += f * p.part_o[(i * rows + row) * D + lane * (D / 32) + e];
+    for (int e = 0; e < D / 32; ++e) o[e] += f * p.part_o[at * D + lane * (D / 32) + e];
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: zeros
   __nv_bfloat16* out = p.out + b * p.out_batch + h * p.out_head + lane * (D / 32);
@@ -344,11 +726,20 @@ __global__ void __launch_bounds__(128) join(const AttnParams p) {
 
 int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Keys per item and items per row, so that the items fill the GPU once or twice.
+// How the keys are split.
 struct Plan {
+  bool many;  // prefix on the tensor core
   int prefix_chunk, prefix_slots, own_chunk, own_slots;
+  int wide_blocks, narrow_rows, wide_splits, wide_tiles, narrow_splits, narrow_tiles;
   long long part_bytes;
 };
+
+// Query rows of a KV head from which many_rows takes the prefix.
+constexpr int kManyRows = 17;
+
+bool has_zero_stride(const EkKvTensor& t, int rows, int heads) {
+  return (rows > 1 && t.stride_row == 0) || (heads > 1 && t.stride_head == 0);
+}
 
 int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   using ek::fail;
@@ -365,21 +756,79 @@ int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   int sms = 0;
   cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, a->device);
   if (e != cudaSuccess) return ek::cuda_fail(e, "cudaDeviceGetAttribute");
-  const int group = a->q_heads / a->kv_heads;
+  std::memset(&pl, 0, sizeof(pl));
+  const int group = a->q_heads / a->kv_heads, rows = a->batch * group;
+  // few_rows: items that fill the GPU about once
   const long long want = 4ll * sms;
-  const long long tiles = (long long)div_up((long long)a->batch * group, 8) * a->kv_heads;
   auto chunk = [&](long long len, long long items) {
     const long long splits = items < want ? div_up(want, items) : 1;
     const long long c = div_up(div_up(len, splits), 64) * 64ll;
     return (int)(c < 64 ? 64 : c);
   };
-  pl.prefix_chunk = chunk(a->prefix_len, tiles > 0 ? tiles : 1);
-  pl.prefix_slots = div_up(a->prefix_len, pl.prefix_chunk);
   const long long own = (long long)a->batch * div_up(group, 8) * a->kv_heads;
   pl.own_chunk = chunk(a->max_own_len, own > 0 ? own : 1);
   pl.own_slots = div_up(a->max_own_len, pl.own_chunk);
+  pl.many = rows >= kManyRows && a->prefix_len > 0 && !has_zero_stride(a->prefix_k, a->prefix_len, a->kv_heads) &&
+            !has_zero_stride(a->prefix_v, a->prefix_len, a->kv_heads);
+  if (!pl.many) {
+    const long long tiles = (long long)div_up(rows, 8) * a->kv_heads;
+    pl.prefix_chunk = chunk(a->prefix_len, tiles > 0 ? tiles : 1);
+    pl.prefix_slots = div_up(a->prefix_len, pl.prefix_chunk);
+  } else {
+    // Blocks of 256 rows (wide), and one of the rest, which is narrow up to 128 rows. A wide tile costs two
+    // units, a narrow one one; the smallest share of units whose items all run at once.
+    pl.wide_blocks = rows / 256 + (rows % 256 > 128);
+    pl.narrow_rows = rows % 256 > 128 ? 0 : rows % 256;
+    const long long tiles = div_up(a->prefix_len, 128), narrow = pl.narrow_rows ? 1 : 0;
+    const long long units = (2ll * pl.wide_blocks + narrow) * tiles * a->kv_heads;
+    const long long blocks = (pl.wide_blocks + narrow) * a->kv_heads;
+    const long long most = blocks <= sms ? sms : 4 * blocks;
+    long long share = div_up(units, most);
+    for (;; ++share) {
+      pl.wide_tiles = div_up(share, 2), pl.narrow_tiles = (int)share;
+      pl.wide_splits = div_up(tiles, pl.wide_tiles), pl.narrow_splits = div_up(tiles, pl.narrow_tiles);
+      if (((long long)pl.wide_blocks * pl.wide_splits + narrow * pl.narrow_splits) * a->kv_heads <= most) break;
+      if (share >= 2 * tiles) break;
+    }
+    const int wide_slots = pl.wide_blocks ? pl.wide_splits : 0, narrow_slots = narrow ? 2 * pl.narrow_splits : 0;
+    pl.prefix_slots = wide_slots > narrow_slots ? wide_slots : narrow_slots;
+  }
   pl.part_bytes = (long long)(pl.prefix_slots + pl.own_slots) * a->batch * a->q_heads * (a->head_dim * 4 + 8);
   return EK_SUCCESS;
+}
+
+// Map of the prefix rows of all heads: boxes of 128 keys of one head, 64 bf16 values (128-byte swizzle) or
+// `d` codes wide. The smaller stride comes first. Keys past the end read as zeros.
+int encode_prefix(CUtensorMap* m, const EkKvTensor& t, int keys, int heads, int d, bool i8, int* keys_first) {
+  ek::EncodeTiledFn enc = ek::get_encoder();
+  if (!enc) return ek::fail(EK_E_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const long long size = i8 ? 1 : 2;
+  long long row = t.stride_row * size, head = t.stride_head * size;
+  if (heads == 1) head = d * size;
+  if (keys == 1) row = head * heads;
+  *keys_first = row < head;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)(*keys_first ? keys : heads),
+                              (cuuint64_t)(*keys_first ? heads : keys)};
+  const cuuint64_t strides[2] = {(cuuint64_t)(*keys_first ? row : head), (cuuint64_t)(*keys_first ? head : row)};
+  const cuuint32_t box[3] = {(cuuint32_t)(i8 ? d : 64), *keys_first ? 128u : 1u, *keys_first ? 1u : 128u};
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = enc(m, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, t.data, dims,
+                         strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return ek::fail(EK_E_INVALID, "tensor map of the prefix failed (CUresult %d)", (int)r);
+  return EK_SUCCESS;
+}
+
+template <int D, bool I8>
+cudaError_t launch_many(const ManyParams& p, cudaStream_t st) {
+  static_assert(Many<D, I8>::SMEM <= 227 * 1024, "shared memory");
+  const cudaError_t e =
+      cudaFuncSetAttribute(many_rows<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<D, I8>::SMEM);
+  if (e != cudaSuccess) return e;
+  const int items = (p.wide_blocks * p.wide_splits + (p.narrow_rows ? p.narrow_splits : 0)) * p.a.kv_heads;
+  many_rows<D, I8><<<items, Many<D, I8>::WARPS * 32, Many<D, I8>::SMEM, st>>>(p);
+  return cudaGetLastError();
 }
 
 // Fills one side of `s`; checks alignment and kind when there are rows.
@@ -404,13 +853,16 @@ int take_store(const EkKvTensor& k, const EkKvTensor& v, bool rows, bool i8, con
 }
 
 template <int D, bool I8>
-cudaError_t launch(const AttnParams& p, cudaStream_t st) {
-  const long long items = (long long)p.prefix_slots * p.prefix_tiles * p.kv_heads +
-                          (long long)p.own_slots * p.group_tiles * p.kv_heads * p.batch;
+cudaError_t launch(const AttnParams& p, const ManyParams* many, cudaStream_t st) {
+  cudaError_t e;
+  if (many && (e = launch_many<D, I8>(*many, st)) != cudaSuccess) return e;
+  AttnParams few = p;
+  if (many) few.prefix_tiles = 0;  // the prefix is taken care of
+  const long long items = (long long)few.prefix_slots * few.prefix_tiles * few.kv_heads +
+                          (long long)few.own_slots * few.group_tiles * few.kv_heads * few.batch;
   if (items > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  if (items > 0) few_rows<D, I8><<<(unsigned)items, kWarps * 32, 0, st>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (items > 0) few_rows<D, I8><<<(unsigned)items, kWarps * 32, 0, st>>>(few);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   join<D><<<div_up((long long)p.batch * p.q_heads, 4), 128, 0, st>>>(p);
   return cudaGetLastError();
 }
@@ -455,11 +907,39 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
   const long long rows = (long long)a->batch * a->q_heads;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (pl.prefix_slots + pl.own_slots) * rows * a->head_dim);
+  p.wide_rows = pl.wide_blocks * 256;
+  p.wide_slots = pl.wide_splits;
+  p.narrow_slots = pl.many ? 2 * pl.narrow_splits : pl.prefix_slots;
   p.scale_log2 = a->scale * kLog2e;
+  ManyParams m;
+  if (pl.many) {
+    if ((rc = encode_prefix(&m.k, a->prefix_k, a->prefix_len, a->kv_heads, a->head_dim, i8, &m.k_keys_first)) ||
+        (rc = encode_prefix(&m.v, a->prefix_v, a->prefix_len, a->kv_heads, a->head_dim, i8, &m.v_keys_first)))
+      return rc;
+    m.a = p;
+    m.rows = a->batch * p.group;
+    m.wide_blocks = pl.wide_blocks, m.narrow_rows = pl.narrow_rows;
+    m.wide_splits = pl.wide_splits, m.wide_tiles = pl.wide_tiles;
+    m.narrow_splits = pl.narrow_splits, m.narrow_tiles = pl.narrow_tiles;
+    // masked scores are -inf times the scale, so it is kept positive; 1e-30 stands for 0
+    m.negate = p.scale_log2 < 0.f;
+    m.a.scale_log2 = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
+  }
+  const ManyParams* many = pl.many ? &m : nullptr;
   ek::DeviceGuard g(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (a->head_dim == 64) e = i8 ? launch<64, true>(p, st) : launch<64, false>(p, st);
-  else e = i8 ? launch<128, true>(p, st) : launch<128, false>(p, st);
+  if (a->head_dim == 64) e = i8 ? launch<64, true>(p, many, st) : launch<64, false>(p, many, st);
+  else e = i8 ? launch<128, true>(p, many, st) : launch<128, false>(p, many, st);
   return e == cudaSuccess ? EK_SUCCESS : ek::cuda_fail(e, "ek_prefix_attention launch");
+}
+
+extern "C" int ek_prefix_attention_status(int device, int32_t* out, int clear) {
+  if (!out) return ek::fail(EK_E_INVALID, "NULL argument");
+  ek::DeviceGuard g(device);
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(out, g_attention_status, sizeof(int32_t));
+  const int32_t zero = 0;
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(zero));
+  return e == cudaSuccess ? EK_SUCCESS : ek::cuda_fail(e, "ek_prefix_attention_status");
 }

@@ -168,6 +168,7 @@ def load_library(path: Path | str | None = None) -> ctypes.CDLL:
                            ("ek_prefix_attention", EkPrefixAttnArgs), ("ek_sample", EkSampleArgs)):
             getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         lib.ek_prefix_attention_workspace.argtypes = [ctypes.POINTER(EkPrefixAttnArgs)]
+        lib.ek_prefix_attention_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int32), ctypes.c_int]
         lib.ek_prefix_attention_workspace.restype = ctypes.c_int64
         if lib.ek_abi_version() != EK_ABI_VERSION:
             raise RuntimeError(f"{p}: ABI {lib.ek_abi_version()} != expected {EK_ABI_VERSION}")

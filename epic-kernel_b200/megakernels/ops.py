@@ -308,6 +308,17 @@ def shared_prefix_attention(q: Tensor, prefix, own, own_lens: Tensor, *, scale: 
     return (out, lse) if return_lse else out
 
 
+def attention_status(device=None, clear: bool = True) -> int:
+    """Synchronise; 1 if a wait inside a `shared_prefix_attention` kernel ran
+    out on `device` since the last clear (the rows concerned are NaN), else 0."""
+    out = ctypes.c_int32()
+    index = torch.device("cuda" if device is None else device).index
+    index = torch.cuda.current_device() if index is None else index
+    ek.check(ek.load_library().ek_prefix_attention_status(index, ctypes.byref(out), int(clear)),
+             "ek_prefix_attention_status")
+    return out.value
+
+
 def _setting(value, name: str, dtype, logits: Tensor):
     """(device pointer or None, scalar) of a setting given as a number or as a
     tensor with one value per row."""

@@ -339,6 +339,10 @@ int64_t ek_prefix_attention_workspace(const EkPrefixAttnArgs* args);
  * gives zeros and lse -inf. */
 int ek_prefix_attention(const EkPrefixAttnArgs* args, void* stream);
 
+/* *out = 1 if a wait inside an ek_prefix_attention kernel on `device` ran out
+ * since the last clear (its rows are NaN then), else 0. Synchronises. */
+int ek_prefix_attention_status(int device, int32_t* out, int clear);
+
 /* Arguments of ek_sample. */
 typedef struct EkSampleArgs {
   const void* logits;   /* bf16 or f32 [batch, vocab] */
