@@ -29,6 +29,7 @@ from torch import Tensor
 from megakernels import ek
 
 _BF16 = torch.bfloat16
+MAX_VOCAB = 393216  # of sample_tokens
 
 
 def _need(t, name: str, dtype, ndim: int | None = None, like: Tensor | None = None) -> Tensor:
@@ -353,8 +354,8 @@ def sample_tokens(logits: Tensor, uniforms: Tensor, *, temperature: float | Tens
     Uniforms outside [0, 1) count as the nearest value inside."""
     _need(logits, "logits", (_BF16, torch.float32), 2)
     batch, vocab = logits.shape
-    if vocab < 1 or vocab > 1 << 22:
-        raise ValueError(f"logits: vocabulary {vocab} (1 .. {1 << 22})")
+    if not 1 <= vocab <= MAX_VOCAB:
+        raise ValueError(f"logits: vocabulary {vocab} (1 .. {MAX_VOCAB})")
     if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("logits: the last dimension must be contiguous")
     _need(uniforms, "uniforms", torch.float32, 1, logits)

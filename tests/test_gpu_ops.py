@@ -288,3 +288,290 @@ def test_attention_repeats_captures_and_streams(kind, B):
     for _, out in graphs:
         assert torch.equal(out, expected)
     assert ops.attention_status(q.device) == 0
+
+
+# ---------------------------------------------------------------------------
+# 8-bit cache
+
+
+def quantise64(x):
+    """(codes, scales) from the definition, in 64 bits."""
+    x = x.double()
+    f, e = torch.frexp(x.abs().amax(-1) / 127)
+    scale = torch.ldexp(torch.ceil(f * 256) / 256, e).clamp_min(2.0**-126)
+    codes = torch.trunc(x / scale[..., None] + torch.copysign(torch.full_like(x, 0.5), x))
+    return codes, scale
+
+
+def check_rows(cache, k, v, starts):
+    n = k.shape[1]
+    for x, codes, scales in ((k, cache.k_codes, cache.k_scales), (v, cache.v_codes, cache.v_scales)):
+        rc, rs = quantise64(x)
+        for b, s in enumerate(starts):
+            assert torch.equal(scales[b, s : s + n].double(), rs[b])
+            assert torch.equal(codes[b, s : s + n].double(), rc[b])
+
+
+@pytest.mark.parametrize("B,n,H,D", [(1, 1, 1, 64), (3, 7, 5, 64), (2, 33, 8, 128), (64, 1, 8, 128), (1, 1000, 3, 128)])
+def test_cache_write_and_read(B, n, H, D):
+    g = gen(20)
+    qkv = normal(g, B, n, 3 * H * D, std=2.0)
+    k, v = qkv[..., H * D : 2 * H * D].unflatten(-1, (H, D)), qkv[..., 2 * H * D :].unflatten(-1, (H, D))
+    cache = ops.KVCacheInt8.empty(B, n + 11, H, D)
+    start = torch.randint(0, 12, (B,), generator=g, device="cuda", dtype=torch.int32)
+    before = [t.fill_(3).clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+    ops.kv_cache_write(cache, k, v, start)
+    check_rows(cache, k, v, start.tolist())
+    for t, old in zip((cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales), before):
+        for b, s in enumerate(start.tolist()):  # other rows are left as they were
+            assert torch.equal(t[b, :s], old[b, :s]) and torch.equal(t[b, s + n :], old[b, s + n :])
+    rk, rv = ops.kv_cache_read(cache, start, n)
+    for got, codes, scales in ((rk, cache.k_codes, cache.k_scales), (rv, cache.v_codes, cache.v_scales)):
+        for b, s in enumerate(start.tolist()):
+            exact = codes[b, s : s + n].double() * scales[b, s : s + n].double()[..., None]
+            assert torch.equal(got[b], exact.to(BF16))
+    # a value is off by at most half a scale, and bf16 rounds by at most 2^-8 of it
+    for got, x, scales in ((rk, k, cache.k_scales), (rv, v, cache.v_scales)):
+        s = torch.stack([scales[b, i : i + n] for b, i in enumerate(start.tolist())]).double()[..., None]
+        assert ((got.double() - x.double()).abs() <= s / 2 + EPS * got.double().abs()).all()
+
+
+def test_cache_ties_round_away_from_zero():
+    """Codes that lie exactly between two integers, for every scale mantissa."""
+    x = torch.zeros(1, 128, 1, 64, device="cuda", dtype=BF16)
+    m = torch.arange(128, 256, device="cuda")
+    x[0, :, 0, 0] = m.to(BF16)
+    values = m[:, None] * torch.arange(1, 32, device="cuda")[None, :] / 64.0
+    x[0, :, 0, 1:32] = values.to(BF16)
+    x[0, :, 0, 32:63] = -values.to(BF16)
+    cache = ops.KVCacheInt8.empty(1, 128, 1, 64)
+    ops.kv_cache_write(cache, x, x, 0)
+    check_rows(cache, x, x, [0])
+
+
+def test_cache_all_bf16_values():
+    """Every finite bf16 value, each next to maxima of many sizes."""
+    bits = torch.arange(0, 65536, device="cuda", dtype=torch.int32).to(torch.int16)
+    x = bits.view(BF16)
+    x = x[x.isfinite()].view(1, -1, 1, 64)[:, :, :, :].contiguous()
+    x = torch.cat([x, x.flip(1)[:, torch.randperm(x.shape[1], generator=gen(21), device="cuda")]], 1)
+    shuffled = x.reshape(-1)[torch.randperm(x.numel(), generator=gen(22), device="cuda")].view_as(x).contiguous()
+    cache = ops.KVCacheInt8.empty(1, x.shape[1], 1, 64)
+    ops.kv_cache_write(cache, x, shuffled, 0)
+    check_rows(cache, x, shuffled, [0])
+
+
+def test_cache_zero_tiny_and_bad_rows():
+    x = torch.zeros(1, 6, 2, 64, device="cuda", dtype=BF16)
+    x[0, 1] = 9.2e-41  # the smallest subnormals
+    x[0, 2, 0, 3] = math.nan
+    x[0, 3, 1, 63] = -math.inf
+    x[0, 4] = 3.3e38
+    cache = ops.KVCacheInt8.empty(1, 6, 2, 64)
+    ops.kv_cache_write(cache, x, x, 0)
+    k, _ = ops.kv_cache_read(cache, 0, 6)
+    assert not k[0, 0].any()
+    assert ((k[0, 1].double() - x[0, 1].double()).abs() <= 2.0**-127).all()
+    assert k[0, 2, 0].isnan().all() and not k[0, 2, 1].any()
+    assert k[0, 3, 1].isnan().all() and not k[0, 3, 0].any()
+    assert ((k[0, 4].double() / x[0, 4].double() - 1).abs() <= 2.0**-8 + 1 / 254).all()
+    assert not cache.k_codes[0, 2, 0].any()
+
+
+def test_cache_rows_outside_are_skipped():
+    g = gen(23)
+    k, v = normal(g, 4, 3, 2, 64), normal(g, 4, 3, 2, 64)
+    cache = ops.KVCacheInt8.empty(4, 8, 2, 64)
+    guard = [t.clone() for t in (cache.k_codes, cache.v_codes)]
+    start = torch.tensor([-3, -1, 7, 8], device="cuda", dtype=torch.int32)
+    ops.kv_cache_write(cache, k, v, start)
+    rk, _ = ops.kv_cache_read(cache, start, 3)
+    assert torch.equal(cache.k_codes[0], guard[0][0]) and torch.equal(cache.v_codes[3], guard[1][3])
+    assert not rk[0].any() and not rk[3].any() and not rk[1, 0].any() and not rk[2, 1:].any()
+    assert rk[1, 1:].any() and rk[2, 0].any()
+    assert torch.equal(cache.k_codes[1, :2].double(), quantise64(k)[0][1, 1:])
+    assert torch.equal(cache.k_codes[2, 7].double(), quantise64(k)[0][2, 0])
+
+
+def test_cache_views_and_out():
+    g = gen(24)
+    big = ops.KVCacheInt8.empty(3, 40, 2, 128)
+    k, v = normal(g, 1, 10, 2, 128), normal(g, 1, 10, 2, 128)
+    part = big.sequence(1).narrow(5, 20)
+    ops.kv_cache_write(part, k, v, 4)
+    check_rows(big.sequence(1), k, v, [9])
+    assert not big.k_codes[0].any() and not big.k_codes[2].any()
+    model = torch.zeros(2, 1, 50, 2, 128, device="cuda", dtype=BF16)
+    rk, rv = ops.kv_cache_read(part, 4, 10, out=(model[0][:, 7:17], model[1][:, 7:17]))
+    assert torch.equal(rk, ops.kv_cache_read(part, 4, 10)[0]) and rk.data_ptr() == model[0][:, 7:].data_ptr()
+    assert not model[:, :, :7].any() and not model[:, :, 17:].any()
+
+
+def test_cache_64_bit_offsets():
+    cache = ops.KVCacheInt8.empty(1, 8_500_000, 4, 64)
+    assert cache.k_codes.numel() > 2**31
+    g = gen(25)
+    k, v = normal(g, 1, 3, 4, 64), normal(g, 1, 3, 4, 64)
+    ops.kv_cache_write(cache, k, v, 8_499_990)
+    check_rows(cache, k, v, [8_499_990])
+    rk, _ = ops.kv_cache_read(cache, 8_499_990, 3)
+    assert rk.any() and not cache.k_codes[0, :100].any()
+
+
+# ---------------------------------------------------------------------------
+# sampling
+
+
+def sample64(logits, u, temperature, top_k, top_p, min_p):
+    """The definition in 64 bits, one row: (token, distance of the draw to the nearest border)."""
+    import numpy as np
+
+    x = logits.double().cpu().numpy().copy()
+    x[np.isnan(x)] = -np.inf
+    if temperature <= 0 or x.max() == -np.inf:
+        return int(x.argmax()), 1.0
+    with np.errstate(invalid="ignore"):
+        w = np.exp((x - x.max()) / temperature)
+    w[x == x.max()] = 1.0
+    order = np.argsort(-x, kind="stable")
+    if 0 < top_k < len(x):
+        order = order[:top_k]
+    if top_p < 1:
+        cum = np.cumsum(w[order])
+        order = order[: max(1, 1 + np.searchsorted(cum, top_p * cum[-1], side="left"))]
+    order = np.sort(order[w[order] >= min_p])
+    cum = np.cumsum(w[order])
+    at = min(np.searchsorted(cum, u * cum[-1], side="right"), len(order) - 1)
+    return int(order[at]), float(np.abs(cum[:-1] / cum[-1] - u).min(initial=1.0))
+
+
+def check_sample(logits, uniforms, **kw):
+    def row(name, default, b):
+        value = kw.get(name, default)
+        return value[b].item() if isinstance(value, torch.Tensor) else float(torch.tensor(value, dtype=torch.float32))
+
+    tokens = ops.sample_tokens(logits, uniforms, **kw)
+    assert tokens.dtype == torch.int64 and tokens.shape == uniforms.shape
+    for b in range(len(uniforms)):
+        u = min(max(uniforms[b].item(), 0.0), 1 - 2.0**-24)
+        want, gap = sample64(logits[b], u, row("temperature", 1.0, b), int(row("top_k", 0, b)), row("top_p", 1.0, b),
+                             row("min_p", 0.0, b))
+        # fixed point resolves 2^-43 of the largest weight; a draw within 1e-10 of a border may fall on either side
+        assert int(tokens[b]) == want or gap < 1e-10, f"row {b}: {int(tokens[b])}, expected {want} (gap {gap})"
+    assert torch.equal(ops.sample_tokens(logits, uniforms, **kw), tokens)
+    return tokens
+
+
+SETTINGS = [{}, {"temperature": 0.6}, {"top_k": 1}, {"top_k": 7}, {"top_k": 300, "temperature": 1.7},
+            {"top_p": 0.9}, {"top_p": 0.5, "top_k": 40}, {"top_p": 0.999}, {"top_p": 0.0}, {"min_p": 0.1},
+            {"min_p": 1.0}, {"top_k": 50, "top_p": 0.95, "min_p": 0.05, "temperature": 0.8},
+            {"temperature": 0.0}, {"temperature": 30.0, "top_p": 0.7}]
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("B,V", [(1, 1), (2, 2), (3, 17), (5, 1000), (2, 32003), (3, 128256), (40, 4097)])
+def test_sample(B, V, dtype, settings):
+    g = gen(30)
+    logits = (torch.randn(B, V, generator=g, device="cuda") * 2).to(dtype)
+    check_sample(logits, torch.rand(B, generator=g, device="cuda"), **settings)
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+@pytest.mark.parametrize("kind", ["equal", "two values", "one high", "wide", "signed zeros", "close", "steps"])
+@pytest.mark.parametrize("dtype", [BF16, torch.float32], ids=["bf16", "f32"])
+def test_sample_shapes_of_rows(kind, dtype, settings):
+    g = gen(31)
+    V = 20011
+    x = torch.randn(2, V, generator=g, device="cuda")
+    if kind == "equal":
+        x = torch.full_like(x, -3.25)
+    elif kind == "two values":
+        x = (x > 1).float()
+    elif kind == "one high":
+        x[:, 777] = 60.0
+    elif kind == "wide":
+        x *= 1e30
+    elif kind == "signed zeros":
+        x = torch.where(x > 0, 0.0, -0.0)
+    elif kind == "close":
+        x = 1000 + x * 1e-3
+    else:
+        x = torch.arange(V, device="cuda").float().expand(2, V).contiguous() / 500
+    check_sample(x.to(dtype), torch.rand(2, generator=g, device="cuda"), **settings)
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, torch.float32], ids=["bf16", "f32"])
+def test_sample_masked_rows(dtype, settings):
+    """-inf, the type's lowest value, NaN and +inf among the logits; rows with nothing, or one token, left."""
+    g = gen(32)
+    V = 5003
+    x = (torch.randn(9, V, generator=g, device="cuda") * 2).to(dtype)
+    x[0, torch.randperm(V, generator=g, device="cuda")[:4900]] = -math.inf
+    x[1] = -math.inf
+    x[2] = -math.inf
+    x[2, 4321] = -7.5
+    x[3] = math.nan
+    x[4, ::2] = math.nan
+    x[5, ::3] = torch.finfo(dtype).min
+    x[6] = torch.finfo(dtype).min
+    x[7, 100] = x[7, 2000] = math.inf
+    x[8, 1:] = -math.inf
+    tokens = check_sample(x, torch.rand(9, generator=g, device="cuda"), **settings)
+    assert tokens[1] == 0 and tokens[3] == 0 and tokens[2] == 4321 and tokens[8] == 0
+
+
+def test_sample_rows_with_settings_of_their_own():
+    g = gen(33)
+    B, V = 64, 12289
+    x = torch.randn(B, V, generator=g, device="cuda") * 3
+    r = lambda: torch.rand(B, generator=g, device="cuda")  # noqa: E731
+    temperature, top_p, min_p = r() * 2, r() * 1.2, r() * 0.2
+    top_k = torch.randint(-3, 100, (B,), generator=g, device="cuda", dtype=torch.int32)
+    temperature[::7] = 0
+    check_sample(x, r(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+def test_sample_uniforms_at_the_ends():
+    g = gen(34)
+    x = torch.randn(1, 999, generator=g, device="cuda").expand(6, 999).contiguous()
+    u = torch.tensor([0.0, 1 - 2.0**-24, 1.0, 2.0, -1.0, 1e-30], device="cuda")
+    t = check_sample(x, u)
+    assert t[0] == 0 and t[1] == 998 and t[2] == t[3] == t[1] and t[4] == 0
+    assert int(ops.sample_tokens(x[:1], torch.full((1,), math.nan, device="cuda"))) == 0
+
+
+def test_sample_frequencies():
+    """Equally spaced uniforms draw every token as often as its weight says, to within one."""
+    n = 4096
+    p = torch.tensor([0.5, 0.25, 0.125, 0.0625, 0.0625], device="cuda")
+    x = p.log().expand(n, 5).contiguous()
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    counts = torch.bincount(ops.sample_tokens(x, u), minlength=5)
+    assert ((counts - p * n).abs() <= 1).all()
+
+
+def test_sample_strided_rows_out_and_capture():
+    g = gen(35)
+    wide_rows = torch.randn(5, 9000, generator=g, device="cuda").to(BF16)
+    x = wide_rows[:, 3:8123]
+    u = torch.rand(5, generator=g, device="cuda")
+    want = check_sample(x, u, top_p=0.9)
+    out = torch.full((7,), -1, device="cuda", dtype=torch.int64)
+    got = ops.sample_tokens(x, u, top_p=0.9, out=out[1:6])
+    assert torch.equal(got, want) and out[0] == -1 and out[6] == -1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ops.sample_tokens(x, u, top_p=0.9)
+    u.copy_(torch.rand(5, generator=g, device="cuda"))
+    graph.replay()
+    assert torch.equal(again, ops.sample_tokens(x, u, top_p=0.9))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32], ids=["bf16", "f32"])
+def test_sample_largest_vocabulary(dtype):
+    g = gen(36)
+    x = torch.randn(2, ops.MAX_VOCAB, generator=g, device="cuda").to(dtype)
+    check_sample(x, torch.rand(2, generator=g, device="cuda"), top_p=0.97, top_k=100_000)
+    check_sample(x, torch.rand(2, generator=g, device="cuda"), top_p=0.97, temperature=5.0)
