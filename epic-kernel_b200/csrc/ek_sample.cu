@@ -2,23 +2,30 @@
 //
 // All filters keep a prefix of the order (logit descending, index ascending),
 // so a cut is a pair: the key of the last kept logit, and how many of its ties
-// stay. top-k counts tokens and top-p adds weights over the same search: a
-// histogram of 512 bins over the logits' range, then histograms over the
-// order-preserving integer keys of the bin that holds the cut, until a bin is
-// one value (two or three passes).
-//
-// Weights are exp((l - max) / T) in double, rounded to fixed point (at least
-// 43 bits below the largest), so every sum is exact, in any order of the
+// stay. Weights are exp((l - max) / T) in double, rounded to fixed point (at
+// least 43 bits below the largest), so every sum is exact, in any order of the
 // atomics, and a launch repeats bit for bit. Single precision would not do: a
 // flat row has 10^5 borders that are 10^-5 apart, and each border's error
 // moves some tokens.
 //
+// Finding a cut. Counts of the logits in 512 equal bins between the maximum
+// and the lowest logit with a weight put a top-k cut into one bin, and, each
+// count times the weight of the bin's centre, a top-p cut into one of three.
+// One pass then adds up all weights exactly (and shows whether the three bins
+// hold the cut; if not, all do), and the logits of those bins go into
+// histograms over their order-preserving integer keys until a bin is one value. When few tokens are left, they are listed instead, and one block
+// ranks them by counting, n^2 comparisons for n <= 512. For top-k <= 512 the
+// bins are filled with the largest logit of each thread only: at least k
+// logits lie at or above the bin where k of those maxima are reached.
+//
 // A row is spread over a cluster of 1 to 8 blocks that hold it in shared
 // memory, so it is read from HBM once; the blocks exchange maxima, histograms
-// and sums through distributed shared memory. Bound: the bytes of the logits
-// for large batches with few kept tokens, else the weights (about 14 double
-// operations each); for one row, the latency of the load and of two cluster
-// barriers per pass.
+// and sums through distributed shared memory. With more rows than such
+// clusters fit at once, one block per row reads it again in each pass (mostly
+// from L2), and with min-p alone it lists the kept tokens in the first pass,
+// against the maximum so far. Bound: for many rows the bytes of the logits;
+// for few the latency of the load and of the barriers, and with a deep top-p
+// cut the weights (about 14 double operations each, twice).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -32,6 +39,9 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = kThreads;
 constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;
+constexpr int kList = 512;   // tokens that one block ranks by counting
+constexpr int kRaw = 4096;   // logits listed against a maximum that still grows
 constexpr int kMaxSlice = 49152;  // elements per block: 192 KB of fp32; a bin's 16-bit limbs add up below 2^32
 using u64 = unsigned long long;
 
@@ -72,15 +82,15 @@ __device__ __forceinline__ float value_of(unsigned key) {
 // last factor is its Taylor polynomial to the fifth power; |r ln 2 / 32| <=
 // 0.0109 leaves an error below 0.0109^6 / 720 = 2.4e-15. The middle one is a
 // table. Both roundings to whole numbers are additions of 1.5 * 2^52.
+// An infinite maximum (then only infinite logits are weighed) counts as the largest finite number.
 struct Weight {
-  float top;
-  double top_d, c;     // c = 32 log2(e) / T
+  double top, c;       // c = 32 log2(e) / T
   const double* table; // 2^(j / 32), shared memory
   int bits;
 
   __device__ __forceinline__ u64 operator()(float l) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
-    const double x = ((double)l - top_d) * c;
+    const double x = ((double)fminf(l, 3.402823466e38f) - top) * c;
     const double shifted = x + kRound;
     const int n = __double2loint(shifted);
     const double r = x - (shifted - kRound);
@@ -94,20 +104,26 @@ struct Weight {
     p *= table[n & 31];
     p = __hiloint2double(__double2hiint(p) + ((n >> 5) + bits) * (1 << 20), __double2loint(p));
     const double whole = p + 4503599627370496.0;  // 2^52: the low bits are the rounded p
-    return l == top ? 1ull << bits : (u64)__double_as_longlong(whole) & 0xfffffffffffffull;
+    return (u64)__double_as_longlong(whole) & 0xfffffffffffffull;
   }
 };
 
 struct Shared {
   unsigned hist[2][3][kBins];  // counts, or the three 16-bit limbs of weights
   double table[32];
+  double c, min_offset;        // 32 log2(e) / T; T ln(min_p)
   u64 scan[kWarps];
   float top[kMaxCluster], low[kMaxCluster];  // maxima and minima of the blocks
   u64 warp_weight[kMaxCluster * kWarps];     // per warp of the cluster: weight above the cut, ties
   unsigned warp_ties[kMaxCluster * kWarps];
-  u64 found_before;
-  int found_bin;
+  u64 block_above[kMaxCluster], block_total[kMaxCluster];
+  u64 total[2], found_before;
+  int found_bin, last_bin;
   int first[kMaxCluster];
+  unsigned running_top;        // key of the largest logit so far
+  int listed;                  // logits appended by this block; beyond kRaw (kList) they did not fit
+  u64 list[kMaxCluster * kMaxSlice / kBins];  // ~key << 32 | index; kList, or all of one range of the index
+  u64 list_weight[kList];
 };
 
 // Inclusive scan over the block's threads.
@@ -130,21 +146,26 @@ __device__ u64 block_scan(u64 v, Shared& sh) {
   return warp ? v + earlier : v;
 }
 
+// The same out of line, for the places that are not hot.
+__device__ __noinline__ u64 weigh_one(const Weight& weight, float l) { return weight(l); }
+
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
   T x[N];
 };
 
-template <typename T>
+// RESIDENT: a cluster holds the row in shared memory. Otherwise one block reads the row again in each pass.
+template <typename T, bool RESIDENT>
 __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p) {
   using V16 = Vec<T>;
   constexpr int N = V16::N;
   extern __shared__ uint4 dynamic[];
   T* slice = reinterpret_cast<T*>(dynamic);
+  u64* raw_list = reinterpret_cast<u64*>(dynamic);  // without a resident slice
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int C = RESIDENT ? cluster.num_blocks() : 1, rank = RESIDENT ? cluster.block_rank() : 0;
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int first = min(p.vocab, rank * p.slice), count = min(p.vocab - first, p.slice);
   const T* row = static_cast<const T*>(p.logits) + b * p.row_stride + first;
@@ -155,47 +176,139 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
   if (C > 1) cluster.barrier_arrive();  // peers' shared memory may be written once all have started
   auto peer = [&](auto* at, int r) { return C > 1 ? cluster.map_shared_rank(at, r) : at; };
 
-  // ---- load the slice (NaN as -inf, padded with -inf), maximum and minimum
   const float inf = INFINITY;
-  float top = -inf, low = inf;
-  auto clean = [&](T x) {
-    const float l = as_float(x);
-    if (l > -inf) top = fmaxf(top, l), low = fminf(low, l);
-    return l == l ? x : (T)-inf;
-  };
-  const int padded = (count + N - 1) / N * N, vectors = padded / N;
-  if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {
-    const int whole = count / N;
-    constexpr int U = 4;
-    for (int i = tid; i < whole; i += U * kThreads) {
-      uint4 w[U];
+  const int vectors = (count + N - 1) / N, whole = count / N;
+  const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+  // vector i of the slice from memory, -inf past the end
+  auto fetch = [&](int i) {
+    V16 v;
+    if (aligned && i < whole) {
+      *reinterpret_cast<uint4*>(&v) = __ldg(reinterpret_cast<const uint4*>(row) + i);
+    } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < whole) w[u] = __ldg(reinterpret_cast<const uint4*>(row) + i + u * kThreads);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < whole) {
-          V16 v = *reinterpret_cast<V16*>(&w[u]);
-#pragma unroll
-          for (int e = 0; e < N; ++e) v.x[e] = clean(v.x[e]);
-          reinterpret_cast<uint4*>(slice)[i + u * kThreads] = *reinterpret_cast<uint4*>(&v);
-        }
+      for (int e = 0; e < N; ++e) v.x[e] = i * N + e < count ? row[i * N + e] : (T)-inf;
     }
-    for (int i = whole * N + tid; i < padded; i += kThreads) slice[i] = i < count ? clean(row[i]) : (T)-inf;
-  } else {
+    return v;
+  };
+  auto vec = [&](int i) {
+    if (!RESIDENT) return fetch(i);
+    const uint4 raw = reinterpret_cast<const uint4*>(slice)[i];
+    return *reinterpret_cast<const V16*>(&raw);
+  };
+  // f(index in the slice, logit) for this thread's share; small bodies, so that a pass stays in the instruction cache
+  auto for_each = [&](auto f) {
+    if (RESIDENT) {
+#pragma unroll 4
+      for (int i = tid; i < count; i += kThreads) f(i, as_float(slice[i]));
+    } else {
+      V16 v, next, later;
+      if (tid < vectors) next = fetch(tid);
+      if (tid + kThreads < vectors) later = fetch(tid + kThreads);
+#pragma unroll 1
+      for (int i = tid; i < vectors; i += kThreads) {
+        v = next, next = later;
+        if (i + 2 * kThreads < vectors) later = fetch(i + 2 * kThreads);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(i * N + e, as_float(v.x[e]));
+      }
+    }
+  };
+
+  // the same, a contiguous range per warp: sums of warps run by index
+  const int per_warp = (vectors + kWarps - 1) / kWarps;
+  const int v0 = min(vectors, warp * per_warp), v1 = min(vectors, v0 + per_warp);
+  // (four logits at a time, -inf past the end: their weights are independent chains of double operations)
+  auto for_each_by_warp = [&](auto f) {
+    const int end = min(count, v1 * N);
+#pragma unroll 1
+    for (int i = v0 * N + lane; i < end; i += 32 * kBatch) {
+      float l[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int at = i + 32 * u;
+        l[u] = at < end ? as_float(RESIDENT ? slice[at] : __ldg(row + at)) : -inf;
+      }
+      f(i, l);
+    }
+  };
+
+  const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
+  const int k = p.top_k ? p.top_k[b] : p.top_k_all;
+  const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
+  const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
+  const bool use_k = k > 0 && k < p.vocab, use_p = top_p < 1.f;
+  // list the kept tokens while the row is read
+  const bool online = !RESIDENT && min_p > 0.f && !use_k && !use_p && temp > 0.f;
+  if (tid == 0) sh.listed = 0, sh.running_top = 0;
+  if (online) {
+    if (tid == 0) sh.min_offset = (double)temp * log((double)fminf(min_p, 1.f));
+    __syncthreads();
+  }
+  // a little below T ln(min_p), for comparisons in single precision
+  const float reach = online ? __double2float_rd(sh.min_offset * 1.000001) : 0.f;
+
+  // ---- the maximum and the minimum above -inf; NaN fails every comparison, here and below
+  float top = -inf, low = online ? -inf : inf;  // (the minimum only narrows the histograms)
+  auto take = [&](float l) {
+    top = fmaxf(top, l);
+    if (!online && l > -inf) low = fminf(low, l);
+  };
+  if (RESIDENT && !aligned) {  // element by element, so that a warp's loads are contiguous
     constexpr int U = 8;
-    for (int i = tid; i < padded; i += U * kThreads) {
+    for (int i = tid; i < vectors * N; i += U * kThreads) {
       T w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < count) w[u] = row[i + u * kThreads];
+      for (int u = 0; u < U; ++u) w[u] = i + u * kThreads < count ? row[i + u * kThreads] : (T)-inf;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < padded)
-          slice[i + u * kThreads] = i + u * kThreads < count ? clean(w[u]) : (T)-inf;
+        if (i + u * kThreads < vectors * N) take(as_float(w[u])), slice[i + u * kThreads] = w[u];
+    }
+  } else {
+    constexpr int U = 4;
+    for (int i = tid; i - lane < vectors; i += U * kThreads) {  // whole warps
+      V16 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < vectors) v[u] = fetch(i + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < vectors) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) take(as_float(v[u].x[e]));
+          if (RESIDENT) reinterpret_cast<uint4*>(slice)[i + u * kThreads] = *reinterpret_cast<uint4*>(&v[u]);
+        }
+      if (online) {
+        // the largest logit seen by any warp bounds the final one from below
+        unsigned key = __reduce_max_sync(~0u, top > -inf ? key_of<float>(top) : 0u);
+        const unsigned seen = *reinterpret_cast<volatile unsigned*>(&sh.running_top);
+        if (key > seen && lane == 0) atomicMax(&sh.running_top, key);
+        key = max(key, seen);
+        const float bar = key ? value_of<float>(key) + reach : inf;
+        const float bar_down = bar < inf ? bar - fabsf(bar) * 0x1p-22f : inf;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i + u * kThreads >= vectors) continue;
+          float most = -inf;
+#pragma unroll
+          for (int e = 0; e < N; ++e) most = fmaxf(most, as_float(v[u].x[e]));
+          if (!(most >= bar_down) || *reinterpret_cast<volatile int*>(&sh.listed) > kRaw) continue;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float l = as_float(v[u].x[e]);
+            if (l >= bar_down && l > -inf) {
+              const int at = atomicAdd(&sh.listed, 1);
+              if (at < kRaw) raw_list[at] = (u64)~key_of<T>(l) << 32 | (unsigned)((i + u * kThreads) * N + e);
+            }
+          }
+        }
+      }
     }
   }
-  if (tid < 32) sh.table[tid] = exp2((double)tid / 32.0);
+  const float mine_top = top;
+  // the slow double functions once, on different warps
+  if (warp == 1) sh.table[lane] = exp2((double)lane / 32.0);
+  if (warp == 2 && lane == 0) sh.c = 46.166241308446828 / (double)temp;
+  if (warp == 3 && lane == 0) sh.min_offset = min_p > 0.f ? (double)temp * log((double)fminf(min_p, 1.f)) : 0.0;
   for (int i = tid; i < 3 * kBins; i += kThreads) sh.hist[0][0][i] = 0;
 #pragma unroll
   for (int m = 16; m; m >>= 1) {
@@ -206,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     float* wt = reinterpret_cast<float*>(sh.scan);
     if (lane == 0) wt[2 * warp] = top, wt[2 * warp + 1] = low;
     __syncthreads();
+    if (C > 1) cluster.barrier_wait();
     if (warp == 0) {
       top = lane < kWarps ? wt[2 * lane] : -inf, low = lane < kWarps ? wt[2 * lane + 1] : inf;
 #pragma unroll
@@ -213,9 +327,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
         top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
         low = fminf(low, __shfl_xor_sync(~0u, low, m));
       }
-    }
-    if (C > 1) cluster.barrier_wait();
-    if (warp == 0) {
       if (lane < C) *peer(&sh.top[rank], lane) = top, *peer(&sh.low[rank], lane) = low;
     }
   }
@@ -223,15 +334,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
   top = sh.top[0], low = sh.low[0];
   for (int r = 1; r < C; ++r) top = fmaxf(top, sh.top[r]), low = fminf(low, sh.low[r]);
 
-  const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
   if (!(temp > 0.f) || top == -inf) {  // the first of the largest; nothing above -inf gives 0
     int at = 0x7fffffff;
     if (top > -inf)
-      for (int i = tid; i < count; i += kThreads)
-        if (as_float(slice[i]) == top) {
-          at = first + i;
-          break;
-        }
+      for_each([&](int i, float l) { at = l == top ? min(at, first + i) : at; });
     at = __reduce_min_sync(~0u, at);
     int* wi = reinterpret_cast<int*>(sh.scan);
     __syncthreads();
@@ -248,137 +354,409 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     }
     return;
   }
-  const int k = p.top_k ? p.top_k[b] : p.top_k_all;
-  const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
-  const Weight weight{top, (double)top, 46.166241308446828 / (double)temp, sh.table, p.weight_bits};
+  const Weight weight{(double)fminf(top, 3.402823466e38f), sh.c, sh.table, p.weight_bits};
   // below `low` a weight rounds to 0 and the token can never be drawn
   low = fmaxf(low, __double2float_ru((double)top - (double)temp * (0.6931471805599453 * (p.weight_bits + 1))));
+  const float u01 = p.uniforms[b];
+  // the draw among a weight of `total`: the first token whose running weight exceeds this
+  auto target = [&](u64 total) {
+    const u64 t = (u64)((double)(u01 > 0.f ? fminf(u01, 1.f) : 0.f) * (double)total);
+    return min(t, total - 1);
+  };
+  // weight that must be reached for top-p; the first token always stays
+  auto share = [&](u64 total) { return max((u64)ceil((double)fmaxf(top_p, 0.f) * (double)total), 1ull); };
 
   // ---- cuts: keys above `cut` stay, and the first `ties` (by index) of those equal to it
   unsigned cut = key_of<T>(low);
   u64 ties = ~0ull;
   if (min_p > 0.f) {
-    const double lowest = (double)top + (double)temp * log((double)fminf(min_p, 1.f));
-    float l = __double2float_ru(lowest);
-    if (sizeof(T) == 2) {  // the next bf16 at or above
-      const __nv_bfloat16 up = __float2bfloat16_ru(l);
-      l = __bfloat162float(up);
-    }
+    float l = __double2float_ru((double)top + sh.min_offset);
+    if (sizeof(T) == 2) l = __bfloat162float(__float2bfloat16_ru(l));  // the next bf16 at or above
     cut = max(cut, key_of<T>(fminf(l, top)));
   }
-  unsigned k_cut = 0;  // top-k keeps keys above, and k_ties equal ones
-  u64 k_ties = 0;
+
+  // Finishes the row from the n listed tokens, which are all that may stay. `goal`: the weight for top-p, 0 if
+  // it follows from the list.
+  auto finish = [&](int n, u64 goal) {
+    int parts = 1;  // neighbouring lanes that share a token
+    while (parts < 32 && n * parts * 2 <= kThreads) parts *= 2;
+    const int i = tid / parts, sub = tid % parts;
+    const u64 own = i < n ? sh.list[i] : 0;
+    const unsigned key = ~(unsigned)(own >> 32);
+    const u64 w = i < n ? weigh_one(weight, value_of<T>(key)) : 0;
+    if (i < n && sub == 0) sh.list_weight[i] = w;
+    __syncthreads();
+    int rank_of = 0;
+    u64 before = 0;
+    for (int j = sub; j < n && (use_k || use_p); j += parts)
+      if (sh.list[j] < own) ++rank_of, before += sh.list_weight[j];
+    for (int m = 1; m < parts; m <<= 1) {
+      rank_of += __shfl_xor_sync(~0u, rank_of, m);
+      before += __shfl_xor_sync(~0u, before, m);
+    }
+    bool stay = i < n && (!use_k || rank_of < k);
+    if (use_p) {
+      if (goal == 0) {
+        const u64 sum = block_scan(stay && sub == 0 ? w : 0, sh);
+        if (tid == kThreads - 1) sh.found_before = sum;
+        __syncthreads();
+        goal = share(sh.found_before);
+      }
+      stay = stay && before < goal;
+    }
+    stay = stay && key >= cut;
+    __syncthreads();
+    if (i < n && sub == 0) sh.list_weight[i] = stay ? w : 0;
+    __syncthreads();
+    u64 total = 0;
+    before = 0;
+    for (int j = sub; j < n; j += parts) {
+      const u64 x = sh.list_weight[j];
+      total += x;
+      if ((unsigned)sh.list[j] < (unsigned)own) before += x;
+    }
+    for (int m = 1; m < parts; m <<= 1) {
+      total += __shfl_xor_sync(~0u, total, m);
+      before += __shfl_xor_sync(~0u, before, m);
+    }
+    if (stay && sub == 0) {
+      const u64 t = target(total);
+      if (before <= t && t < before + w) p.tokens[b] = (long long)(unsigned)own;
+    }
+  };
+  if (online && sh.listed <= kRaw) {
+    // All kept tokens are listed. Their weights by ranges of the index, 512 of them; the range that holds the draw
+    // is small enough to compare its tokens with each other.
+    const int n = sh.listed, wide = (p.vocab + kBins - 1) / kBins;
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 own = raw_list[i];
+      const unsigned key = ~(unsigned)(own >> 32);
+      if (key < cut) continue;  // ruled out by the final maximum
+      const int at = (int)((unsigned)own / wide);
+      const u64 w = weigh_one(weight, value_of<T>(key));
+      atomicAdd(&sh.hist[0][0][at], (unsigned)w & 0xffffu);
+      atomicAdd(&sh.hist[0][1][at], (unsigned)(w >> 16) & 0xffffu);
+      atomicAdd(&sh.hist[0][2][at], (unsigned)(w >> 32));
+    }
+    __syncthreads();
+    const u64 mine = sh.hist[0][0][tid] + ((u64)sh.hist[0][1][tid] << 16) + ((u64)sh.hist[0][2][tid] << 32);
+    const u64 sum = block_scan(mine, sh);
+    if (tid == kThreads - 1) sh.found_before = sum;
+    __syncthreads();
+    const u64 goal = target(sh.found_before);
+    __syncthreads();
+    if (sum > goal && sum - mine <= goal) sh.found_bin = tid, sh.found_before = sum - mine;
+    __syncthreads();
+    const u64 before_range = sh.found_before;
+    const unsigned from = sh.found_bin * wide;
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 own = raw_list[i];
+      if ((unsigned)own - from < (unsigned)wide && ~(unsigned)(own >> 32) >= cut) sh.list[atomicAdd(&sh.listed, 1)] = own;
+    }
+    __syncthreads();
+    for (int i = tid; i < sh.listed; i += kThreads) {
+      const unsigned index = (unsigned)sh.list[i];
+      u64 before = before_range;
+      for (int j = 0; j < sh.listed; ++j)
+        if ((unsigned)sh.list[j] < index) before += weigh_one(weight, value_of<T>(~(unsigned)(sh.list[j] >> 32)));
+      const u64 w = weigh_one(weight, value_of<T>(~(unsigned)(sh.list[i] >> 32)));
+      if (before <= goal && goal < before + w) p.tokens[b] = (long long)index;
+    }
+    return;
+  }
+
   int buffer = 0;
-  const float bins_per = top > low && top < inf ? (float)kBins / (top - low) : 0.f;
-  auto bin_of = [&](float l) { return min((int)((top - l) * bins_per), kBins - 1); };
-  for (int stage = 0; stage < 2; ++stage) {  // 0: top-k; 1: top-p among what top-k left
-    if (stage == 0 ? (k <= 0 || k >= p.vocab) : !(top_p < 1.f)) continue;
-    u64 goal = stage == 0 ? (u64)k : 0, before = 0;
-    unsigned high = 0, base = 0;  // keys still in question
-    int bin1 = -1, shift = 0;
-    bool all = false;
-    for (;;) {
-      auto& hist = sh.hist[buffer];
-      for (int i = tid; i < vectors; i += kThreads) {
-        const uint4 raw = reinterpret_cast<const uint4*>(slice)[i];
-        const V16 v = *reinterpret_cast<const V16*>(&raw);
+  const float bins_per = top > low && top < inf ? fminf((float)(kBins - 1) / (top - low), 3e38f) : 0.f;
+  // (top - l) * bins_per to the nearest whole number, by an addition of 1.5 * 2^23; within 0 .. kBins - 1 for
+  // l >= low. An infinite maximum makes it NaN and the bin kBins - 1.
+  auto bin_of = [&](float l) {
+    return (int)(__float_as_uint(fmaf(top - l, bins_per, 12582912.f)) & (kBins - 1));
+  };
+  // An upper (-1/2) or lower (+1/2) bound of the logits of a bin, widened by the rounding of bin_of.
+  auto edge_of = [&](int bin, float half) {
+    const float margin = (top - low) * 0x1p-18f + fmaxf(fabsf(top), fabsf(low)) * 0x1p-20f;
+    return top - ((float)bin + half) / bins_per - copysignf(margin, half);
+  };
+  // The cluster's sum of bin `tid` of the current histogram (one count, or three limbs); call after sync(). Turns
+  // to the other buffer, which is free: its last readers were past it before that barrier.
+  auto collect = [&](bool limbs) {
+    unsigned h[3][RESIDENT ? kMaxCluster : 1];
+    constexpr int R = RESIDENT ? kMaxCluster : 1;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float l = as_float(v.x[e]);
-          if (!(l >= low)) continue;
-          int bin = bin_of(l);
-          if (bin1 >= 0 && bin != bin1) continue;
-          const unsigned key = key_of<T>(l);
-          if (stage == 1 && key <= k_cut) continue;
-          if (bin1 >= 0) {
-            if (key > high || key < base) continue;
-            bin = (int)((high - key) >> shift);
-          }
-          if (stage == 0) {
-            atomicAdd(&hist[0][bin], 1u);
-          } else {
-            const u64 w = weight(l);
-            atomicAdd(&hist[0][bin], (unsigned)w & 0xffffu);
-            atomicAdd(&hist[1][bin], (unsigned)(w >> 16) & 0xffffu);
-            atomicAdd(&hist[2][bin], (unsigned)(w >> 32));
+    for (int r = 0; r < R; ++r)
+      if (r < C) {
+        const unsigned* other = peer(&sh.hist[buffer][0][0], r);
+        h[0][r] = other[tid];
+        if (limbs) h[1][r] = other[kBins + tid], h[2][r] = other[2 * kBins + tid];
+      }
+    u64 sum = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r < C) sum += limbs ? h[0][r] + ((u64)h[1][r] << 16) + ((u64)h[2][r] << 32) : (u64)h[0][r];
+    buffer ^= 1;
+    for (int i = tid; i < 3 * kBins; i += kThreads) sh.hist[buffer][0][i] = 0;
+    return sum;
+  };
+  // All blocks' lists together in the first block's: their number, or -1 (nothing moved) if they are too many.
+  auto join_lists = [&] {
+    int sum = 0, mine = 0;
+    for (int r = 0; r < C; ++r) {
+      if (r == rank) mine = sum;
+      sum += *peer(&sh.listed, r);
+    }
+    if (sum > kList) return -1;
+    if (rank > 0)
+      for (int i = tid; i < sh.listed; i += kThreads) *peer(&sh.list[mine + i], 0) = sh.list[i];
+    sync();
+    return sum;
+  };
+  auto append = [&](unsigned key, int index) {
+    if (*reinterpret_cast<volatile int*>(&sh.listed) > kList) return;
+    const int at = atomicAdd(&sh.listed, 1);
+    if (at < kList) sh.list[at] = (u64)~key << 32 | (unsigned)index;
+  };
+
+  if (use_k && k <= kList) {  // at least k logits lie in the bins down to that of the k-th largest thread maximum
+    if (tid == 0) sh.listed = 0;
+    if (mine_top >= low) atomicAdd(&sh.hist[buffer][0][bin_of(mine_top)], 1u);
+    sync();
+    const u64 count_here = collect(false);
+    const u64 sum = block_scan(count_here, sh);
+    if (tid == kThreads - 1) sh.found_bin = -1;
+    __syncthreads();
+    if (sum >= (u64)k && sum - count_here < (u64)k) sh.found_bin = tid;
+    __syncthreads();
+    const int last = sh.found_bin;
+    if (last >= 0) {
+      const float bar = last == kBins - 1 || bins_per == 0.f ? low : fmaxf(low, edge_of(last, 0.5f));
+      if (RESIDENT) {  // 16 bytes at a time: most hold nothing above the bar
+#pragma unroll 2
+        for (int i = tid; i < vectors; i += kThreads) {
+          const V16 v = vec(i);
+          float most = as_float(v.x[0]);
+#pragma unroll
+          for (int e = 1; e < N; ++e) most = fmaxf(most, as_float(v.x[e]));
+          if (!(most >= bar)) continue;
+#pragma unroll 1
+          for (int j = i * N; j < (i + 1) * N; ++j) {
+            const float l = as_float(slice[j]);
+            if (l >= bar && bin_of(l) <= last) append(key_of<T>(l), first + j);
           }
         }
+      } else {
+        for_each([&](int i, float l) {
+          if (l >= bar && bin_of(l) <= last) append(key_of<T>(l), first + i);
+        });
       }
       sync();
-      // every block adds up all blocks' bins, one per thread
-      u64 mine = 0;
-      for (int r = 0; r < C; ++r) {
-        const unsigned* other = peer(&hist[0][0], r);
-        mine += other[tid];
-        if (stage == 1) mine += (u64)other[kBins + tid] * 65536ull + ((u64)other[2 * kBins + tid] << 32);
+      const int n = join_lists();
+      if (n >= 0) {
+        if (rank == 0) finish(n, 0);
+        return;
       }
-      // the other buffer is free: its last readers were past it before this barrier
-      buffer ^= 1;
-      for (int i = tid; i < 3 * kBins; i += kThreads) sh.hist[buffer][0][i] = 0;
+    }
+    sync();  // sh.listed and the lists may be used again
+  }
+
+  unsigned weighed_cut = 0;  // the cut of top-p, when `weighed` holds this thread's weights above bin d1
+  u64 weighed = 0;
+  int d1 = 0, d2 = 0;  // the bins that hold a cut
+  unsigned k_cut = 0;  // top-k keeps keys above, and k_ties equal ones
+  u64 k_ties = 0;
+  for (int stage = 0; stage < 2; ++stage) {  // 0: top-k; 1: top-p among what top-k left
+    if (stage == 0 ? !use_k : !use_p) continue;
+    // the lowest logit that takes part; NaN (none) above an infinite k_cut
+    const float next = value_of<T>(k_cut + 1);
+    const float lowest = stage == 0 || k_cut == 0 || next <= low ? low : next;
+    auto takes_part = [&](float l) { return l >= lowest; };
+    if (tid == 0) sh.listed = 0;
+    for_each([&](int, float l) {
+      const int bin = bin_of(l);
+      if (takes_part(l)) atomicAdd(&sh.hist[buffer][0][bin], 1u);
+    });
+    sync();
+    const u64 tied = stage == 1 && k_ties ? k_ties * weigh_one(weight, value_of<T>(k_cut)) : 0;
+    const u64 counted = collect(false);
+    const u64 counts = block_scan(counted, sh);
+    int candidates = kList + 1;
+    u64 goal = 0, before = 0;
+    if (tid == 0) sh.found_bin = kBins;
+    __syncthreads();
+    if (stage == 0) {
+      goal = k;
+      if (counts >= goal && counts - counted < goal) sh.found_bin = tid, sh.found_before = counts - counted;
+      __syncthreads();
+      d1 = d2 = sh.found_bin;
+      if (d1 == kBins) {  // fewer than k have a weight: all stay
+        __syncthreads();
+        continue;
+      }
+      before = sh.found_before;
+    } else {
+      const float centre = bins_per > 0.f ? top - (float)tid / bins_per : top;
+      const u64 about = counted ? counted * weigh_one(weight, fmaxf(centre, low)) : 0;
+      const u64 sum = block_scan(about, sh);
+      if (tid == kThreads - 1) sh.found_before = sum;
+      __syncthreads();
+      const u64 goal_about = share(sh.found_before + tied);
+      if (counted && sum >= goal_about && sum - about < goal_about) sh.found_bin = tid;
+      __syncthreads();
+      const int found = sh.found_bin;  // kBins: the cut seems to lie among the ties of top-k
+      d1 = found == kBins ? kBins : max(found - 1, 0);
+      d2 = found == kBins ? kBins : min(found + 1, kBins - 1);
+      if (tid == d2) sh.found_before = counts;
+      __syncthreads();
+      if (d2 < kBins && k_ties == 0) candidates = (int)min(sh.found_before, (u64)kList + 1);
+    }
+    unsigned high, base;  // keys still in question
+    auto keys_of_bins = [&] {
+      high = key_of<T>(top), base = key_of<T>(low);
+      if (bins_per > 0.f) {
+        const float hi = edge_of(d1, -0.5f), lo = edge_of(d2, 0.5f);
+        if (hi < top) high = key_of<T>(hi);
+        if (lo > low && d2 < kBins - 1) base = key_of<T>(lo);
+        high = max(high, base);
+      }
+    };
+    keys_of_bins();
+    bool gather = candidates <= kList;
+    bool all = false, weigh = stage == 1, reuse = true;  // all weights are added up once
+    for (int pass = 0;;) {
+      const unsigned span = high - base;  // bins of 2^shift keys
+      const int shift = span < kBins ? 0 : 32 - __clz(span) - 9;
+      u64 above = 0, total = 0;
+      auto count_key = [&](float l) {  // into the histogram of keys
+        const unsigned key = key_of<T>(l);
+        if (pass > 0 && (key > high || key < base)) return;
+        const int at = key > high ? 0 : (int)((high - max(key, base)) >> shift);
+        if (stage == 0) {
+          atomicAdd(&sh.hist[buffer][0][at], 1u);
+        } else {
+          const u64 w = weigh_one(weight, l);
+          atomicAdd(&sh.hist[buffer][0][at], (unsigned)w & 0xffffu);
+          atomicAdd(&sh.hist[buffer][1][at], (unsigned)(w >> 16) & 0xffffu);
+          atomicAdd(&sh.hist[buffer][2][at], (unsigned)(w >> 32));
+        }
+      };
+      if (weigh) {  // all weights are added up once
+        for_each_by_warp([&](int i, const float (&l)[kBatch]) {
+          u64 w[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) w[u] = weight(fmaxf(l[u], low));
+          unsigned hits = 0;
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int bin = bin_of(l[u]);
+            const bool in = takes_part(l[u]);
+            total += in ? w[u] : 0;
+            above += in && bin < d1 ? w[u] : 0;
+            hits |= in && bin <= d2 && (gather || bin >= d1) ? 1u << u : 0;
+          }
+          while (hits) {
+            const int u = __ffs(hits) - 1;
+            hits &= hits - 1;
+            const int at = i + 32 * u;
+            const float x = as_float(RESIDENT ? slice[at] : row[at]);
+            if (gather) append(key_of<T>(x), first + at);
+            if (bin_of(x) >= d1) count_key(x);
+          }
+        });
+      } else {
+        for_each([&](int, float l) {
+          const int bin = bin_of(l);
+          if (bin >= d1 && bin <= d2 && takes_part(l)) count_key(l);
+        });
+      }
+      if (weigh) {  // the block's sums to every block
+        weighed = above;
+        const u64 block_above = block_scan(above, sh);
+        __syncthreads();
+        const u64 block_total = block_scan(total, sh);
+        if (tid == kThreads - 1)
+          for (int r = 0; r < C; ++r)
+            *peer(&sh.block_above[rank], r) = block_above, *peer(&sh.block_total[rank], r) = block_total;
+      }
+      sync();
+      if (weigh) {
+        u64 sum = tied;
+        for (int r = 0; r < C; ++r) sum += sh.block_total[r], before += sh.block_above[r];
+        goal = share(sum);
+      }
+      const u64 mine = collect(stage == 1);
       const u64 sum = before + block_scan(mine, sh);
       if (tid == kThreads - 1) sh.found_bin = kBins, sh.found_before = sum;
       __syncthreads();
-      if (bin1 < 0) {
-        const u64 total = sh.found_before;
-        if (stage == 1) {
-          const u64 tied = k_ties ? k_ties * weight(value_of<T>(k_cut)) : 0;
-          goal = (u64)ceil((double)fmaxf(top_p, 0.f) * (double)(total + tied));
-          goal = goal < 1 ? 1 : goal;  // the first token always stays
-        }
-        all = total < goal;  // the cut lies below all of these
-      }
+      const bool below = sh.found_before < goal, beside = before >= goal;
       __syncthreads();
-      if (all) break;
+      if (beside || below) {
+        all = below && d1 == kBins;  // among the ties of top-k
+        if (all || d2 - d1 == kBins - 1) {
+          all = true;
+          break;
+        }
+        d1 = 0, d2 = kBins - 1, before = 0;  // not in these bins: search all
+        keys_of_bins();
+        gather = weigh = reuse = false;
+        continue;
+      }
+      weigh = false;
+      if (gather) {
+        gather = false;
+        const int n = join_lists();
+        if (n >= 0) {
+          if (rank == 0) finish(n, goal);
+          return;
+        }
+      }
       if (sum >= goal && sum - mine < goal) sh.found_bin = tid, sh.found_before = sum - mine;
       __syncthreads();
-      const int found = sh.found_bin;
       before = sh.found_before;
-      if (bin1 < 0) {
-        // bounds of the bin, widened by the rounding of bin_of; bin1 itself stays the filter
-        bin1 = found;
-        high = key_of<T>(top), base = key_of<T>(low);
-        if (bins_per > 0.f) {
-          const float margin = (top - low) * 0x1p-18f + fmaxf(fabsf(top), fabsf(low)) * 0x1p-20f;
-          const float hi = top - (float)found / bins_per + margin, lo = top - (float)(found + 1) / bins_per - margin;
-          if (hi < top) high = key_of<T>(hi);
-          if (lo > low && found < kBins - 1) base = key_of<T>(lo);
-        }
-      } else {
-        high -= (unsigned)found << shift;
-        if (shift == 0) break;
-        base = max(base, high - ((1u << shift) - 1u));
-      }
-      const unsigned span = high - base;  // bins of 2^shift keys
-      shift = span < kBins ? 0 : 32 - __clz(span) - 9;
+      high -= (unsigned)sh.found_bin << shift;
+      if (shift == 0 || ++pass == 4) break;  // 9 bits a pass: shift is at most 23, 14, 5, 0
+      base = max(base, high - ((1u << shift) - 1u));
     }
-    __syncthreads();
-    if (all && stage == 0) continue;
-    const unsigned key = all ? k_cut : high;
     if (all) before = sh.found_before;
-    const u64 unit = stage == 0 ? 1 : weight(value_of<T>(key));
-    u64 r = (goal - before + unit - 1) / unit;
+    __syncthreads();
+    const unsigned key = all ? k_cut : high;
+    const u64 unit = stage == 0 ? 1 : weigh_one(weight, value_of<T>(key));
+    u64 r = (goal - before + unit - 1) / max(unit, 1ull);
     if (stage == 0) k_cut = key, k_ties = r;
     else if (all) r = min(r, k_ties);
+    else if (reuse) weighed_cut = key;
     if (key > cut) cut = key, ties = r;
     else if (key == cut) ties = min(ties, r);
   }
 
   // ---- the draw: a warp owns a contiguous range, so that sums run by index
-  const int per_warp = (vectors + kWarps - 1) / kWarps;
-  const int v0 = min(vectors, warp * per_warp), v1 = min(vectors, v0 + per_warp);
   const float cut_value = value_of<T>(cut);
   u64 above = 0;
   unsigned tied = 0;
-  for (int i = v0 + lane; i < v1; i += 32) {
-    const uint4 raw = reinterpret_cast<const uint4*>(slice)[i];
-    const V16 v = *reinterpret_cast<const V16*>(&raw);
+  if (cut == weighed_cut) {  // top-p has added up all weights but those of its bins
+    above = weighed;
+    for_each_by_warp([&](int, const float (&l)[kBatch]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float l = as_float(v.x[e]);
-      if (l > cut_value) above += weight(l);
-      else if (l == cut_value) ++tied;
-    }
+      for (int u = 0; u < kBatch; ++u) {
+        tied += l[u] == cut_value;
+        if (l[u] > cut_value && bin_of(l[u]) >= d1) above += weigh_one(weight, l[u]);
+      }
+    });
+  } else {
+    for_each_by_warp([&](int, const float (&l)[kBatch]) {
+      bool any = false;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        tied += l[u] == cut_value;
+        any |= l[u] > cut_value;
+      }
+      if (!any) return;
+      u64 w[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) w[u] = weight(fmaxf(l[u], cut_value));
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) above += l[u] > cut_value ? w[u] : 0;
+    });
   }
   tied = __reduce_add_sync(~0u, tied);
 #pragma unroll
@@ -389,8 +767,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
   }
   sync();
   // each warp finds the range that holds the draw from all warps' sums, four per lane
-  const u64 unit = weight(cut_value);
-  constexpr int E = kMaxCluster * kWarps / 32;
+  const u64 unit = weigh_one(weight, cut_value);
+  constexpr int E = (RESIDENT ? kMaxCluster : 2) * kWarps / 32;
   u64 w[E], t[E], weights = 0, tie_sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -420,10 +798,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     const u64 o = __shfl_up_sync(~0u, upto, m);
     if (lane >= m) upto += o;
   }
-  const u64 total = __shfl_sync(~0u, upto, 31);
-  const float u = p.uniforms[b];
-  u64 goal = (u64)((double)(u > 0.f ? fminf(u, 1.f) : 0.f) * (double)total);
-  goal = min(goal, total - 1);
+  const u64 goal = target(__shfl_sync(~0u, upto, 31));
   u64 running = upto - weights;
   int owner = -1;
   u64 owner_before = 0, owner_ties = 0;
@@ -432,23 +807,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     if (owner < 0 && running <= goal && goal < running + w[e]) owner = lane * E + e, owner_before = running, owner_ties = ahead[e];
     running += w[e];
   }
-  const unsigned who = __ballot_sync(~0u, owner >= 0);
-  const int from = __ffs(who) - 1;
+  const int from = __ffs(__ballot_sync(~0u, owner >= 0)) - 1;
   owner = __shfl_sync(~0u, owner, from);
   if (owner == rank * kWarps + warp) {
     u64 sum = __shfl_sync(~0u, owner_before, from), seen = __shfl_sync(~0u, owner_ties, from);
     for (int i0 = v0; i0 < v1; i0 += 32) {
       const int i = i0 + lane;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (i < v1) raw = reinterpret_cast<const uint4*>(slice)[i];
-      const V16 v = *reinterpret_cast<const V16*>(&raw);
+      V16 v;
       unsigned mine = 0;
       u64 heavy = 0;
+      if (i < v1) {
+        v = vec(i);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float l = as_float(v.x[e]);
-        if (i < v1 && l == cut_value) ++mine;
-        if (i < v1 && l > cut_value) heavy += weight(l);
+        for (int e = 0; e < N; ++e) {
+          const float l = as_float(v.x[e]);
+          mine += l == cut_value;
+          if (l > cut_value) heavy += weigh_one(weight, l);
+        }
       }
       unsigned tb = mine;
 #pragma unroll
@@ -471,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float l = as_float(v.x[e]);
-          if (l > cut_value) at += weight(l);
+          if (l > cut_value) at += weigh_one(weight, l);
           else if (l == cut_value && tt++ < ties) at += unit;
           if (pick < 0 && at > goal) pick = e;
         }
@@ -487,8 +862,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
 
 template <typename T>
 cudaError_t launch(const SampleParams& p, int batch, int cluster, cudaStream_t st) {
+  if (cluster == 0) {
+    const cudaError_t e = cudaFuncSetAttribute(sample_rows<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kRaw * (int)sizeof(u64));
+    if (e != cudaSuccess) return e;
+    sample_rows<T, false><<<batch, kThreads, kRaw * sizeof(u64), st>>>(p);
+    return cudaGetLastError();
+  }
   const int bytes = p.slice * (int)sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(sample_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(sample_rows<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kMaxSlice * (int)sizeof(T));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -501,7 +883,7 @@ cudaError_t launch(const SampleParams& p, int batch, int cluster, cudaStream_t s
   attr.val.clusterDim.x = cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_rows<T>, p);
+  return cudaLaunchKernelEx(&cfg, sample_rows<T, true>, p);
 }
 
 }  // namespace
@@ -534,14 +916,14 @@ extern "C" int ek_sample(const EkSampleArgs* a, void* stream) {
   int bits = 62;
   for (long long n = 1; n < a->vocab; n *= 2) --bits;
   p.weight_bits = bits < 46 ? bits : 46;
-  // Blocks per row: as many as keep 2048 elements each, up to 8, so that a few rows use the whole cluster's
-  // bandwidth; with many rows, only as many as hold the row in 64 KB each (three blocks fit an SM).
+  // Blocks per row: up to 8 that keep 2048 elements each and run at once with the other rows' (two blocks fit an
+  // SM). A row that would not fit so few blocks is read in every pass by one block (0).
   int cluster = 1;
-  while (cluster < kMaxCluster &&
-         ((long long)a->vocab * size > cluster * 65536ll ||
-          (a->vocab >= cluster * 4096 && (long long)a->batch * cluster < 296)))
-    cluster *= 2;
-  p.slice = (int)(((long long)a->vocab + cluster - 1) / cluster + 15) / 16 * 16;
+  while (cluster < kMaxCluster && a->vocab >= cluster * 4096 && (long long)a->batch * cluster * 2 <= 296) cluster *= 2;
+  if ((long long)a->vocab * size > cluster * (cluster == kMaxCluster ? (long long)kMaxSlice * size : 96 * 1024ll))
+    cluster = 0;
+  const int blocks = cluster ? cluster : 1;
+  p.slice = (int)(((long long)a->vocab + blocks - 1) / blocks + 15) / 16 * 16;
   ek::DeviceGuard g(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = a->logits_f32 ? launch<float>(p, a->batch, cluster, st)

@@ -477,6 +477,27 @@ def test_sample(B, V, dtype, settings):
     check_sample(logits, torch.rand(B, generator=g, device="cuda"), **settings)
 
 
+@pytest.mark.parametrize("settings", SETTINGS + [{"min_p": 0.5}, {"top_k": 2000, "top_p": 0.8}], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, torch.float32], ids=["bf16", "f32"])
+def test_sample_many_rows(dtype, settings):
+    """More rows than resident clusters; ragged row starts, rising rows (the maximum comes last), masked rows."""
+    g = gen(37)
+    B, V = 160, 100_003
+    x = torch.randn(B, V, generator=g, device="cuda").mul_(2)
+    x[1] = torch.arange(V, device="cuda") / 9000.0
+    x[2] = 0.5
+    x[3, 1:] = -math.inf
+    x[4] = -math.inf
+    x[5, ::2] = math.nan
+    x[6, 50_000] = x[6, 70_000] = math.inf
+    x[7, 99_999] = 40.0
+    x = x.to(dtype)
+    rows = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, 20, 99, 159], device="cuda")
+    u = torch.rand(B, generator=g, device="cuda")
+    tokens = ops.sample_tokens(x, u, **settings)
+    assert torch.equal(tokens[rows], check_sample(x[rows], u[rows], **settings))
+
+
 @pytest.mark.parametrize("settings", SETTINGS, ids=str)
 @pytest.mark.parametrize("kind", ["equal", "two values", "one high", "wide", "signed zeros", "close", "steps"])
 @pytest.mark.parametrize("dtype", [BF16, torch.float32], ids=["bf16", "f32"])
