@@ -8,12 +8,13 @@
 // flat row has 10^5 borders that are 10^-5 apart, and each border's error
 // moves some tokens.
 //
-// Finding a cut. Counts of the logits in 512 equal bins between the maximum
+// Finding a cut. Counts of the logits in 1024 (or 512) equal bins between the maximum
 // and the lowest logit with a weight put a top-k cut into one bin, and, each
-// count times the weight of the bin's centre, a top-p cut into one of three.
-// One pass then adds up all weights exactly (and shows whether the three bins
-// hold the cut; if not, all do), and the logits of those bins go into
-// histograms over their order-preserving integer keys until a bin is one value. When few tokens are left, they are listed instead, and one block
+// count times the weight of the bin's centre, a top-p cut into one or two. One
+// pass then adds up all weights exactly (which shows whether those bins hold
+// the cut; if not, all logits are searched) and lists the logits of those bins,
+// which go into histograms over their order-preserving integer keys until a
+// bin is one value. When few tokens are left, they are listed instead, and one block
 // ranks them by counting, n^2 comparisons for n <= 512. For top-k <= 512 the
 // bins are filled with the largest logit of each thread only: at least k
 // logits lie at or above the bin where k of those maxima are reached.
@@ -35,14 +36,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kBins = kThreads;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxElements = 65536;    // per block: a bin's 16-bit limbs add up below 2^32
+constexpr int kMaxBytes = 176 * 1024;  // of logits per block
 constexpr int kBatch = 4;
 constexpr int kList = 512;   // tokens that one block ranks by counting
+constexpr int kRoom = 1024;  // a block's list; also room for all of one of 512 ranges of the index
 constexpr int kRaw = 4096;   // logits listed against a maximum that still grows
-constexpr int kMaxSlice = 49152;  // elements per block: 192 KB of fp32; a bin's 16-bit limbs add up below 2^32
+constexpr int kMaxVocab = kMaxCluster * kMaxBytes / 4;
 using u64 = unsigned long long;
 
 struct SampleParams {
@@ -108,7 +109,9 @@ struct Weight {
   }
 };
 
+template <int kThreads>
 struct Shared {
+  static constexpr int kWarps = kThreads / 32, kBins = kThreads;
   unsigned hist[2][3][kBins];  // counts, or the three 16-bit limbs of weights
   double table[32];
   double c, min_offset;        // 32 log2(e) / T; T ln(min_p)
@@ -121,13 +124,28 @@ struct Shared {
   int found_bin, last_bin;
   int first[kMaxCluster];
   unsigned running_top;        // key of the largest logit so far
-  int listed;                  // logits appended by this block; beyond kRaw (kList) they did not fit
-  u64 list[kMaxCluster * kMaxSlice / kBins];  // ~key << 32 | index; kList, or all of one range of the index
+  int listed;                  // logits appended by this block; beyond kRaw (kRoom) they did not fit
+  u64 extra[kWarps];           // listed logits above the cut, by the warp that owns their index: weight and ties
+  unsigned extra_ties[kWarps];
+  u64 list[kRoom];             // ~key << 32 | index
   u64 list_weight[kList];
 };
 
+// ceil(a / b) for quotients below 2^20: one float division, off by at most one, put right.
+__device__ __forceinline__ u64 quotient_up(u64 a, u64 b) {
+  u64 q = (u64)(unsigned)__fdividef((float)a, (float)b);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (q > 0 && (q - 1) * b >= a) --q;
+    if (q * b < a) ++q;
+  }
+  return q;
+}
+
 // Inclusive scan over the block's threads.
-__device__ u64 block_scan(u64 v, Shared& sh) {
+template <int kThreads>
+__device__ u64 block_scan(u64 v, Shared<kThreads>& sh) {
+  constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
@@ -146,9 +164,6 @@ __device__ u64 block_scan(u64 v, Shared& sh) {
   return warp ? v + earlier : v;
 }
 
-// The same out of line, for the places that are not hot.
-__device__ __noinline__ u64 weigh_one(const Weight& weight, float l) { return weight(l); }
-
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
@@ -156,14 +171,16 @@ struct Vec {
 };
 
 // RESIDENT: a cluster holds the row in shared memory. Otherwise one block reads the row again in each pass.
-template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p) {
+template <typename T, bool RESIDENT, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const SampleParams p) {
+  constexpr int kWarps = kThreads / 32, kBins = kThreads;
+  constexpr int kBinBits = kThreads == 1024 ? 10 : 9;
   using V16 = Vec<T>;
   constexpr int N = V16::N;
   extern __shared__ uint4 dynamic[];
   T* slice = reinterpret_cast<T*>(dynamic);
   u64* raw_list = reinterpret_cast<u64*>(dynamic);  // without a resident slice
-  __shared__ Shared sh;
+  __shared__ Shared<kThreads> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = RESIDENT ? cluster.num_blocks() : 1, rank = RESIDENT ? cluster.block_rank() : 0;
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -383,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     const int i = tid / parts, sub = tid % parts;
     const u64 own = i < n ? sh.list[i] : 0;
     const unsigned key = ~(unsigned)(own >> 32);
-    const u64 w = i < n ? weigh_one(weight, value_of<T>(key)) : 0;
+    const u64 w = i < n ? weight(value_of<T>(key)) : 0;
     if (i < n && sub == 0) sh.list_weight[i] = w;
     __syncthreads();
     int rank_of = 0;
@@ -433,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
       const unsigned key = ~(unsigned)(own >> 32);
       if (key < cut) continue;  // ruled out by the final maximum
       const int at = (int)((unsigned)own / wide);
-      const u64 w = weigh_one(weight, value_of<T>(key));
+      const u64 w = weight(value_of<T>(key));
       atomicAdd(&sh.hist[0][0][at], (unsigned)w & 0xffffu);
       atomicAdd(&sh.hist[0][1][at], (unsigned)(w >> 16) & 0xffffu);
       atomicAdd(&sh.hist[0][2][at], (unsigned)(w >> 32));
@@ -460,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
       const unsigned index = (unsigned)sh.list[i];
       u64 before = before_range;
       for (int j = 0; j < sh.listed; ++j)
-        if ((unsigned)sh.list[j] < index) before += weigh_one(weight, value_of<T>(~(unsigned)(sh.list[j] >> 32)));
-      const u64 w = weigh_one(weight, value_of<T>(~(unsigned)(sh.list[i] >> 32)));
+        if ((unsigned)sh.list[j] < index) before += weight(value_of<T>(~(unsigned)(sh.list[j] >> 32)));
+      const u64 w = weight(value_of<T>(~(unsigned)(sh.list[i] >> 32)));
       if (before <= goal && goal < before + w) p.tokens[b] = (long long)index;
     }
     return;
@@ -513,9 +530,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     return sum;
   };
   auto append = [&](unsigned key, int index) {
-    if (*reinterpret_cast<volatile int*>(&sh.listed) > kList) return;
+    if (*reinterpret_cast<volatile int*>(&sh.listed) > kRoom) return;
     const int at = atomicAdd(&sh.listed, 1);
-    if (at < kList) sh.list[at] = (u64)~key << 32 | (unsigned)index;
+    if (at < kRoom) sh.list[at] = (u64)~key << 32 | (unsigned)index;
   };
 
   if (use_k && k <= kList) {  // at least k logits lie in the bins down to that of the k-th largest thread maximum
@@ -560,9 +577,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     sync();  // sh.listed and the lists may be used again
   }
 
-  unsigned weighed_cut = 0;  // the cut of top-p, when `weighed` holds this thread's weights above bin d1
-  u64 weighed = 0;
-  int d1 = 0, d2 = 0;  // the bins that hold a cut
+  unsigned weighed_cut = 0;  // the cut of top-p, when `weighed` holds this thread's weights
+  u64 weighed = 0;           // above weighed_high; the logits in question are those from there down
+  float weighed_high = 0.f;
+  bool listed = false;       // sh.list holds this block's logits in question
   unsigned k_cut = 0;  // top-k keeps keys above, and k_ties equal ones
   u64 k_ties = 0;
   for (int stage = 0; stage < 2; ++stage) {  // 0: top-k; 1: top-p among what top-k left
@@ -572,75 +590,83 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
     const float lowest = stage == 0 || k_cut == 0 || next <= low ? low : next;
     auto takes_part = [&](float l) { return l >= lowest; };
     if (tid == 0) sh.listed = 0;
+    listed = false;
     for_each([&](int, float l) {
       const int bin = bin_of(l);
       if (takes_part(l)) atomicAdd(&sh.hist[buffer][0][bin], 1u);
     });
     sync();
-    const u64 tied = stage == 1 && k_ties ? k_ties * weigh_one(weight, value_of<T>(k_cut)) : 0;
+    const u64 tied = stage == 1 && k_ties ? k_ties * weight(value_of<T>(k_cut)) : 0;
     const u64 counted = collect(false);
     const u64 counts = block_scan(counted, sh);
     int candidates = kList + 1;
-    u64 goal = 0, before = 0;
+    u64 goal = k, before = 0;
     if (tid == 0) sh.found_bin = kBins;
+    if (tid == kThreads - 1) sh.found_before = counts;
     __syncthreads();
-    if (stage == 0) {
-      goal = k;
-      if (counts >= goal && counts - counted < goal) sh.found_bin = tid, sh.found_before = counts - counted;
+    if (stage == 0 && sh.found_before < goal) {  // fewer than k have a weight: all stay
       __syncthreads();
-      d1 = d2 = sh.found_bin;
-      if (d1 == kBins) {  // fewer than k have a weight: all stay
-        __syncthreads();
-        continue;
-      }
-      before = sh.found_before;
-    } else {
-      const float centre = bins_per > 0.f ? top - (float)tid / bins_per : top;
-      const u64 about = counted ? counted * weigh_one(weight, fmaxf(centre, low)) : 0;
-      const u64 sum = block_scan(about, sh);
-      if (tid == kThreads - 1) sh.found_before = sum;
-      __syncthreads();
-      const u64 goal_about = share(sh.found_before + tied);
-      if (counted && sum >= goal_about && sum - about < goal_about) sh.found_bin = tid;
-      __syncthreads();
-      const int found = sh.found_bin;  // kBins: the cut seems to lie among the ties of top-k
-      d1 = found == kBins ? kBins : max(found - 1, 0);
-      d2 = found == kBins ? kBins : min(found + 1, kBins - 1);
-      if (tid == d2) sh.found_before = counts;
-      __syncthreads();
-      if (d2 < kBins && k_ties == 0) candidates = (int)min(sh.found_before, (u64)kList + 1);
+      continue;
     }
-    unsigned high, base;  // keys still in question
-    auto keys_of_bins = [&] {
-      high = key_of<T>(top), base = key_of<T>(low);
-      if (bins_per > 0.f) {
-        const float hi = edge_of(d1, -0.5f), lo = edge_of(d2, 0.5f);
-        if (hi < top) high = key_of<T>(hi);
-        if (lo > low && d2 < kBins - 1) base = key_of<T>(lo);
-        high = max(high, base);
-      }
-    };
-    keys_of_bins();
+    u64 about = counted, sum_about = counts, goal_about = goal;
+    if (stage == 1) {
+      const float centre = bins_per > 0.f ? top - (float)tid / bins_per : top;
+      about = counted ? counted * weight(fmaxf(centre, low)) : 0;
+      sum_about = block_scan(about, sh);
+      __syncthreads();
+      if (tid == kThreads - 1) sh.found_before = sum_about;
+      __syncthreads();
+      goal_about = share(sh.found_before + tied);
+    }
+    if (counted && sum_about >= goal_about && sum_about - about < goal_about) {
+      // near an edge of the bin, the neighbour too
+      const float part = stage == 0 ? 0.5f : (float)(goal_about - (sum_about - about)) / (float)about;
+      sh.found_bin = part < 0.05f ? max(tid - 1, 0) : tid;
+      sh.last_bin = part > 0.95f ? min(tid + 1, kBins - 1) : tid;
+    }
+    __syncthreads();
+    const int d1 = sh.found_bin, d2 = sh.last_bin;  // d1 == kBins: the cut seems to lie among the ties of top-k
+    if (d1 < kBins && tid == d2) sh.found_before = counts;
+    __syncthreads();
+    if (stage == 1 && d1 < kBins && k_ties == 0) candidates = (int)min(sh.found_before, (u64)kList + 1);
+    // the logits in question, whatever their bins: keys base .. high
+    unsigned high = key_of<T>(top), base = key_of<T>(low);
+    if (d1 == kBins) {
+      high = base, base = base + 1;  // none
+    } else if (bins_per > 0.f) {
+      const float hi = edge_of(d1, -0.5f), lo = edge_of(d2, 0.5f);
+      if (hi < top) high = key_of<T>(hi);
+      if (lo > low && d2 < kBins - 1) base = key_of<T>(lo);
+      high = max(high, base);
+    }
     bool gather = candidates <= kList;
-    bool all = false, weigh = stage == 1, reuse = true;  // all weights are added up once
+    bool all = false, weigh = true, reuse = stage == 1;  // weigh: add up all weights (counts), once
     for (int pass = 0;;) {
-      const unsigned span = high - base;  // bins of 2^shift keys
-      const int shift = span < kBins ? 0 : 32 - __clz(span) - 9;
+      const bool none = high < base;
+      const unsigned span = none ? 0 : high - base;  // bins of 2^shift keys
+      const int shift = span < kBins ? 0 : 32 - __clz(span) - kBinBits;
       u64 above = 0, total = 0;
+      const float high_value = none ? -inf : value_of<T>(high), base_value = none ? inf : value_of<T>(base);
+      const float reach_value = gather ? inf : high_value;
       auto count_key = [&](float l) {  // into the histogram of keys
         const unsigned key = key_of<T>(l);
-        if (pass > 0 && (key > high || key < base)) return;
-        const int at = key > high ? 0 : (int)((high - max(key, base)) >> shift);
+        if (key > high || key < base) return;
+        const int at = (int)((high - key) >> shift);
         if (stage == 0) {
           atomicAdd(&sh.hist[buffer][0][at], 1u);
         } else {
-          const u64 w = weigh_one(weight, l);
+          const u64 w = weight(l);
           atomicAdd(&sh.hist[buffer][0][at], (unsigned)w & 0xffffu);
           atomicAdd(&sh.hist[buffer][1][at], (unsigned)(w >> 16) & 0xffffu);
           atomicAdd(&sh.hist[buffer][2][at], (unsigned)(w >> 32));
         }
       };
-      if (weigh) {  // all weights are added up once
+      if (weigh && stage == 0) {
+        for_each([&](int i, float l) {
+          if (l > high_value) ++above;
+          else if (l >= base_value) append(key_of<T>(l), first + i);
+        });
+      } else if (weigh) {
         for_each_by_warp([&](int i, const float (&l)[kBatch]) {
           u64 w[kBatch];
 #pragma unroll
@@ -648,41 +674,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
           unsigned hits = 0;
 #pragma unroll
           for (int u = 0; u < kBatch; ++u) {
-            const int bin = bin_of(l[u]);
             const bool in = takes_part(l[u]);
             total += in ? w[u] : 0;
-            above += in && bin < d1 ? w[u] : 0;
-            hits |= in && bin <= d2 && (gather || bin >= d1) ? 1u << u : 0;
+            above += in && l[u] > high_value ? w[u] : 0;
+            hits |= in && l[u] >= base_value && l[u] <= reach_value ? 1u << u : 0;
           }
           while (hits) {
             const int u = __ffs(hits) - 1;
             hits &= hits - 1;
             const int at = i + 32 * u;
-            const float x = as_float(RESIDENT ? slice[at] : row[at]);
-            if (gather) append(key_of<T>(x), first + at);
-            if (bin_of(x) >= d1) count_key(x);
+            append(key_of<T>(as_float(RESIDENT ? slice[at] : row[at])), first + at);
           }
-        });
-      } else {
-        for_each([&](int, float l) {
-          const int bin = bin_of(l);
-          if (bin >= d1 && bin <= d2 && takes_part(l)) count_key(l);
         });
       }
       if (weigh) {  // the block's sums to every block
-        weighed = above;
+        weighed = above, weighed_high = high_value;
         const u64 block_above = block_scan(above, sh);
         __syncthreads();
         const u64 block_total = block_scan(total, sh);
         if (tid == kThreads - 1)
           for (int r = 0; r < C; ++r)
             *peer(&sh.block_above[rank], r) = block_above, *peer(&sh.block_total[rank], r) = block_total;
+        listed = sh.listed <= kRoom;
+      }
+      if (listed) {
+        for (int i = tid; i < sh.listed; i += kThreads) count_key(value_of<T>(~(unsigned)(sh.list[i] >> 32)));
+      } else {
+        for_each([&](int, float l) {
+          if (l >= base_value && l <= high_value && takes_part(l)) count_key(l);
+        });
       }
       sync();
       if (weigh) {
         u64 sum = tied;
         for (int r = 0; r < C; ++r) sum += sh.block_total[r], before += sh.block_above[r];
-        goal = share(sum);
+        if (stage == 1) goal = share(sum);
       }
       const u64 mine = collect(stage == 1);
       const u64 sum = before + block_scan(mine, sh);
@@ -691,14 +717,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
       const bool below = sh.found_before < goal, beside = before >= goal;
       __syncthreads();
       if (beside || below) {
-        all = below && d1 == kBins;  // among the ties of top-k
-        if (all || d2 - d1 == kBins - 1) {
+        const bool whole = high == key_of<T>(top) && base == key_of<T>(low);
+        if (whole || (below && d1 == kBins)) {  // among the ties of top-k
           all = true;
           break;
         }
-        d1 = 0, d2 = kBins - 1, before = 0;  // not in these bins: search all
-        keys_of_bins();
-        gather = weigh = reuse = false;
+        high = key_of<T>(top), base = key_of<T>(low), before = 0;  // not here: search all
+        gather = weigh = reuse = listed = false;
         continue;
       }
       weigh = false;
@@ -714,14 +739,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
       __syncthreads();
       before = sh.found_before;
       high -= (unsigned)sh.found_bin << shift;
-      if (shift == 0 || ++pass == 4) break;  // 9 bits a pass: shift is at most 23, 14, 5, 0
+      if (shift == 0 || ++pass == 4) break;  // at least 9 bits a pass: four are enough for 32
       base = max(base, high - ((1u << shift) - 1u));
     }
     if (all) before = sh.found_before;
     __syncthreads();
     const unsigned key = all ? k_cut : high;
-    const u64 unit = stage == 0 ? 1 : weigh_one(weight, value_of<T>(key));
-    u64 r = (goal - before + unit - 1) / max(unit, 1ull);
+    const u64 unit = stage == 0 ? 1 : weight(value_of<T>(key));
+    u64 r = quotient_up(goal - before, max(unit, 1ull));
     if (stage == 0) k_cut = key, k_ties = r;
     else if (all) r = min(r, k_ties);
     else if (reuse) weighed_cut = key;
@@ -735,13 +760,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
   unsigned tied = 0;
   if (cut == weighed_cut) {  // top-p has added up all weights but those of its bins
     above = weighed;
-    for_each_by_warp([&](int, const float (&l)[kBatch]) {
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        tied += l[u] == cut_value;
-        if (l[u] > cut_value && bin_of(l[u]) >= d1) above += weigh_one(weight, l[u]);
+    if (listed) {
+      if (tid < kWarps) sh.extra[tid] = 0, sh.extra_ties[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < sh.listed; i += kThreads) {
+        const float l = value_of<T>(~(unsigned)(sh.list[i] >> 32));
+        const int owner = (int)((unsigned)sh.list[i] - first) / N / per_warp;
+        if (l > cut_value && l <= weighed_high) atomicAdd(&sh.extra[owner], weight(l));
+        if (l == cut_value) atomicAdd(&sh.extra_ties[owner], 1u);
       }
-    });
+      __syncthreads();
+      if (lane == 0) above += sh.extra[warp], tied = sh.extra_ties[warp];
+    } else {
+      for_each_by_warp([&](int, const float (&l)[kBatch]) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          tied += l[u] == cut_value;
+          if (l[u] > cut_value && l[u] <= weighed_high) above += weight(l[u]);
+        }
+      });
+    }
   } else {
     for_each_by_warp([&](int, const float (&l)[kBatch]) {
       bool any = false;
@@ -767,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
   }
   sync();
   // each warp finds the range that holds the draw from all warps' sums, four per lane
-  const u64 unit = weigh_one(weight, cut_value);
+  const u64 unit = weight(cut_value);
   constexpr int E = (RESIDENT ? kMaxCluster : 2) * kWarps / 32;
   u64 w[E], t[E], weights = 0, tie_sum = 0;
 #pragma unroll
@@ -822,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
         for (int e = 0; e < N; ++e) {
           const float l = as_float(v.x[e]);
           mine += l == cut_value;
-          if (l > cut_value) heavy += weigh_one(weight, l);
+          if (l > cut_value) heavy += weight(l);
         }
       }
       unsigned tb = mine;
@@ -846,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float l = as_float(v.x[e]);
-          if (l > cut_value) at += weigh_one(weight, l);
+          if (l > cut_value) at += weight(l);
           else if (l == cut_value && tt++ < ties) at += unit;
           if (pick < 0 && at > goal) pick = e;
         }
@@ -860,21 +898,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleParams p)
   if (C > 1) cluster.sync();  // no block leaves while another reads its shared memory
 }
 
-template <typename T>
-cudaError_t launch(const SampleParams& p, int batch, int cluster, cudaStream_t st) {
-  if (cluster == 0) {
-    const cudaError_t e = cudaFuncSetAttribute(sample_rows<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kRaw * (int)sizeof(u64));
-    if (e != cudaSuccess) return e;
-    sample_rows<T, false><<<batch, kThreads, kRaw * sizeof(u64), st>>>(p);
-    return cudaGetLastError();
-  }
-  const int bytes = p.slice * (int)sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(sample_rows<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kMaxSlice * (int)sizeof(T));
+template <typename T, bool RESIDENT, int kThreads>
+cudaError_t launch(const SampleParams& p, int blocks, int cluster, int bytes, cudaStream_t st) {
+  const auto kernel = sample_rows<T, RESIDENT, kThreads>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             RESIDENT ? kMaxBytes : kRaw * (int)sizeof(u64));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)batch * cluster);
+  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -883,7 +914,36 @@ cudaError_t launch(const SampleParams& p, int batch, int cluster, cudaStream_t s
   attr.val.clusterDim.x = cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_rows<T, true>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T>
+cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
+  const int size = sizeof(T);
+  auto slice = [&](int n) { return (int)(((long long)p.vocab + n - 1) / n + 15) / 16 * 16; };
+  auto fits = [&](int n) { return slice(n) <= kMaxElements && slice(n) * size <= kMaxBytes; };
+  // Blocks per row: up to 8 that keep 2048 elements each and run at once with the other rows' (what fits of
+  // clusters of 2, 4 and 8: 148, 71 and 33 with two blocks of 512 threads on an SM, 74, 33 and 15 with one of 1024).
+  int cluster = 1, threads = 512;
+  while (cluster < kMaxCluster && p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 148 : cluster == 2 ? 71 : 33))
+    cluster *= 2;
+  if (slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
+    // Much work per block: 1024 threads. 64 rows of 128256 bf16 logits with top-p take 66 us on 2 x 1024 threads
+    // and 75 us on 4 x 512; one row with top-k takes 15.9 us on 8 x 1024 and 13.8 us on 8 x 512.
+    threads = 1024;
+    cluster = 1;
+    while (cluster < kMaxCluster &&
+           ((p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 74 : cluster == 2 ? 33 : 15)) ||
+            (!fits(cluster) && batch < 148)))
+      cluster *= 2;
+  }
+  if (!fits(cluster)) {  // from 148 rows on: one block per row reads it in every pass
+    p.slice = slice(1);
+    return launch<T, false, 512>(p, batch, 1, kRaw * sizeof(u64), st);
+  }
+  p.slice = slice(cluster);
+  if (threads == 1024) return launch<T, true, 1024>(p, batch * cluster, cluster, p.slice * size, st);
+  return launch<T, true, 512>(p, batch * cluster, cluster, p.slice * size, st);
 }
 
 }  // namespace
@@ -892,9 +952,7 @@ extern "C" int ek_sample(const EkSampleArgs* a, void* stream) {
   using ek::fail;
   if (!a) return fail(EK_E_INVALID, "NULL arguments");
   if (a->batch < 0 || a->vocab < 1) return fail(EK_E_INVALID, "bad sizes batch=%d vocab=%d", a->batch, a->vocab);
-  const int size = a->logits_f32 ? 4 : 2;
-  if (a->vocab > kMaxCluster * kMaxSlice)
-    return fail(EK_E_UNSUPPORTED, "vocab %d (at most %d)", a->vocab, kMaxCluster * kMaxSlice);
+  if (a->vocab > kMaxVocab) return fail(EK_E_UNSUPPORTED, "vocab %d (at most %d)", a->vocab, kMaxVocab);
   if (a->batch > (1 << 27)) return fail(EK_E_UNSUPPORTED, "batch %d", a->batch);
   if (a->batch == 0) return EK_SUCCESS;
   if (!a->logits || !a->uniforms || !a->tokens) return fail(EK_E_INVALID, "NULL pointer argument");
@@ -916,17 +974,8 @@ extern "C" int ek_sample(const EkSampleArgs* a, void* stream) {
   int bits = 62;
   for (long long n = 1; n < a->vocab; n *= 2) --bits;
   p.weight_bits = bits < 46 ? bits : 46;
-  // Blocks per row: up to 8 that keep 2048 elements each and run at once with the other rows' (two blocks fit an
-  // SM). A row that would not fit so few blocks is read in every pass by one block (0).
-  int cluster = 1;
-  while (cluster < kMaxCluster && a->vocab >= cluster * 4096 && (long long)a->batch * cluster * 2 <= 296) cluster *= 2;
-  if ((long long)a->vocab * size > cluster * (cluster == kMaxCluster ? (long long)kMaxSlice * size : 96 * 1024ll))
-    cluster = 0;
-  const int blocks = cluster ? cluster : 1;
-  p.slice = (int)(((long long)a->vocab + blocks - 1) / blocks + 15) / 16 * 16;
   ek::DeviceGuard g(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->logits_f32 ? launch<float>(p, a->batch, cluster, st)
-                                      : launch<__nv_bfloat16>(p, a->batch, cluster, st);
+  const cudaError_t e = a->logits_f32 ? launch<float>(p, a->batch, st) : launch<__nv_bfloat16>(p, a->batch, st);
   return e == cudaSuccess ? EK_SUCCESS : ek::cuda_fail(e, "ek_sample launch");
 }

@@ -29,7 +29,7 @@ from torch import Tensor
 from megakernels import ek
 
 _BF16 = torch.bfloat16
-MAX_VOCAB = 393216  # of sample_tokens
+MAX_VOCAB = 360448  # of sample_tokens
 
 
 def _need(t, name: str, dtype, ndim: int | None = None, like: Tensor | None = None) -> Tensor:
