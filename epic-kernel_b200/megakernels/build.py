@@ -1,4 +1,4 @@
-"""Build libek.so in-tree for sm_100a (nvcc, no JIT cache).
+"""Build libek.so and the tensor binding _ekops.so in-tree for sm_100a (nvcc, no JIT cache).
 
     python -m megakernels.build [--force]
 
@@ -15,6 +15,7 @@ from pathlib import Path
 PKG_ROOT = Path(__file__).resolve().parent.parent
 CSRC = PKG_ROOT / "csrc"
 OUT = PKG_ROOT / "libek.so"
+BINDING = PKG_ROOT / "_ekops.so"  # ek_torch.cpp
 # ek_decode.cu is compiled once per kernel variant (model x prefetch paths),
 # so that each kernel carries only the code its model runs.
 VARIANTS = [
@@ -37,11 +38,35 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found")
 
 
+def gxx_path() -> str:
+    for cand in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")):
+        if cand:
+            return cand
+    raise RuntimeError("g++ not found")
+
+
+def binding_command(out: Path) -> list[str]:
+    """Compiles the tensor binding against torch's headers. It is linked against the torch libraries that the
+    process has loaded by then."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(cuda / "include")]
+    lib = Path(torch.__file__).parent / "lib"
+    return [gxx_path(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-I{i}" for i in include), "-o", str(out), str(CSRC / "ek_torch.cpp"),
+            f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+
+
 def stale() -> bool:
-    if not OUT.exists():
+    if not OUT.exists() or not BINDING.exists():
         return True
-    t = OUT.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h"))
+    t = min(OUT.stat().st_mtime, BINDING.stat().st_mtime)
+    deps = [f for kind in ("*.cu", "*.cuh", "*.h", "*.cpp") for f in CSRC.glob(kind)]
     deps.append(PKG_ROOT.parent / "include" / "ek.h")
     return any(d.stat().st_mtime > t for d in deps if d.exists())
 
@@ -67,8 +92,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, cwd=PKG_ROOT)
 
+    binding = BINDING.with_suffix(".so.tmp")
+    jobs.append(binding_command(binding))
     with ThreadPoolExecutor(max_workers=len(jobs)) as ex:
         list(ex.map(run, jobs))
+    binding.replace(BINDING)
     tmp = OUT.with_suffix(".so.tmp")
     objs = [str(objdir / f"ek_decode_{n}.o") for n, _ in VARIANTS] + [str(objdir / f"{n}.o") for n in SOURCES]
     run([nvcc, *LINK_FLAGS, "-o", str(tmp), *objs])

@@ -98,46 +98,6 @@ class EkMixtralArgs(ctypes.Structure):
     ]
 
 
-_L = ctypes.c_int64
-_F = ctypes.c_float
-
-
-class EkKvTensor(ctypes.Structure):
-    _fields_ = [
-        ("data", _P), ("scales", _P),
-        ("stride_batch", _L), ("stride_row", _L), ("stride_head", _L),
-        ("scale_stride_batch", _L), ("scale_stride_row", _L), ("scale_stride_head", _L),
-    ]
-
-
-class EkKvCopyArgs(ctypes.Structure):
-    _fields_ = [
-        ("k_values", EkKvTensor), ("v_values", EkKvTensor), ("k_cache", EkKvTensor), ("v_cache", EkKvTensor),
-        ("start", _P), ("start_all", _L),
-        ("batch", _I), ("length", _I), ("capacity", _I), ("kv_heads", _I), ("head_dim", _I), ("device", _I),
-    ]
-
-
-class EkPrefixAttnArgs(ctypes.Structure):
-    _fields_ = [
-        ("q", _P), ("q_stride_batch", _L), ("q_stride_head", _L),
-        ("prefix_k", EkKvTensor), ("prefix_v", EkKvTensor), ("own_k", EkKvTensor), ("own_v", EkKvTensor),
-        ("own_lens", _P), ("out", _P), ("out_stride_batch", _L), ("out_stride_head", _L), ("lse", _P),
-        ("workspace", _P), ("workspace_bytes", _L),
-        ("batch", _I), ("q_heads", _I), ("kv_heads", _I), ("head_dim", _I),
-        ("prefix_len", _I), ("own_capacity", _I), ("max_own_len", _I), ("scale", _F), ("device", _I),
-    ]
-
-
-class EkSampleArgs(ctypes.Structure):
-    _fields_ = [
-        ("logits", _P), ("row_stride", _L), ("uniforms", _P),
-        ("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P), ("tokens", _P),
-        ("temperature_all", _F), ("top_p_all", _F), ("min_p_all", _F), ("top_k_all", _I),
-        ("logits_f32", _I), ("batch", _I), ("vocab", _I), ("device", _I),
-    ]
-
-
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -164,16 +124,24 @@ def load_library(path: Path | str | None = None) -> ctypes.CDLL:
         lib.ek_tp_setup.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                     ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]
         lib.ek_tp_connect.argtypes = [ctypes.c_void_p, ctypes.c_char_p]
-        for name, args in (("ek_kv_write", EkKvCopyArgs), ("ek_kv_read", EkKvCopyArgs),
-                           ("ek_prefix_attention", EkPrefixAttnArgs), ("ek_sample", EkSampleArgs)):
-            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
-        lib.ek_prefix_attention_workspace.argtypes = [ctypes.POINTER(EkPrefixAttnArgs)]
         lib.ek_prefix_attention_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int32), ctypes.c_int]
-        lib.ek_prefix_attention_workspace.restype = ctypes.c_int64
         if lib.ek_abi_version() != EK_ABI_VERSION:
             raise RuntimeError(f"{p}: ABI {lib.ek_abi_version()} != expected {EK_ABI_VERSION}")
         _lib = lib
         return lib
+
+
+def load_extension(name: str):
+    """Import the compiled module `name` from the directory that holds libek.so's Python modules."""
+    import importlib.util
+
+    path = PKG_ROOT / f"{name}.so"
+    if not path.exists():
+        raise RuntimeError(f"{path} not found: build the CUDA engine first (python -m megakernels.build)")
+    spec = importlib.util.spec_from_file_location(name, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def check(rc: int, what: str):
