@@ -345,8 +345,11 @@ struct Many {
   static constexpr int RAW = 128 * D;                 // bytes of an 8-bit tile
   static constexpr int STAGES = I8 ? (D == 128 ? 3 : 4) : (D == 128 ? 5 : 8);
   static constexpr int RAW_STAGES = I8 ? (D == 128 ? 3 : 6) : 0;
-  static constexpr int WARPS = I8 ? 14 : 10;          // 8 softmax, [4 widening,] loads, products
-  static constexpr int LOADER = WARPS - 2, MMA = WARPS - 1;
+  static constexpr int WARPS = I8 ? 16 : 12;          // 8 softmax, [4 widening,] loads, products, 2 idle
+  static constexpr int LOADER = WARPS - 4, MMA = WARPS - 3;
+  // registers per thread: at launch, of the softmax, widening and other warpgroups
+  static constexpr int REGS = I8 ? 128 : 168, SOFTMAX_REGS = I8 ? 200 : 208, WIDEN_REGS = 72, OTHER_REGS = I8 ? 40 : 88;
+  static_assert(2 * SOFTMAX_REGS + (I8 ? WIDEN_REGS : 0) + OTHER_REGS == WARPS / 4 * REGS, "registers of the block");
   static constexpr int OFF_STAGE = 2 * TILE;          // after two Q tiles
   static constexpr int OFF_RAW = OFF_STAGE + STAGES * TILE;
   static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;
@@ -365,6 +368,9 @@ struct ManyParams {
   int negate;                   // scale < 0: q is negated and |scale| used
 };
 
+// Pairs out of every eight whose exponentials are taken by exp2_cubic.
+constexpr int CUBIC = 0;
+
 __device__ int g_attention_status;
 
 // Columns from `keys` on of 32 scores become -inf.
@@ -372,6 +378,26 @@ __device__ __forceinline__ void mask_tail(uint32_t (&x)[32], int keys) {
 #pragma unroll
   for (int e = 0; e < 32; ++e)
     if (e >= keys) x[e] = 0xff800000u;
+}
+
+__device__ __forceinline__ uint64_t score_pair(const uint32_t (&x)[32], int e) {
+  return ek::pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+}
+
+// 2^x of a pair without the exponential unit: x = n + r, |r| <= 1/2, 2^r by a cubic that is fitted at the Chebyshev
+// nodes of the interval (relative error below 1.1e-4, a fortieth of the rounding of P to bf16) and n added to the
+// exponent. x below -126 counts as -126.
+__device__ __forceinline__ float2 exp2_cubic(float2 x) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+  const uint64_t t = ek::pair(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const uint64_t z = ek::add2(t, ek::pair(kRound, kRound));
+  const uint64_t r = ek::add2(t, ek::mul2(ek::add2(z, ek::pair(-kRound, -kRound)), ek::pair(-1.f, -1.f)));
+  uint64_t p = ek::fma2(ek::pair(0.0558382829f, 0.0558382829f), r, ek::pair(0.242639479f, 0.242639479f));
+  p = ek::fma2(p, r, ek::pair(0.693136734f, 0.693136734f));
+  p = ek::fma2(p, r, ek::pair(0.999924557f, 0.999924557f));
+  const float2 pf = ek::unpair(p), zf = ek::unpair(z);
+  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(zf.x) << 23)),
+                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(zf.y) << 23)));
 }
 
 template <int D, bool I8>
@@ -389,7 +415,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   uint64_t* drained = o_full + 2;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_at + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0);  // uniform
 
   // the item
   int id = blockIdx.x;
@@ -436,130 +462,12 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   // Ring order of the tiles: K_0 .. K_{lead-1}, then V_i, K_{i+lead} in turn, then the last V.
   const int items = 2 * tiles;
   const int lead_now = min(lead, tiles);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // for a whole warp, which goes on or gives up together
+    return __all_sync(~0u, ek::mbar_wait_bounded(bar, parity, abort)) != 0;
+  };
 
-  if (warp == C::LOADER) {
-    if (lane == 0) {
-      constexpr int N = I8 ? C::RAW_STAGES : C::STAGES;
-      uint64_t* f = I8 ? raw_full : full;
-      uint64_t* e = I8 ? raw_empty : empty;
-      uint8_t* base = smem + (I8 ? C::OFF_RAW : C::OFF_STAGE);
-      constexpr int BYTES = I8 ? C::RAW : C::TILE;
-      int n = 0;
-      for (; n < items; ++n) {
-        const int s = n % N;
-        if (n >= N && !ek::mbar_wait_bounded(e + s, (n / N - 1) & 1, abort)) break;
-        bool is_v;
-        int tile;
-        if (n < lead_now) is_v = false, tile = n;
-        else {
-          const int m = n - lead_now, both = 2 * (tiles - lead_now);
-          is_v = m >= both || m % 2 == 0;
-          tile = m >= both ? m - (tiles - lead_now) : m / 2 + (is_v ? 0 : lead_now);
-        }
-        const int key = (tile0 + tile) * 128;
-        const CUtensorMap* map = is_v ? &p.v : &p.k;
-        const bool keys_first = is_v ? p.v_keys_first : p.k_keys_first;
-        ek::mbar_arrive_expect_tx(f + s, BYTES);
-        for (int blk = 0; blk < (I8 ? 1 : C::BLOCKS); ++blk)
-          ek::tma_load_3d(base + s * BYTES + blk * 16384, map, blk * 64, keys_first ? key : head,
-                          keys_first ? head : key, f + s);
-      }
-      if (n < items) {  // gave up: let the copies in flight land
-        int quiet = 0;
-        for (int i = max(0, n - N); i < n; ++i) ek::mbar_wait_bounded(f + i % N, (i / N) & 1, &quiet);
-      }
-    }
-  } else if (warp == C::MMA) {
-    if (lane == 0) {
-      constexpr uint32_t SD = ek::mma_desc(128, 128, false), OD = ek::mma_desc(128, D, true);
-      const uint32_t stage = ek::smem_u32(smem + C::OFF_STAGE);
-      int n = 0;  // ring position
-      auto scores = [&](int w, uint32_t k) {
-        const uint32_t q = ek::smem_u32(smem) + (wide ? w * C::TILE : 0);
-#pragma unroll
-        for (int kt = 0; kt < D / 16; ++kt) {
-          const uint32_t off = kt / 4 * 16384 + kt % 4 * 32;
-          ek::mma_ss(tmem + w * 128, ek::smem_desc(q + off, 16), ek::smem_desc(k + off, 16), SD, kt > 0);
-        }
-        ek::mma_commit(s_full + w);
-      };
-      auto values = [&](int w, uint32_t v, bool add) {
-#pragma unroll
-        for (int kt = 0; kt < 8; ++kt)
-          ek::mma_ts(tmem + 256 + w * D, tmem + w * 128 + kt * 8, ek::smem_desc(v + kt * 2048, 16384), OD, add || kt > 0);
-      };
-      auto wait_stage = [&](int i) { return ek::mbar_wait_bounded(full + i % C::STAGES, (i / C::STAGES) & 1, abort); };
-      bool ok = true;
-      for (int i = 0; ok && i < lead_now; ++i) {  // first scores
-        if (!(ok = wait_stage(n))) break;
-        ek::tcgen05_after_sync();
-        const uint32_t k = stage + n % C::STAGES * C::TILE;
-        if (wide) scores(0, k), scores(1, k);
-        else scores(i, k);
-        ek::mma_commit(empty + n % C::STAGES);
-        ++n;
-      }
-      for (int i = 0; ok && i < tiles; ++i) {
-        const bool more = i + lead_now < tiles;
-        const int nv = n, nk = n + 1;
-        n += more ? 2 : 1;
-        for (int turn = 0; turn < (wide ? 2 : 1); ++turn) {
-          const int w = wide ? turn : i % 2, use = wide ? i : i / 2;
-          if (turn == 0 && !(ok = wait_stage(nv))) break;
-          if (!(ok = ek::mbar_wait_bounded(p_full + w, use & 1, abort))) break;
-          ek::tcgen05_after_sync();
-          values(w, stage + nv % C::STAGES * C::TILE, use > 0);
-          const bool last_turn = !wide || turn == 1;
-          if (last_turn) ek::mma_commit(empty + nv % C::STAGES);
-          if (more) {
-            if (turn == 0 && !(ok = wait_stage(nk))) break;
-            ek::tcgen05_after_sync();
-            scores(w, stage + nk % C::STAGES * C::TILE);
-            if (last_turn) ek::mma_commit(empty + nk % C::STAGES);
-          }
-          if (i + (wide ? 1 : 2) >= tiles) ek::mma_commit(o_full + w);
-        }
-      }
-      // tensor memory is freed below: nothing may be in flight
-      int quiet = 0;
-      ek::mma_commit(drained);
-      ek::mbar_wait_bounded(drained, 0, &quiet);
-    }
-  } else if (I8 && warp >= 8) {
-    const int t = threadIdx.x - 256;
-    for (int n = 0; n < items; ++n) {
-      const int rs = n % (I8 ? C::RAW_STAGES : 1), cs = n % C::STAGES;
-      if (!ek::mbar_wait_bounded(raw_full + rs, (n / (I8 ? C::RAW_STAGES : 1)) & 1, abort)) break;
-      if (n >= C::STAGES && !ek::mbar_wait_bounded(empty + cs, (n / C::STAGES - 1) & 1, abort)) break;
-      const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW;
-      uint8_t* to = smem + C::OFF_STAGE + cs * C::TILE;
-#pragma unroll 4
-      for (int i = t; i < 128 * D / 16; i += 128) {
-        const int r = i / (D / 16), piece = i % (D / 16);
-        const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 16);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t y[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[2 * e] = codes_to_bf16(__byte_perm(w[e], w[e], 0x1100));
-          y[2 * e + 1] = codes_to_bf16(__byte_perm(w[e], w[e], 0x3322));
-        }
-        // two 16-byte pieces of the 128-byte row; the second block writes them in the other order, so
-        // that the eight lanes of a row hit different banks
-        uint8_t* row = to + piece / 4 * 16384 + r * 128;
-        const int c0 = piece % 4 * 2, flip = D == 128 ? piece / 4 : 0;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool hi = (e ^ flip) & 1;
-          *reinterpret_cast<uint4*>(row + (((c0 + (hi ? 1 : 0)) ^ (r & 7)) << 4)) =
-              hi ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
-        }
-      }
-      ek::fence_proxy_async_smem();
-      ek::mbar_arrive(full + cs);
-      ek::mbar_arrive(raw_empty + rs);
-    }
-  } else if (warp < 8) {
+  if (warp < 8) {
+    ek::registers_up<C::SOFTMAX_REGS>();
     const int w = warp / 4, t = threadIdx.x % 128;
     const int row = row0 + (wide ? w * 128 : 0) + t;
     const bool idle = row0 + (wide ? w * 128 : 0) + (warp % 4) * 32 >= row1;  // no row in this warp
@@ -590,73 +498,89 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         ks = sc, vs = sc + 128;
         next_ks = key_scale(use + 1, 0), next_vs = key_scale(use + 1, 1);
       }
-      if (!(ok = ek::mbar_wait_bounded(s_full + w, use & 1, abort))) break;
+      if (!(ok = wait(s_full + w, use & 1))) break;
       ek::tcgen05_after_sync();
       if (!idle) {
-        // row maximum, in units of scale (base 2)
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint32_t r[2][32];
-        ek::tmem_ld32(r[0], ts);
+        uint32_t x[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ek::tmem_ld32(x[c], ts + c * 32);
+        ek::tmem_wait_ld(x[0]);
+#pragma unroll
+        for (int c = 1; c < 4; ++c) ek::tmem_after(x[c]);
+        if (I8) {  // scores in units of base 2
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(ks + c * 32 + e);
+              const float2 a = ek::unpair(ek::mul2(score_pair(x[c], e), ek::pair(f.x, f.y)));
+              const float2 b = ek::unpair(ek::mul2(score_pair(x[c], e + 2), ek::pair(f.z, f.w)));
+              x[c][e] = __float_as_uint(a.x), x[c][e + 1] = __float_as_uint(a.y);
+              x[c][e + 2] = __float_as_uint(b.x), x[c][e + 3] = __float_as_uint(b.y);
+            }
+        }
+        if (keys < 128) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask_tail(x[c], keys - c * 32);
+        }
+        float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t(&x)[32] = r[c & 1];
-          ek::tmem_wait_ld(x);
-          if (c < 3) ek::tmem_ld32(r[(c + 1) & 1], ts + (c + 1) * 32);
-          if (keys < 128) mask_tail(x, keys - c * 32);
+          top[c] = __uint_as_float(x[c][0]);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float v = __uint_as_float(x[e]);
-            top[e & 3] = fmaxf(top[e & 3], I8 ? v * ks[c * 32 + e] : v);
-          }
+          for (int e = 1; e < 31; e += 2) top[c] = ek::max3_nan(top[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+          top[c] = ek::max3_nan(top[c], __uint_as_float(x[c][31]), top[c]);
         }
-        float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (!I8) high *= scale;
-        ek::tmem_ld32(r[0], ts);
-        const float grown = fmaxf(m, high);
+        const float high = ek::max3_nan(ek::max3_nan(top[0], top[1], top[2]), top[3], top[3]) * (I8 ? 1.f : scale);
+        const float grown = ek::max3_nan(m, high, high);
         if (use == 0) m = grown;
-        const float fix = grown - m > 8.f ? exp2_approx(m - grown) : 1.f;  // false for NaN
-        if (__any_sync(~0u, fix != 1.f)) {
-          ek::tmem_wait_ld(r[0]);
-          if (fix != 1.f) m = grown, l *= fix;
+        const bool far = grown > m + 8.f || grown != grown;
+        if (__any_sync(~0u, far)) {
+          const float fix = far ? exp2_approx(m - grown) : 1.f;
+          if (far) m = grown, l *= fix;
+          if (use > 0) {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            ek::tmem_ld32(r[1], to + c * 32);
-            ek::tmem_wait_ld(r[1]);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              ek::tmem_ld16(o, to + c * 16);
+              ek::tmem_wait_ld(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[1][e] = __float_as_uint(__uint_as_float(r[1][e]) * fix);
-            ek::tmem_st32(to + c * 32, r[1]);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fix);
+              ek::tmem_st16(to + c * 16, o);
+            }
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t slope = ek::pair(scale, scale), shift = ek::pair(-base, -base);
+        uint64_t sums[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t(&x)[32] = r[c & 1];
-          ek::tmem_wait_ld(x);
-          if (c < 3) ek::tmem_ld32(r[(c + 1) & 1], ts + (c + 1) * 32);
-          if (keys < 128) mask_tail(x, keys - c * 32);
           uint32_t out[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float pr[2];
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-              const float v = __uint_as_float(x[e + f]);
-              pr[f] = exp2_approx(fmaf(v, I8 ? ks[c * 32 + e + f] : scale, -base));
-              sum[(e + f) & 3] += pr[f];
-              if (I8) pr[f] *= vs[c * 32 + e + f];
+            const uint64_t s2 = score_pair(x[c], e);
+            const float2 t2 = ek::unpair(I8 ? ek::add2(s2, shift) : ek::fma2(s2, slope, shift));
+            float2 pr;
+            if (e % 16 >= 16 - 2 * CUBIC) pr = exp2_cubic(t2);
+            else pr = make_float2(exp2_approx(t2.x), exp2_approx(t2.y));
+            uint64_t p2 = ek::pair(pr.x, pr.y);
+            sums[e / 2 & 1] = ek::add2(sums[e / 2 & 1], p2);
+            if (I8) {
+              const float2 f = *reinterpret_cast<const float2*>(vs + c * 32 + e);
+              pr = ek::unpair(ek::mul2(p2, ek::pair(f.x, f.y)));
             }
-            out[e / 2] = pack_bf16(pr[0], pr[1]);
+            out[e / 2] = pack_bf16(pr.x, pr.y);
           }
           ek::tmem_st16(ts + c * 16, out);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 sum2 = ek::unpair(ek::add2(sums[0], sums[1]));
+        l += sum2.x + sum2.y;
         ek::tmem_wait_st();
       }
       ek::tcgen05_before_sync();
       ek::mbar_arrive(p_full + w);
     }
-    if (ok && mine > 0) ok = ek::mbar_wait_bounded(o_full + w, 0, abort);
+    if (ok && mine > 0) ok = wait(o_full + w, 0);
     ek::tcgen05_after_sync();
     if (!ok) m = NAN, l = NAN;  // a wait ran out: the result is NaN and the status is set
     if (!idle) {
@@ -679,6 +603,141 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
       }
     }
     ek::tcgen05_before_sync();
+  } else if (I8 && warp < C::LOADER) {
+    ek::registers_down<C::WIDEN_REGS>();
+    const int t = threadIdx.x - 256;
+    for (int n = 0; n < items; ++n) {
+      const int rs = n % (I8 ? C::RAW_STAGES : 1), cs = n % C::STAGES;
+      if (!wait(raw_full + rs, (n / (I8 ? C::RAW_STAGES : 1)) & 1)) break;
+      if (n >= C::STAGES && !wait(empty + cs, (n / C::STAGES - 1) & 1)) break;
+      const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW;
+      uint8_t* to = smem + C::OFF_STAGE + cs * C::TILE;
+#pragma unroll 4
+      for (int i = t; i < 128 * D / 16; i += 128) {
+        const int r = i / (D / 16), piece = i % (D / 16);
+        const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 16);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = codes_to_bf16(__byte_perm(w[e], w[e], 0x1100));
+          y[2 * e + 1] = codes_to_bf16(__byte_perm(w[e], w[e], 0x3322));
+        }
+        // two 16-byte pieces of the 128-byte row; the second block writes them in the other order, so
+        // that the eight lanes of a row hit different banks
+        uint8_t* row = to + piece / 4 * 16384 + r * 128;
+        const int c0 = piece % 4 * 2, flip = D == 128 ? piece / 4 : 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool hi = (e ^ flip) & 1;
+          *reinterpret_cast<uint4*>(row + (((c0 + (hi ? 1 : 0)) ^ (r & 7)) << 4)) =
+              hi ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+      ek::fence_proxy_async_smem();
+      ek::mbar_arrive(full + cs);
+      ek::mbar_arrive(raw_empty + rs);
+    }
+  } else {
+    ek::registers_down<C::OTHER_REGS>();
+    if (warp == C::LOADER) {
+      constexpr int N = I8 ? C::RAW_STAGES : C::STAGES;
+      uint64_t* f = I8 ? raw_full : full;
+      uint64_t* e = I8 ? raw_empty : empty;
+      uint8_t* base = smem + (I8 ? C::OFF_RAW : C::OFF_STAGE);
+      constexpr int BYTES = I8 ? C::RAW : C::TILE;
+      int n = 0;
+      for (; n < items; ++n) {
+        const int s = n % N;
+        if (n >= N && !wait(e + s, (n / N - 1) & 1)) break;
+        bool is_v;
+        int tile;
+        if (n < lead_now) is_v = false, tile = n;
+        else {
+          const int m = n - lead_now, both = 2 * (tiles - lead_now);
+          is_v = m >= both || m % 2 == 0;
+          tile = m >= both ? m - (tiles - lead_now) : m / 2 + (is_v ? 0 : lead_now);
+        }
+        const int key = (tile0 + tile) * 128;
+        const CUtensorMap* map = is_v ? &p.v : &p.k;
+        const bool keys_first = is_v ? p.v_keys_first : p.k_keys_first;
+        if (ek::elect_one()) {
+          ek::mbar_arrive_expect_tx(f + s, BYTES);
+          for (int blk = 0; blk < (I8 ? 1 : C::BLOCKS); ++blk)
+            ek::tma_load_3d(base + s * BYTES + blk * 16384, map, blk * 64, keys_first ? key : head,
+                            keys_first ? head : key, f + s);
+        }
+        __syncwarp();
+      }
+      if (n < items) {  // gave up: let the copies in flight land
+        int quiet = 0;
+        for (int i = max(0, n - N); i < n; ++i) ek::mbar_wait_bounded(f + i % N, (i / N) & 1, &quiet);
+      }
+    } else if (warp == C::MMA) {
+      constexpr uint32_t SD = ek::mma_desc(128, 128, false), OD = ek::mma_desc(128, D, true);
+      const uint32_t stage = ek::smem_u32(smem + C::OFF_STAGE);
+      int n = 0;  // ring position
+      auto scores = [&](int w, uint32_t k) {
+        const uint32_t q = ek::smem_u32(smem) + (wide ? w * C::TILE : 0);
+#pragma unroll
+        for (int kt = 0; kt < D / 16; ++kt) {
+          const uint32_t off = kt / 4 * 16384 + kt % 4 * 32;
+          ek::mma_ss(tmem + w * 128, ek::smem_desc(q + off, 16), ek::smem_desc(k + off, 16), SD, kt > 0);
+        }
+        ek::mma_commit(s_full + w);
+      };
+      auto values = [&](int w, uint32_t v, bool add) {
+#pragma unroll
+        for (int kt = 0; kt < 8; ++kt)
+          ek::mma_ts(tmem + 256 + w * D, tmem + w * 128 + kt * 8, ek::smem_desc(v + kt * 2048, 16384), OD, add || kt > 0);
+      };
+      auto wait_stage = [&](int i) { return wait(full + i % C::STAGES, (i / C::STAGES) & 1); };
+      bool ok = true;
+      for (int i = 0; ok && i < lead_now; ++i) {  // first scores
+        if (!(ok = wait_stage(n))) break;
+        ek::tcgen05_after_sync();
+        const uint32_t k = stage + n % C::STAGES * C::TILE;
+        if (ek::elect_one()) {
+          if (wide) scores(0, k), scores(1, k);
+          else scores(i, k);
+          ek::mma_commit(empty + n % C::STAGES);
+        }
+        __syncwarp();
+        ++n;
+      }
+      for (int i = 0; ok && i < tiles; ++i) {
+        const bool more = i + lead_now < tiles;
+        const int nv = n, nk = n + 1;
+        n += more ? 2 : 1;
+        for (int turn = 0; turn < (wide ? 2 : 1); ++turn) {
+          const int w = wide ? turn : i % 2, use = wide ? i : i / 2;
+          const bool last_turn = !wide || turn == 1;
+          if (turn == 0 && !(ok = wait_stage(nv))) break;
+          if (!(ok = wait(p_full + w, use & 1))) break;
+          ek::tcgen05_after_sync();
+          if (ek::elect_one()) {
+            values(w, stage + nv % C::STAGES * C::TILE, use > 0);
+            if (last_turn) ek::mma_commit(empty + nv % C::STAGES);
+            if (i + (wide ? 1 : 2) >= tiles) ek::mma_commit(o_full + w);
+          }
+          __syncwarp();
+          if (more) {
+            if (turn == 0 && !(ok = wait_stage(nk))) break;
+            ek::tcgen05_after_sync();
+            if (ek::elect_one()) {
+              scores(w, stage + nk % C::STAGES * C::TILE);
+              if (last_turn) ek::mma_commit(empty + nk % C::STAGES);
+            }
+            __syncwarp();
+          }
+        }
+      }
+      // tensor memory is freed below: nothing may be in flight
+      int quiet = 0;
+      if (ek::elect_one()) ek::mma_commit(drained);
+      __syncwarp();
+      ek::mbar_wait_bounded(drained, 0, &quiet);
+    }
   }
   __syncwarp();
   __syncthreads();
@@ -823,9 +882,13 @@ int encode_prefix(CUtensorMap* m, const EkKvTensor& t, int keys, int heads, int 
 template <int D, bool I8>
 cudaError_t launch_many(const ManyParams& p, cudaStream_t st) {
   static_assert(Many<D, I8>::SMEM <= 227 * 1024, "shared memory");
-  const cudaError_t e =
+  cudaError_t e =
       cudaFuncSetAttribute(many_rows<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<D, I8>::SMEM);
   if (e != cudaSuccess) return e;
+  // the warpgroups take more registers out of those that the block is launched with
+  cudaFuncAttributes attr;
+  if ((e = cudaFuncGetAttributes(&attr, many_rows<D, I8>)) != cudaSuccess) return e;
+  if (attr.numRegs != Many<D, I8>::REGS) return cudaErrorLaunchOutOfResources;
   const int items = (p.wide_blocks * p.wide_splits + (p.narrow_rows ? p.narrow_splits : 0)) * p.a.kv_heads;
   many_rows<D, I8><<<items, Many<D, I8>::WARPS * 32, Many<D, I8>::SMEM, st>>>(p);
   return cudaGetLastError();
