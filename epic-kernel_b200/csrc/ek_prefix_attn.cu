@@ -321,9 +321,11 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows(const AttnParams p) {
 //
 // One block takes one KV head, up to 256 query rows and a range of keys, in
 // tiles of 128 keys. S = Q K^T (128 x 128 fp32) and O += P V (128 x D) stay in
-// tensor memory; P goes back over S as bf16 and is read from there as the A
-// operand. Two softmax warpgroups work in turn with the tensor core: while one
-// takes exponentials, the products of the other run. With more than 128 rows
+// tensor memory; P goes there as bf16 and is read as the A operand. Two softmax
+// warpgroups work in turn with the tensor core. They take S into registers at
+// once, so that one S buffer serves both: the next scores are computed while
+// exponentials are taken, and no warpgroup waits for the products of its own
+// tile. With more than 128 rows
 // the warpgroups hold two row tiles and share every K and V tile ("wide");
 // with fewer they hold the same rows and take alternate key tiles, each with a
 // running maximum, sum and O of its own ("narrow"). A thread owns one row, so
@@ -345,8 +347,8 @@ struct Many {
   static constexpr int RAW = 128 * D;                 // bytes of an 8-bit tile
   static constexpr int STAGES = I8 ? (D == 128 ? 3 : 4) : (D == 128 ? 5 : 8);
   static constexpr int RAW_STAGES = I8 ? (D == 128 ? 3 : 6) : 0;
-  static constexpr int WARPS = I8 ? 16 : 12;          // 8 softmax, [4 widening,] loads, products, 2 idle
-  static constexpr int LOADER = WARPS - 4, MMA = WARPS - 3;
+  static constexpr int WARPS = I8 ? 16 : 12;          // 8 softmax, [4 widening,] loads, scores, values, 1 idle
+  static constexpr int LOADER = WARPS - 4, SCORES = WARPS - 3, VALUES = WARPS - 2;
   // registers per thread: at launch, of the softmax, widening and other warpgroups
   static constexpr int REGS = I8 ? 128 : 168, SOFTMAX_REGS = I8 ? 200 : 208, WIDEN_REGS = 72, OTHER_REGS = I8 ? 40 : 88;
   static_assert(2 * SOFTMAX_REGS + (I8 ? WIDEN_REGS : 0) + OTHER_REGS == WARPS / 4 * REGS, "registers of the block");
@@ -355,7 +357,8 @@ struct Many {
   static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;
   static constexpr int SCALE_BYTES = I8 ? 2 * 2 * 2 * 128 * 4 : 0;  // warpgroup, parity, k / v, key
   static constexpr int OFF_BAR = OFF_SCALE + SCALE_BYTES;
-  static constexpr int BARS = 2 * STAGES + 2 * RAW_STAGES + 6 + 1;
+  static constexpr int BARS = 2 * STAGES + 2 * RAW_STAGES + 6 + 2;
+  static constexpr int S = 0, P = 128, O = 256;       // columns of tensor memory: scores, P and O of both warpgroups
   static constexpr int SMEM = OFF_BAR + BARS * 8 + 16 + 1024;  // + alignment
 };
 
@@ -411,8 +414,9 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   uint64_t* raw_empty = raw_full + C::RAW_STAGES;
   uint64_t* s_full = raw_empty + C::RAW_STAGES;
   uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
-  uint64_t* drained = o_full + 2;
+  uint64_t* p_empty = p_full + 2;   // the products with P are done
+  uint64_t* s_empty = p_empty + 2;  // the scores are in registers
+  uint64_t* drained = s_empty + 1;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_at + 1);
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0);  // uniform
@@ -430,14 +434,14 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   const int row1 = wide ? min(p.rows, row0 + 256) : p.rows;
   const int tile0 = split * per;
   const int tiles = min(per, (p.a.prefix_len + 127) / 128 - tile0);
-  const int lead = wide ? 1 : 2;  // K tiles in use before the first V tile
+  const int lead = wide ? 2 : 3;  // K tiles in use before the first V tile
 
-  if (warp == C::MMA) ek::tmem_alloc(tmem_at, 512);
+  if (warp == C::SCORES) ek::tmem_alloc(tmem_at, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) ek::mbar_init(full + i, I8 ? 128 : 1), ek::mbar_init(empty + i, 1);
     for (int i = 0; i < C::RAW_STAGES; ++i) ek::mbar_init(raw_full + i, 1), ek::mbar_init(raw_empty + i, 128);
-    for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 128), ek::mbar_init(o_full + i, 1);
-    ek::mbar_init(drained, 1);
+    for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 128), ek::mbar_init(p_empty + i, 1);
+    ek::mbar_init(s_empty, 128), ek::mbar_init(drained, 2);
     *abort = 0;
     ek::fence_mbar_init();
   }
@@ -462,8 +466,12 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   // Ring order of the tiles: K_0 .. K_{lead-1}, then V_i, K_{i+lead} in turn, then the last V.
   const int items = 2 * tiles;
   const int lead_now = min(lead, tiles);
-  auto wait = [&](uint64_t* bar, uint32_t parity) {  // for a whole warp, which goes on or gives up together
-    return __all_sync(~0u, ek::mbar_wait_bounded(bar, parity, abort)) != 0;
+  // For a whole warp. False once any wait of the block has run out (then all give up; what is computed meanwhile
+  // stays within the block's own buffers).
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    ek::mbar_wait_bounded(bar, parity, abort);
+    __syncwarp();
+    return *abort == 0;
   };
 
   if (warp < 8) {
@@ -472,7 +480,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     const int row = row0 + (wide ? w * 128 : 0) + t;
     const bool idle = row0 + (wide ? w * 128 : 0) + (warp % 4) * 32 >= row1;  // no row in this warp
     const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16);
-    const uint32_t ts = lanes + w * 128, to = lanes + 256 + w * D;
+    const uint32_t ts = lanes + C::S, tp = lanes + C::P + w * 64, to = lanes + C::O + w * D;
     const int mine = wide ? tiles : (tiles - w + 1) / 2;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -500,13 +508,18 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
       }
       if (!(ok = wait(s_full + w, use & 1))) break;
       ek::tcgen05_after_sync();
-      if (!idle) {
+      if (idle) {
+        ek::mbar_arrive(s_empty);
+        if (use > 0 && !(ok = wait(p_empty + w, (use - 1) & 1))) break;
+      } else {
         uint32_t x[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) ek::tmem_ld32(x[c], ts + c * 32);
         ek::tmem_wait_ld(x[0]);
 #pragma unroll
         for (int c = 1; c < 4; ++c) ek::tmem_after(x[c]);
+        ek::tcgen05_before_sync();
+        ek::mbar_arrive(s_empty);
         if (I8) {  // scores in units of base 2
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -534,6 +547,9 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         const float high = ek::max3_nan(ek::max3_nan(top[0], top[1], top[2]), top[3], top[3]) * (I8 ? 1.f : scale);
         const float grown = ek::max3_nan(m, high, high);
         if (use == 0) m = grown;
+        // O and P are free once the products of the tile before are done
+        if (use > 0 && !(ok = wait(p_empty + w, (use - 1) & 1))) break;
+        ek::tcgen05_after_sync();
         const bool far = grown > m + 8.f || grown != grown;
         if (__any_sync(~0u, far)) {
           const float fix = far ? exp2_approx(m - grown) : 1.f;
@@ -571,7 +587,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
             }
             out[e / 2] = pack_bf16(pr.x, pr.y);
           }
-          ek::tmem_st16(ts + c * 16, out);
+          ek::tmem_st16(tp + c * 16, out);
         }
         const float2 sum2 = ek::unpair(ek::add2(sums[0], sums[1]));
         l += sum2.x + sum2.y;
@@ -580,7 +596,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
       ek::tcgen05_before_sync();
       ek::mbar_arrive(p_full + w);
     }
-    if (ok && mine > 0) ok = wait(o_full + w, 0);
+    if (ok && mine > 0) ok = wait(p_empty + w, (mine - 1) & 1);
     ek::tcgen05_after_sync();
     if (!ok) m = NAN, l = NAN;  // a wait ran out: the result is NaN and the status is set
     if (!idle) {
@@ -673,63 +689,46 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         int quiet = 0;
         for (int i = max(0, n - N); i < n; ++i) ek::mbar_wait_bounded(f + i % N, (i / N) & 1, &quiet);
       }
-    } else if (warp == C::MMA) {
+    } else if (warp == C::SCORES || warp == C::VALUES) {
+      // Two warps issue the products, so that neither's waits hold up the other's: the queue of issued products is
+      // short, and a thread that issues is in step with the tensor core.
       constexpr uint32_t SD = ek::mma_desc(128, 128, false), OD = ek::mma_desc(128, D, true);
       const uint32_t stage = ek::smem_u32(smem + C::OFF_STAGE);
-      int n = 0;  // ring position
-      auto scores = [&](int w, uint32_t k) {
-        const uint32_t q = ek::smem_u32(smem) + (wide ? w * C::TILE : 0);
-#pragma unroll
-        for (int kt = 0; kt < D / 16; ++kt) {
-          const uint32_t off = kt / 4 * 16384 + kt % 4 * 32;
-          ek::mma_ss(tmem + w * 128, ek::smem_desc(q + off, 16), ek::smem_desc(k + off, 16), SD, kt > 0);
-        }
-        ek::mma_commit(s_full + w);
-      };
-      auto values = [&](int w, uint32_t v, bool add) {
-#pragma unroll
-        for (int kt = 0; kt < 8; ++kt)
-          ek::mma_ts(tmem + 256 + w * D, tmem + w * 128 + kt * 8, ek::smem_desc(v + kt * 2048, 16384), OD, add || kt > 0);
-      };
-      auto wait_stage = [&](int i) { return wait(full + i % C::STAGES, (i / C::STAGES) & 1); };
-      bool ok = true;
-      for (int i = 0; ok && i < lead_now; ++i) {  // first scores
-        if (!(ok = wait_stage(n))) break;
-        ek::tcgen05_after_sync();
-        const uint32_t k = stage + n % C::STAGES * C::TILE;
-        if (ek::elect_one()) {
-          if (wide) scores(0, k), scores(1, k);
-          else scores(i, k);
-          ek::mma_commit(empty + n % C::STAGES);
-        }
-        __syncwarp();
-        ++n;
-      }
-      for (int i = 0; ok && i < tiles; ++i) {
-        const bool more = i + lead_now < tiles;
-        const int nv = n, nk = n + 1;
-        n += more ? 2 : 1;
-        for (int turn = 0; turn < (wide ? 2 : 1); ++turn) {
-          const int w = wide ? turn : i % 2, use = wide ? i : i / 2;
-          const bool last_turn = !wide || turn == 1;
-          if (turn == 0 && !(ok = wait_stage(nv))) break;
-          if (!(ok = wait(p_full + w, use & 1))) break;
+      const int count = wide ? 2 * tiles : tiles;  // products; number i belongs to warpgroup i % 2
+      if (warp == C::SCORES) {
+        // S = Q K^T of product i, once the scores before it have been taken
+        for (int i = 0; i < count; ++i) {
+          const int w = i % 2, t = wide ? i / 2 : i, at = t < lead_now ? t : 2 * t - lead_now + 1;  // ring position of K
+          if (!wait(full + at % C::STAGES, (at / C::STAGES) & 1) || (i > 0 && !wait(s_empty, (i - 1) & 1))) break;
           ek::tcgen05_after_sync();
+          const uint32_t q = ek::smem_u32(smem) + (wide ? w * C::TILE : 0), k = stage + at % C::STAGES * C::TILE;
           if (ek::elect_one()) {
-            values(w, stage + nv % C::STAGES * C::TILE, use > 0);
-            if (last_turn) ek::mma_commit(empty + nv % C::STAGES);
-            if (i + (wide ? 1 : 2) >= tiles) ek::mma_commit(o_full + w);
+#pragma unroll
+            for (int kt = 0; kt < D / 16; ++kt) {
+              const uint32_t off = kt / 4 * 16384 + kt % 4 * 32;
+              ek::mma_ss(tmem + C::S, ek::smem_desc(q + off, 16), ek::smem_desc(k + off, 16), SD, kt > 0);
+            }
+            ek::mma_commit(s_full + w);
+            if (!wide || w == 1) ek::mma_commit(empty + at % C::STAGES);
           }
           __syncwarp();
-          if (more) {
-            if (turn == 0 && !(ok = wait_stage(nk))) break;
-            ek::tcgen05_after_sync();
-            if (ek::elect_one()) {
-              scores(w, stage + nk % C::STAGES * C::TILE);
-              if (last_turn) ek::mma_commit(empty + nk % C::STAGES);
-            }
-            __syncwarp();
+        }
+      } else {
+        // O += P V of product i
+        for (int i = 0; i < count; ++i) {
+          const int w = i % 2, t = wide ? i / 2 : i, at = t < tiles - lead_now ? lead_now + 2 * t : tiles + t;
+          if (!wait(full + at % C::STAGES, (at / C::STAGES) & 1) || !wait(p_full + w, (i / 2) & 1)) break;
+          ek::tcgen05_after_sync();
+          const uint32_t v = stage + at % C::STAGES * C::TILE;
+          if (ek::elect_one()) {
+#pragma unroll
+            for (int kt = 0; kt < 8; ++kt)
+              ek::mma_ts(tmem + C::O + w * D, tmem + C::P + w * 64 + kt * 8, ek::smem_desc(v + kt * 2048, 16384), OD,
+                         i > 1 || kt > 0);
+            ek::mma_commit(p_empty + w);
+            if (!wide || w == 1) ek::mma_commit(empty + at % C::STAGES);
           }
+          __syncwarp();
         }
       }
       // tensor memory is freed below: nothing may be in flight
@@ -742,7 +741,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   __syncwarp();
   __syncthreads();
   if (threadIdx.x == 0 && *abort) g_attention_status = 1;
-  if (warp == C::MMA) {
+  if (warp == C::SCORES) {
     ek::tcgen05_after_sync();
     ek::tmem_free(tmem, 512);
   }
