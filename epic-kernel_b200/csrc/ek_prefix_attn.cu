@@ -345,21 +345,23 @@ struct Many {
   static constexpr int BLOCKS = D / 64;               // 64-element column blocks of a tile
   static constexpr int TILE = 128 * D * 2;            // bytes of a bf16 tile
   static constexpr int RAW = 128 * D;                 // bytes of an 8-bit tile
-  static constexpr int STAGES = I8 ? (D == 128 ? 3 : 4) : (D == 128 ? 5 : 8);
-  static constexpr int RAW_STAGES = I8 ? (D == 128 ? 3 : 6) : 0;
+  // K and V have rings of their own: two warps consume them, and each must see every phase of its barriers
+  static constexpr int KS = D == 64 ? 4 : I8 ? 2 : 3, VS = D == 64 ? 4 : 2;
+  static constexpr int RAW_STAGES = I8 ? (D == 128 ? 2 : 4) : 0;
   static constexpr int WARPS = I8 ? 16 : 12;          // 8 softmax, [4 widening,] loads, scores, values, 1 idle
   static constexpr int LOADER = WARPS - 4, SCORES = WARPS - 3, VALUES = WARPS - 2;
   // registers per thread: at launch, of the softmax, widening and other warpgroups
   static constexpr int REGS = I8 ? 128 : 168, SOFTMAX_REGS = I8 ? 200 : 208, WIDEN_REGS = 72, OTHER_REGS = I8 ? 40 : 88;
   static_assert(2 * SOFTMAX_REGS + (I8 ? WIDEN_REGS : 0) + OTHER_REGS == WARPS / 4 * REGS, "registers of the block");
-  static constexpr int OFF_STAGE = 2 * TILE;          // after two Q tiles
-  static constexpr int OFF_RAW = OFF_STAGE + STAGES * TILE;
+  static constexpr int OFF_K = 2 * TILE;              // after two Q tiles
+  static constexpr int OFF_V = OFF_K + KS * TILE;
+  static constexpr int OFF_RAW = OFF_V + VS * TILE;
   static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;
-  static constexpr int SCALE_BYTES = I8 ? 2 * 2 * 2 * 128 * 4 : 0;  // warpgroup, parity, k / v, key
+  static constexpr int SCALE_BYTES = I8 ? 2 * 2 * 128 * 4 : 0;  // warpgroup, k / v, key
   static constexpr int OFF_BAR = OFF_SCALE + SCALE_BYTES;
-  static constexpr int BARS = 2 * STAGES + 2 * RAW_STAGES + 6 + 2;
+  static constexpr int BARS = 2 * KS + 2 * VS + 2 * RAW_STAGES + 6 + 2;
   static constexpr int S = 0, P = 128, O = 256;       // columns of tensor memory: scores, P and O of both warpgroups
-  static constexpr int SMEM = OFF_BAR + BARS * 8 + 16 + 1024;  // + alignment
+  static constexpr int SMEM = OFF_BAR + BARS * 8 + 16;
 };
 
 struct ManyParams {
@@ -370,9 +372,6 @@ struct ManyParams {
   int wide_splits, wide_tiles, narrow_splits, narrow_tiles;  // splits of the keys and 128-key tiles of each
   int negate;                   // scale < 0: q is negated and |scale| used
 };
-
-// Pairs out of every eight whose exponentials are taken by exp2_cubic.
-constexpr int CUBIC = 0;
 
 __device__ int g_attention_status;
 
@@ -387,30 +386,15 @@ __device__ __forceinline__ uint64_t score_pair(const uint32_t (&x)[32], int e) {
   return ek::pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
 }
 
-// 2^x of a pair without the exponential unit: x = n + r, |r| <= 1/2, 2^r by a cubic that is fitted at the Chebyshev
-// nodes of the interval (relative error below 1.1e-4, a fortieth of the rounding of P to bf16) and n added to the
-// exponent. x below -126 counts as -126.
-__device__ __forceinline__ float2 exp2_cubic(float2 x) {
-  constexpr float kRound = 12582912.f;  // 1.5 * 2^23
-  const uint64_t t = ek::pair(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const uint64_t z = ek::add2(t, ek::pair(kRound, kRound));
-  const uint64_t r = ek::add2(t, ek::mul2(ek::add2(z, ek::pair(-kRound, -kRound)), ek::pair(-1.f, -1.f)));
-  uint64_t p = ek::fma2(ek::pair(0.0558382829f, 0.0558382829f), r, ek::pair(0.242639479f, 0.242639479f));
-  p = ek::fma2(p, r, ek::pair(0.693136734f, 0.693136734f));
-  p = ek::fma2(p, r, ek::pair(0.999924557f, 0.999924557f));
-  const float2 pf = ek::unpair(p), zf = ek::unpair(z);
-  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(zf.x) << 23)),
-                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(zf.y) << 23)));
-}
-
 template <int D, bool I8>
 __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __grid_constant__ ManyParams p) {
   using C = Many<D, I8>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024 - (ek::smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* empty = full + C::STAGES;
-  uint64_t* raw_full = empty + C::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem[];  // atoms of the swizzle start on 1024 bytes
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* k_empty = k_full + C::KS;
+  uint64_t* v_full = k_empty + C::KS;
+  uint64_t* v_empty = v_full + C::VS;
+  uint64_t* raw_full = v_empty + C::VS;
   uint64_t* raw_empty = raw_full + C::RAW_STAGES;
   uint64_t* s_full = raw_empty + C::RAW_STAGES;
   uint64_t* p_full = s_full + 2;
@@ -434,14 +418,14 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   const int row1 = wide ? min(p.rows, row0 + 256) : p.rows;
   const int tile0 = split * per;
   const int tiles = min(per, (p.a.prefix_len + 127) / 128 - tile0);
-  const int lead = wide ? 2 : 3;  // K tiles in use before the first V tile
 
   if (warp == C::SCORES) ek::tmem_alloc(tmem_at, 512);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::STAGES; ++i) ek::mbar_init(full + i, I8 ? 128 : 1), ek::mbar_init(empty + i, 1);
+    for (int i = 0; i < C::KS; ++i) ek::mbar_init(k_full + i, I8 ? 128 : 1), ek::mbar_init(k_empty + i, 1);
+    for (int i = 0; i < C::VS; ++i) ek::mbar_init(v_full + i, I8 ? 128 : 1), ek::mbar_init(v_empty + i, 1);
     for (int i = 0; i < C::RAW_STAGES; ++i) ek::mbar_init(raw_full + i, 1), ek::mbar_init(raw_empty + i, 128);
-    for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 128), ek::mbar_init(p_empty + i, 1);
-    ek::mbar_init(s_empty, 128), ek::mbar_init(drained, 2);
+    for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 4), ek::mbar_init(p_empty + i, 1);
+    ek::mbar_init(s_empty, 4), ek::mbar_init(drained, 2);
     *abort = 0;
     ek::fence_mbar_init();
   }
@@ -463,15 +447,20 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   ek::tcgen05_after_sync();
   const uint32_t tmem = *tmem_at;
 
-  // Ring order of the tiles: K_0 .. K_{lead-1}, then V_i, K_{i+lead} in turn, then the last V.
-  const int items = 2 * tiles;
-  const int lead_now = min(lead, tiles);
-  // For a whole warp. False once any wait of the block has run out (then all give up; what is computed meanwhile
-  // stays within the block's own buffers).
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    ek::mbar_wait_bounded(bar, parity, abort);
+  // Order in which tiles are fetched: K_0 .. K_{lead-1}, then V_i, K_{i+lead} in turn, then the last V. Item n:
+  const int items = 2 * tiles, lead = min(C::KS, tiles);
+  auto item = [&](int n, bool& is_v) {
+    const int m = n - lead, both = 2 * (tiles - lead);
+    is_v = m >= both || (m >= 0 && m % 2 == 0);
+    return m < 0 ? n : m >= both ? m - (tiles - lead) : m / 2 + (is_v ? 0 : lead);
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // for a whole warp, which goes on or gives up together
+    return __all_sync(~0u, ek::mbar_wait_bounded(bar, parity, abort)) != 0;
+  };
+  // One arrival per warp: 128 on one barrier are serialised.
+  auto arrive = [&](uint64_t* bar) {
     __syncwarp();
-    return *abort == 0;
+    if (threadIdx.x % 32 == 0) ek::mbar_arrive(bar);
   };
 
   if (warp < 8) {
@@ -499,17 +488,21 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
       const float* ks = nullptr;
       const float* vs = nullptr;
       if (I8) {
-        float* sc = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (w * 2 + (use & 1)) * 256;
+        float* sc = reinterpret_cast<float*>(smem + C::OFF_SCALE) + w * 256;
+        auto sync = [&] {
+          if (w == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+          else asm volatile("bar.sync 2, 128;" ::: "memory");
+        };
+        sync();  // the scales of the tile before are done with
         sc[t] = next_ks * scale, sc[128 + t] = next_vs;
-        if (w == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-        else asm volatile("bar.sync 2, 128;" ::: "memory");
+        sync();
         ks = sc, vs = sc + 128;
         next_ks = key_scale(use + 1, 0), next_vs = key_scale(use + 1, 1);
       }
       if (!(ok = wait(s_full + w, use & 1))) break;
       ek::tcgen05_after_sync();
       if (idle) {
-        ek::mbar_arrive(s_empty);
+        arrive(s_empty);
         if (use > 0 && !(ok = wait(p_empty + w, (use - 1) & 1))) break;
       } else {
         uint32_t x[4][32];
@@ -519,7 +512,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 #pragma unroll
         for (int c = 1; c < 4; ++c) ek::tmem_after(x[c]);
         ek::tcgen05_before_sync();
-        ek::mbar_arrive(s_empty);
+        arrive(s_empty);
         if (I8) {  // scores in units of base 2
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -576,9 +569,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
           for (int e = 0; e < 32; e += 2) {
             const uint64_t s2 = score_pair(x[c], e);
             const float2 t2 = ek::unpair(I8 ? ek::add2(s2, shift) : ek::fma2(s2, slope, shift));
-            float2 pr;
-            if (e % 16 >= 16 - 2 * CUBIC) pr = exp2_cubic(t2);
-            else pr = make_float2(exp2_approx(t2.x), exp2_approx(t2.y));
+            float2 pr = make_float2(exp2_approx(t2.x), exp2_approx(t2.y));
             uint64_t p2 = ek::pair(pr.x, pr.y);
             sums[e / 2 & 1] = ek::add2(sums[e / 2 & 1], p2);
             if (I8) {
@@ -594,7 +585,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         ek::tmem_wait_st();
       }
       ek::tcgen05_before_sync();
-      ek::mbar_arrive(p_full + w);
+      arrive(p_full + w);
     }
     if (ok && mine > 0) ok = wait(p_empty + w, (mine - 1) & 1);
     ek::tcgen05_after_sync();
@@ -623,11 +614,14 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     ek::registers_down<C::WIDEN_REGS>();
     const int t = threadIdx.x - 256;
     for (int n = 0; n < items; ++n) {
-      const int rs = n % (I8 ? C::RAW_STAGES : 1), cs = n % C::STAGES;
-      if (!wait(raw_full + rs, (n / (I8 ? C::RAW_STAGES : 1)) & 1)) break;
-      if (n >= C::STAGES && !wait(empty + cs, (n / C::STAGES - 1) & 1)) break;
+      constexpr int RS = I8 ? C::RAW_STAGES : 1;
+      bool is_v;
+      const int tile = item(n, is_v), rs = n % RS;
+      const int stages = is_v ? C::VS : C::KS, cs = tile % stages;
+      if (!wait(raw_full + rs, (n / RS) & 1)) break;
+      if (tile >= stages && !wait((is_v ? v_empty : k_empty) + cs, (tile / stages - 1) & 1)) break;
       const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW;
-      uint8_t* to = smem + C::OFF_STAGE + cs * C::TILE;
+      uint8_t* to = smem + (is_v ? C::OFF_V : C::OFF_K) + cs * C::TILE;
 #pragma unroll 4
       for (int i = t; i < 128 * D / 16; i += 128) {
         const int r = i / (D / 16), piece = i % (D / 16);
@@ -651,57 +645,68 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         }
       }
       ek::fence_proxy_async_smem();
-      ek::mbar_arrive(full + cs);
+      ek::mbar_arrive((is_v ? v_full : k_full) + cs);
       ek::mbar_arrive(raw_empty + rs);
     }
   } else {
     ek::registers_down<C::OTHER_REGS>();
     if (warp == C::LOADER) {
-      constexpr int N = I8 ? C::RAW_STAGES : C::STAGES;
-      uint64_t* f = I8 ? raw_full : full;
-      uint64_t* e = I8 ? raw_empty : empty;
-      uint8_t* base = smem + (I8 ? C::OFF_RAW : C::OFF_STAGE);
-      constexpr int BYTES = I8 ? C::RAW : C::TILE;
-      int n = 0;
+      constexpr int RS = I8 ? C::RAW_STAGES : 1, BYTES = I8 ? C::RAW : C::TILE;
+      // buffer and barriers of item n
+      auto slot = [&](int n, bool& is_v, int& tile, uint64_t*& f, uint64_t*& e, int& round, uint8_t*& to) {
+        tile = item(n, is_v);
+        const int stages = I8 ? RS : is_v ? C::VS : C::KS, at = I8 ? n : tile;
+        round = at / stages;
+        f = (I8 ? raw_full : is_v ? v_full : k_full) + at % stages;
+        e = (I8 ? raw_empty : is_v ? v_empty : k_empty) + at % stages;
+        to = smem + (I8 ? C::OFF_RAW : is_v ? C::OFF_V : C::OFF_K) + at % stages * BYTES;
+      };
+      bool is_v;
+      int n = 0, tile, round;
+      uint64_t *f, *e;
+      uint8_t* to;
       for (; n < items; ++n) {
-        const int s = n % N;
-        if (n >= N && !wait(e + s, (n / N - 1) & 1)) break;
-        bool is_v;
-        int tile;
-        if (n < lead_now) is_v = false, tile = n;
-        else {
-          const int m = n - lead_now, both = 2 * (tiles - lead_now);
-          is_v = m >= both || m % 2 == 0;
-          tile = m >= both ? m - (tiles - lead_now) : m / 2 + (is_v ? 0 : lead_now);
-        }
+        slot(n, is_v, tile, f, e, round, to);
+        if (round > 0 && !wait(e, (round - 1) & 1)) break;
         const int key = (tile0 + tile) * 128;
         const CUtensorMap* map = is_v ? &p.v : &p.k;
         const bool keys_first = is_v ? p.v_keys_first : p.k_keys_first;
         if (ek::elect_one()) {
-          ek::mbar_arrive_expect_tx(f + s, BYTES);
+          ek::mbar_arrive_expect_tx(f, BYTES);
           for (int blk = 0; blk < (I8 ? 1 : C::BLOCKS); ++blk)
-            ek::tma_load_3d(base + s * BYTES + blk * 16384, map, blk * 64, keys_first ? key : head,
-                            keys_first ? head : key, f + s);
+            ek::tma_load_3d(to + blk * 16384, map, blk * 64, keys_first ? key : head, keys_first ? head : key, f);
         }
         __syncwarp();
       }
-      if (n < items) {  // gave up: let the copies in flight land
+      if (n < items) {  // gave up: let the copies in flight land, the last of each buffer
         int quiet = 0;
-        for (int i = max(0, n - N); i < n; ++i) ek::mbar_wait_bounded(f + i % N, (i / N) & 1, &quiet);
+        for (int i = max(0, n - 2 * (C::KS + C::VS)); i < n; ++i) {
+          slot(i, is_v, tile, f, e, round, to);
+          bool last = true;
+          for (int j = i + 1; j < n; ++j) {
+            bool v2;
+            int t2, r2;
+            uint64_t *f2, *e2;
+            uint8_t* to2;
+            slot(j, v2, t2, f2, e2, r2, to2);
+            last = last && f2 != f;
+          }
+          if (last) ek::mbar_wait_bounded(f, round & 1, &quiet);
+        }
       }
     } else if (warp == C::SCORES || warp == C::VALUES) {
       // Two warps issue the products, so that neither's waits hold up the other's: the queue of issued products is
       // short, and a thread that issues is in step with the tensor core.
       constexpr uint32_t SD = ek::mma_desc(128, 128, false), OD = ek::mma_desc(128, D, true);
-      const uint32_t stage = ek::smem_u32(smem + C::OFF_STAGE);
       const int count = wide ? 2 * tiles : tiles;  // products; number i belongs to warpgroup i % 2
       if (warp == C::SCORES) {
         // S = Q K^T of product i, once the scores before it have been taken
         for (int i = 0; i < count; ++i) {
-          const int w = i % 2, t = wide ? i / 2 : i, at = t < lead_now ? t : 2 * t - lead_now + 1;  // ring position of K
-          if (!wait(full + at % C::STAGES, (at / C::STAGES) & 1) || (i > 0 && !wait(s_empty, (i - 1) & 1))) break;
+          const int w = i % 2, t = wide ? i / 2 : i;
+          if (!wait(k_full + t % C::KS, (t / C::KS) & 1) || (i > 0 && !wait(s_empty, (i - 1) & 1))) break;
           ek::tcgen05_after_sync();
-          const uint32_t q = ek::smem_u32(smem) + (wide ? w * C::TILE : 0), k = stage + at % C::STAGES * C::TILE;
+          const uint32_t base = ek::smem_u32(smem);
+          const uint32_t q = base + (wide ? w * C::TILE : 0), k = base + C::OFF_K + t % C::KS * C::TILE;
           if (ek::elect_one()) {
 #pragma unroll
             for (int kt = 0; kt < D / 16; ++kt) {
@@ -709,24 +714,24 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
               ek::mma_ss(tmem + C::S, ek::smem_desc(q + off, 16), ek::smem_desc(k + off, 16), SD, kt > 0);
             }
             ek::mma_commit(s_full + w);
-            if (!wide || w == 1) ek::mma_commit(empty + at % C::STAGES);
+            if (!wide || w == 1) ek::mma_commit(k_empty + t % C::KS);
           }
           __syncwarp();
         }
       } else {
         // O += P V of product i
         for (int i = 0; i < count; ++i) {
-          const int w = i % 2, t = wide ? i / 2 : i, at = t < tiles - lead_now ? lead_now + 2 * t : tiles + t;
-          if (!wait(full + at % C::STAGES, (at / C::STAGES) & 1) || !wait(p_full + w, (i / 2) & 1)) break;
+          const int w = i % 2, t = wide ? i / 2 : i;
+          if (!wait(v_full + t % C::VS, (t / C::VS) & 1) || !wait(p_full + w, (i / 2) & 1)) break;
           ek::tcgen05_after_sync();
-          const uint32_t v = stage + at % C::STAGES * C::TILE;
+          const uint32_t v = ek::smem_u32(smem) + C::OFF_V + t % C::VS * C::TILE;
           if (ek::elect_one()) {
 #pragma unroll
             for (int kt = 0; kt < 8; ++kt)
               ek::mma_ts(tmem + C::O + w * D, tmem + C::P + w * 64 + kt * 8, ek::smem_desc(v + kt * 2048, 16384), OD,
                          i > 1 || kt > 0);
             ek::mma_commit(p_empty + w);
-            if (!wide || w == 1) ek::mma_commit(empty + at % C::STAGES);
+            if (!wide || w == 1) ek::mma_commit(v_empty + t % C::VS);
           }
           __syncwarp();
         }

@@ -190,11 +190,11 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // Waits for phase `parity` of `bar`. False once *abort is set, by this wait
 // after about two seconds or by another one.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
   uint64_t t0 = 0;
   for (;;) {
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+    // test_wait does not suspend the thread: a suspended one takes some 300 cycles to come back
+    for (int i = 0; i < 1024; ++i)
+      if (mbar_test_wait(bar, parity)) return true;
     if (*abort) return false;
     uint64_t now;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
