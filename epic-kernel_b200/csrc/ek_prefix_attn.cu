@@ -359,7 +359,9 @@ struct Many {
   static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;
   static constexpr int SCALE_BYTES = I8 ? 2 * 2 * 128 * 4 : 0;  // warpgroup, k / v, key
   static constexpr int OFF_BAR = OFF_SCALE + SCALE_BYTES;
-  static constexpr int BARS = 2 * KS + 2 * VS + 2 * RAW_STAGES + 6 + 2;
+  static constexpr int BARS = 2 * KS + 2 * VS + 2 * RAW_STAGES + 6 + 3;
+  static constexpr int OUT_ROW = D * 4 + 16;          // bytes of a row of O on its way out; eight rows meet all banks
+  static_assert(256 * OUT_ROW <= OFF_RAW, "rows of O in the place of Q, K and V");
   static constexpr int S = 0, P = 128, O = 256;       // columns of tensor memory: scores, P and O of both warpgroups
   static constexpr int SMEM = OFF_BAR + BARS * 8 + 16;
 };
@@ -400,7 +402,8 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   uint64_t* p_full = s_full + 2;
   uint64_t* p_empty = p_full + 2;   // the products with P are done
   uint64_t* s_empty = p_empty + 2;  // the scores are in registers
-  uint64_t* drained = s_empty + 1;
+  uint64_t* q_full = s_empty + 1;
+  uint64_t* drained = q_full + 1;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_at + 1);
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0);  // uniform
@@ -425,23 +428,10 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     for (int i = 0; i < C::VS; ++i) ek::mbar_init(v_full + i, I8 ? 128 : 1), ek::mbar_init(v_empty + i, 1);
     for (int i = 0; i < C::RAW_STAGES; ++i) ek::mbar_init(raw_full + i, 1), ek::mbar_init(raw_empty + i, 128);
     for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 4), ek::mbar_init(p_empty + i, 1);
-    ek::mbar_init(s_empty, 4), ek::mbar_init(drained, 2);
+    ek::mbar_init(s_empty, 4), ek::mbar_init(q_full, 8), ek::mbar_init(drained, 2);
     *abort = 0;
     ek::fence_mbar_init();
   }
-  // Q rows, zeros past the last
-  for (int i = threadIdx.x; i < (wide ? 256 : 128) * (D / 8); i += C::WARPS * 32) {
-    const int r = i / (D / 8), piece = i % (D / 8), at = row0 + r;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (at < row1) {
-      const int b = at / p.a.group, h = head * p.a.group + at % p.a.group;
-      x = __ldg(reinterpret_cast<const uint4*>(p.a.q + b * p.a.q_batch + h * p.a.q_head) + piece);
-      if (p.negate) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
-    }
-    const int t = r % 128;
-    *reinterpret_cast<uint4*>(smem + r / 128 * C::TILE + piece / 8 * 16384 + t * 128 + ((piece % 8 ^ (t & 7)) << 4)) = x;
-  }
-  ek::fence_proxy_async_smem();
   ek::tcgen05_before_sync();
   __syncthreads();
   ek::tcgen05_after_sync();
@@ -465,6 +455,32 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 
   if (warp < 8) {
     ek::registers_up<C::SOFTMAX_REGS>();
+    {  // Q rows into the swizzled tiles, zeros past the last; eight loads at a time
+      constexpr int PIECES = D / 8, ROWS = 32 / PIECES, BATCH = 8;
+      const int piece = threadIdx.x % PIECES, r0 = warp * 32 + threadIdx.x % 32 / PIECES;
+      const int rows = wide ? 32 : 16, first = wide ? r0 : warp * 16 + threadIdx.x % 32 / PIECES;
+      for (int i = 0; i < rows; i += ROWS * BATCH) {
+        uint4 x[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int r = first + i + u * ROWS, at = row0 + r;
+          x[u] = make_uint4(0, 0, 0, 0);
+          if (i + u * ROWS < rows && at < row1) {
+            const int b = at / p.a.group, h = head * p.a.group + at % p.a.group;
+            x[u] = __ldg(reinterpret_cast<const uint4*>(p.a.q + b * p.a.q_batch + h * p.a.q_head) + piece);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          if (i + u * ROWS >= rows) continue;
+          const int r = first + i + u * ROWS, t = r % 128;
+          if (p.negate) x[u].x ^= 0x80008000u, x[u].y ^= 0x80008000u, x[u].z ^= 0x80008000u, x[u].w ^= 0x80008000u;
+          *reinterpret_cast<uint4*>(smem + r / 128 * C::TILE + piece / 8 * 16384 + t * 128 + ((piece % 8 ^ (t & 7)) << 4)) = x[u];
+        }
+      }
+      ek::fence_proxy_async_smem();
+      arrive(q_full);
+    }
     const int w = warp / 4, t = threadIdx.x % 128;
     const int row = row0 + (wide ? w * 128 : 0) + t;
     const bool idle = row0 + (wide ? w * 128 : 0) + (warp % 4) * 32 >= row1;  // no row in this warp
@@ -590,23 +606,27 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     if (ok && mine > 0) ok = wait(p_empty + w, (mine - 1) & 1);
     ek::tcgen05_after_sync();
     if (!ok) m = NAN, l = NAN;  // a wait ran out: the result is NaN and the status is set
+    asm volatile("bar.sync 3, 256;" ::: "memory");  // all products of both warpgroups are done: Q, K and V are free
     if (!idle) {
       const int b = row / p.a.group, h = head * p.a.group + row % p.a.group;
       const long long total_rows = (long long)p.a.batch * p.a.q_heads;
       const long long at = (wide ? split : 2 * split + w) * total_rows + (long long)b * p.a.q_heads + h;
       if (row < row1) p.a.part_ml[at] = make_float2(m, l);
-      if (mine > 0) {
-#pragma unroll 1
+      // each row of O through shared memory as one bulk copy: a thread's own 16-byte stores would fill half sectors
+      if (mine > 0 && ok) {
+        uint8_t* mine_row = smem + (w * 128 + t) * C::OUT_ROW;
+#pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
           ek::tmem_ld32(r, to + c * 32);
           ek::tmem_wait_ld(r);
-          if (row < row1) {
-            uint4* out = reinterpret_cast<uint4*>(p.a.part_o + at * D + c * 32);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
-          }
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(mine_row + c * 128 + e * 16) = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
         }
+        ek::fence_proxy_async_smem();
+        if (row < row1) ek::bulk_store(p.a.part_o + at * D, mine_row, D * 4);
+        ek::bulk_store_wait();
       }
     }
     ek::tcgen05_before_sync();
@@ -701,7 +721,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
       const int count = wide ? 2 * tiles : tiles;  // products; number i belongs to warpgroup i % 2
       if (warp == C::SCORES) {
         // S = Q K^T of product i, once the scores before it have been taken
-        for (int i = 0; i < count; ++i) {
+        for (int i = 0; i < count && (i > 0 || wait(q_full, 0)); ++i) {
           const int w = i % 2, t = wide ? i / 2 : i;
           if (!wait(k_full + t % C::KS, (t / C::KS) & 1) || (i > 0 && !wait(s_empty, (i - 1) & 1))) break;
           ek::tcgen05_after_sync();

@@ -142,6 +142,14 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// Bulk copy of this thread's bytes from shared to global memory (16-byte aligned, a multiple of 16).
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---------------------------------------------------------------- registers
 // Registers per thread of the calling warpgroup; all warpgroups together at most what the block was launched with.
 template <int N>
