@@ -12,12 +12,12 @@
 // `few_rows` computes an item for up to 8 query rows with mma.m16n8k16 on the
 // transposed products, S^T = K Q^T and O^T = V^T P^T, so that the 16-row side
 // of the instruction carries keys (or dimensions) and the 8-row side the query
-// rows. K and V go from global memory to fragment registers with 16-byte
-// loads: the contraction order over d is free, so lane c of a quad takes 8
-// (bf16) or 16 (int8) consecutive dimensions and q is laid out to match. P^T
-// becomes a B fragment by one 8x8 transpose in registers. 8-bit codes are
-// exact in bf16; K's scale multiplies the score and V's scale the probability.
-// Bound: bytes (4 flops per byte and query row).
+// rows. With 8-bit rows the contraction order over d is free, so lane c of a
+// quad takes 16 consecutive codes and q is laid out to match. P^T becomes a B
+// fragment by one 8x8 transpose in registers. 8-bit codes are exact in bf16;
+// K's scale multiplies the score and V's scale the probability. Bound: bytes
+// (4 flops per byte and query row). `many_rows` takes the prefix when it serves
+// many query rows.
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -29,6 +29,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ int g_attention_status;  // 1: a wait inside a kernel ran out
 
 struct Store {
   const char* k;
@@ -92,94 +94,80 @@ __device__ __forceinline__ uint32_t codes_to_bf16(uint32_t x) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The fragments of 16 keys of one KV head.
+// ---------------------------------------------------------------------------
+// `few_rows`: an item of up to 8 query rows of one KV head. A loader warp brings
+// 64 keys a stage into shared memory by TMA (K and V of the head, swizzled), and
+// each of four warps takes 16 of them.
 template <int D, bool I8>
-struct Rows {
-  // K: keys lane/4 and lane/4 + 8, dimensions by quad lane; V: keys 2c, 2c+1, 2c+8, 2c+9 of quad lane c,
-  // dimensions by lane/4
-  static constexpr int KV = I8 ? D / 64 : D / 32;  // 16-byte pieces of a key per quad lane
-  static constexpr int VW = I8 ? D / 32 : D / 16;  // 4-byte words of a key per lane/4
-  uint4 k[2][KV];
-  uint32_t v[4][VW];
-  float ks[2], vs[2][2];
+struct Few {
+  static constexpr int KEYS = 64, BOX = 32;            // keys of a stage, and of a TMA copy
+  static constexpr int TILE = KEYS * D * (I8 ? 1 : 2);  // bytes of a stage's K (or V)
+  static constexpr int STAGES = I8 ? (D == 128 ? 3 : 4) : (D == 128 ? 2 : 3);
+  static constexpr int OFF_BAR = 2 * STAGES * TILE;
+  static constexpr int SMEM = OFF_BAR + 2 * STAGES * 8 + 16 + kWarps * 8 * 8;
+  static_assert(kWarps * 8 * D * 4 <= 2 * STAGES * TILE, "the warps' O in the place of the stages");
+};
+
+// A tensor map of rows [batch][row][head][D] and where the coordinates go: the dimensions behind D are sorted by stride.
+struct RowMap {
+  CUtensorMap map;
+  int8_t head, row, batch;  // place of the coordinate, or -1: the dimension is not there (one entry, or stride 0)
+
+  __device__ __forceinline__ void load(void* dst, int d, int h, int r, int b, uint64_t* bar) const {
+    const int c0 = head == 0 ? h : row == 0 ? r : batch == 0 ? b : 0;
+    const int c1 = head == 1 ? h : row == 1 ? r : batch == 1 ? b : 0;
+    const int c2 = head == 2 ? h : row == 2 ? r : batch == 2 ? b : 0;
+    ek::tma_load_4d(dst, &map, d, c0, c1, c2, bar);
+  }
+};
+
+struct FewParams {
+  RowMap prefix_k, prefix_v, own_k, own_v;
+  AttnParams a;
 };
 
 template <int D, bool I8>
-__device__ __forceinline__ void load_rows(Rows<D, I8>& r, const Store& s, long long b, int head, int t0, int t1) {
-  const int lane = threadIdx.x % 32, c = lane % 4, j = lane / 4;
-  const char* kb = s.k + b * s.k_batch + head * s.k_head + c * 16;
-  const char* vb = s.v + b * s.v_batch + head * s.v_head;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = t0 + j + 8 * i;
-    const bool in = t < t1;
-#pragma unroll
-    for (int m = 0; m < r.KV; ++m)
-      r.k[i][m] = in ? __ldg(reinterpret_cast<const uint4*>(kb + t * s.k_row + m * 64)) : make_uint4(0, 0, 0, 0);
-    if (I8) r.ks[i] = in ? __bfloat162float(s.ks[b * s.ks_batch + t * s.ks_row + head * s.ks_head]) : 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = t0 + 2 * c + (i & 1) + (i & 2) * 4;
-    const bool in = t < t1;
-    const char* at = vb + t * s.v_row;
-    if (I8 && D == 64) {
-      const uint2 x = in ? __ldg(reinterpret_cast<const uint2*>(at + j * 8)) : make_uint2(0, 0);
-      r.v[i][0] = x.x, r.v[i][1] = x.y;
-    } else {
-#pragma unroll
-      for (int m = 0; m < r.VW / 4; ++m) {
-        const uint4 x = in ? __ldg(reinterpret_cast<const uint4*>(at + m * 128 + j * 16)) : make_uint4(0, 0, 0, 0);
-        r.v[i][4 * m] = x.x, r.v[i][4 * m + 1] = x.y, r.v[i][4 * m + 2] = x.z, r.v[i][4 * m + 3] = x.w;
-      }
-    }
-  }
-  if (I8) {
-    // scales of keys lane/4 (+8), where P is still laid out by key
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = t0 + j + 8 * i;
-      r.vs[i][0] = t < t1 ? __bfloat162float(s.vs[b * s.vs_batch + t * s.vs_row + head * s.vs_head]) : 0.f;
-    }
-  }
-}
-
-// Dimension of element ee (0 .. D/8 - 1) that lane/4 = j holds of V.
-template <int D, bool I8>
-__device__ __forceinline__ int v_dim(int j, int ee) {
-  if (I8) return j * (D / 8) + ee;
-  return (ee / 8) * 64 + j * 8 + ee % 8;
-}
-
-template <int D, bool I8>
-__global__ void __launch_bounds__(kWarps * 32) few_rows(const AttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_constant__ FewParams fp) {
+  using C = Few<D, I8>;
   constexpr int KT = D / 16;  // 16-wide steps over the dimensions
-  __shared__ float s_o[kWarps][8][D];
-  __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = lane % 4, j = lane / 4;
+  const AttnParams& p = fp.a;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* empty = full + C::STAGES;
+  volatile int* abort = reinterpret_cast<volatile int*>(empty + C::STAGES);
+  float* s_m = reinterpret_cast<float*>(smem + C::OFF_BAR + 2 * C::STAGES * 8 + 16);
+  float* s_l = s_m + kWarps * 8;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32, c = lane % 4, j = lane / 4;
 
   // the item
   long long id = blockIdx.x;
   const long long prefix_items = (long long)p.prefix_slots * p.prefix_tiles * p.kv_heads;
   const bool shared = id < prefix_items;
-  int head, tile, slot, seq = 0, t0, t1;
+  int head, tile, slot, seq = 0;
   if (shared) {
     head = (int)(id % p.kv_heads), id /= p.kv_heads;
     tile = (int)(id % p.prefix_tiles);
     slot = (int)(id / p.prefix_tiles);
-    t0 = slot * p.prefix_chunk;
-    t1 = min(p.prefix_len, t0 + p.prefix_chunk);
   } else {
     id -= prefix_items;
     head = (int)(id % p.kv_heads), id /= p.kv_heads;
     tile = (int)(id % p.group_tiles), id /= p.group_tiles;
     seq = (int)(id % p.batch);
     slot = (int)(id / p.batch);
-    t0 = slot * p.own_chunk;
-    t1 = min(min(max(p.own_lens[seq], 0), p.max_own), t0 + p.own_chunk);
-    if (t0 >= t1) return;
   }
-  const Store& store = shared ? p.prefix : p.own;
+  const int chunk = shared ? p.prefix_chunk : p.own_chunk, t0 = slot * chunk;
+  const int t1 = min(t0 + chunk, shared ? p.prefix_len : min(max(__ldg(p.own_lens + seq), 0), p.max_own));
+  if (t0 >= t1) return;
+  const int steps = (t1 - t0 + C::KEYS - 1) / C::KEYS;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) ek::mbar_init(full + i, 1), ek::mbar_init(empty + i, kWarps);
+    *abort = 0;
+    ek::fence_mbar_init();
+  }
+  __syncthreads();
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // for a whole warp, which goes on or gives up together
+    return __all_sync(~0u, ek::mbar_wait_bounded(bar, parity, abort)) != 0;
+  };
   const int rows = shared ? p.batch * p.group : p.group;
   // row n of the tile -> (sequence, query head)
   auto locate = [&](int n, int& b, int& h) {
@@ -188,130 +176,219 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows(const AttnParams p) {
     h = head * p.group + (shared ? r % p.group : r);
     return r < rows;
   };
-
-  // q of row lane/4 as B fragments: the dimensions that quad lane c holds of K
-  uint32_t q[KT][2];
-  {
-    int b, h;
-    const bool in = locate(j, b, h);
-    const __nv_bfloat16* at = p.q + b * p.q_batch + h * p.q_head;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const int d = I8 ? (kt / 4) * 64 + c * 16 + (kt % 4) * 4 : (kt / 2) * 32 + c * 8 + (kt % 2) * 4;
-      const uint2 x = in ? __ldg(reinterpret_cast<const uint2*>(at + d)) : make_uint2(0, 0);
-      q[kt][0] = x.x, q[kt][1] = x.y;
-    }
-  }
-
-  float o[KT][4] = {};  // O^T: dimensions v_dim(j, 2 kt), v_dim(j, 2 kt + 1) of rows 2c, 2c + 1
+  float o[KT][4] = {};  // O^T: two dimensions of rows 2c, 2c + 1
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  for (int t = t0 + warp * 16; t < t1; t += kWarps * 16) {
-    Rows<D, I8> r;
-    load_rows<D, I8>(r, store, seq, head, t, t1);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (I8) {
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const uint32_t w0 = reinterpret_cast<const uint32_t*>(&r.k[0][kt / 4])[kt % 4];
-        const uint32_t w1 = reinterpret_cast<const uint32_t*>(&r.k[1][kt / 4])[kt % 4];
-        mma_16x8x16(s, codes_to_bf16(__byte_perm(w0, w0, 0x1100)), codes_to_bf16(__byte_perm(w1, w1, 0x1100)),
-                    codes_to_bf16(__byte_perm(w0, w0, 0x3322)), codes_to_bf16(__byte_perm(w1, w1, 0x3322)), q[kt][0],
-                    q[kt][1]);
+
+  if (warp == kWarps) {
+    int n = 0;
+    for (; n < steps; ++n) {
+      const int s = n % C::STAGES, t = t0 + n * C::KEYS;
+      if (n >= C::STAGES && !wait(empty + s, (n / C::STAGES - 1) & 1)) break;
+      if (ek::elect_one()) {
+        // copies of 32 keys, those that begin before the end
+        const int boxes = t + C::BOX < t1 ? 2 : 1;
+        ek::mbar_arrive_expect_tx(full + s, boxes * (C::TILE / 2) * 2);
+        for (int kv = 0; kv < 2; ++kv) {
+          const RowMap& map = shared ? (kv ? fp.prefix_v : fp.prefix_k) : kv ? fp.own_v : fp.own_k;
+          uint8_t* to = smem + (2 * s + kv) * C::TILE;
+          constexpr int ROW = I8 ? D : 128;  // bytes of a row of a copy
+          for (int blk = 0; blk < (I8 ? 1 : D / 64); ++blk)
+            for (int half = 0; half < boxes; ++half)
+              map.load(to + (blk * C::KEYS + half * C::BOX) * ROW, blk * 64, head, t + half * C::BOX, seq, full + s);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] *= r.ks[i / 2];
-    } else {
+      __syncwarp();
+    }
+    if (n < steps) {  // gave up: let the copies in flight land
+      int quiet = 0;
+      for (int i = max(0, n - C::STAGES); i < n; ++i) ek::mbar_wait_bounded(full + i % C::STAGES, (i / C::STAGES) & 1, &quiet);
+    }
+  } else {
+    // q of row lane/4 as B fragments
+    uint32_t q[KT][2];
+    {
+      int b, h;
+      const bool in = locate(j, b, h);
+      const __nv_bfloat16* at = p.q + b * p.q_batch + h * p.q_head;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&r.k[0][kt / 2]) + (kt % 2) * 2;
-        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&r.k[1][kt / 2]) + (kt % 2) * 2;
-        mma_16x8x16(s, w0[0], w1[0], w0[1], w1[1], q[kt][0], q[kt][1]);
+        if (I8) {  // the dimensions that quad lane c takes of K: 16 codes at a time
+          const uint2 x = in ? __ldg(reinterpret_cast<const uint2*>(at + (kt / 4) * 64 + c * 16 + (kt % 4) * 4)) : make_uint2(0, 0);
+          q[kt][0] = x.x, q[kt][1] = x.y;
+        } else {
+          q[kt][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(at + kt * 16 + c * 2)) : 0u;
+          q[kt][1] = in ? __ldg(reinterpret_cast<const uint32_t*>(at + kt * 16 + c * 2 + 8)) : 0u;
+        }
       }
     }
-    // s[0], s[1]: key t + j of rows 2c, 2c + 1; s[2], s[3]: key t + j + 8
-    float fix[2];
-    bool grew = false;
+    const Store& store = shared ? p.prefix : p.own;
+    const __nv_bfloat16* ksb = store.ks + seq * store.ks_batch + head * store.ks_head;
+    const __nv_bfloat16* vsb = store.vs + seq * store.vs_batch + head * store.vs_head;
+    float ks[2], vs[2];  // scales of keys j and j + 8 of the step
+    auto load_scales = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool in = t + j + 8 * i < t1;
+        ks[i] = in ? __bfloat162float(ksb[(t + j + 8 * i) * store.ks_row]) : 0.f;
+        vs[i] = in ? __bfloat162float(vsb[(t + j + 8 * i) * store.vs_row]) : 0.f;
+      }
+    };
+    if (I8) load_scales(t0 + warp * 16);
+    bool ok = true;
+    for (int n = 0; n < steps; ++n) {
+      const int st = n % C::STAGES, t = t0 + n * C::KEYS + warp * 16;
+      if (!(ok = wait(full + st, (n / C::STAGES) & 1))) break;
+      if (t < t1) {
+        const uint32_t kt0 = ek::smem_u32(smem + 2 * st * C::TILE), vt0 = kt0 + C::TILE;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (I8) {
+#pragma unroll
+          for (int m4 = 0; m4 < KT / 4; ++m4) {
+            uint4 w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int r = warp * 16 + j + 8 * i, ch = m4 * 4 + c;
+              w[i] = ek::lds128(kt0 + r * D + ((D == 128 ? ch ^ (r & 7) : ch ^ (r >> 1 & 3)) << 4));
+            }
+            const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&w[0]);
+            const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&w[1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mma_16x8x16(s, codes_to_bf16(__byte_perm(w0[e], w0[e], 0x1100)), codes_to_bf16(__byte_perm(w1[e], w1[e], 0x1100)),
+                          codes_to_bf16(__byte_perm(w0[e], w0[e], 0x3322)), codes_to_bf16(__byte_perm(w1[e], w1[e], 0x3322)),
+                          q[m4 * 4 + e][0], q[m4 * 4 + e][1]);
+          }
+        } else {
+          const int r = warp * 16 + lane % 16;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const int ch = 2 * kt + lane / 16;
+            uint32_t a[4];
+            ek::ldmatrix4<false>(a, kt0 + ch / 8 * (C::KEYS * 128) + r * 128 + ((ch % 8 ^ (r & 7)) << 4));
+            mma_16x8x16(s, a[0], a[1], a[2], a[3], q[kt][0], q[kt][1]);
+          }
+        }
+        // s[0], s[1]: key t + j of rows 2c, 2c + 1; s[2], s[3]: key t + j + 8
+        float fix[2];
+        bool grew = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[i] = t + j + 8 * (i / 2) < t1 ? s[i] * (I8 ? p.scale_log2 * ks[i / 2] : p.scale_log2) : -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float top = fmaxf(s[r], s[2 + r]);
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          const float next = fmaxf(m[r], top);
+          const float base = next == -INFINITY ? 0.f : next;
+          fix[r] = exp2_approx(m[r] - base);
+          grew |= next != m[r];
+          m[r] = next;
+          s[r] = exp2_approx(s[r] - base);
+          s[2 + r] = exp2_approx(s[2 + r] - base);
+          l[r] = l[r] * fix[r] + s[r] + s[2 + r];
+        }
+        if (grew) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            o[kt][0] *= fix[0], o[kt][1] *= fix[1];
+            o[kt][2] *= fix[0], o[kt][3] *= fix[1];
+          }
+        }
+        if (I8) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[i] = s[i] == 0.f ? 0.f : s[i] * vs[i / 2];
+          load_scales(t + C::KEYS);
+        }
+        // probabilities are rounded to bf16 for the product: half a step is 2^-8 of each, as for V itself
+        const uint32_t b0 = transpose_8x8(pack_bf16(s[0], s[1])), b1 = transpose_8x8(pack_bf16(s[2], s[3]));
+        if (I8) {
+          uint32_t v[4][D / 32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = warp * 16 + 2 * c + (i & 1) + (i & 2) * 4;
+            if (D == 128) {
+              const uint4 x = ek::lds128(vt0 + r * 128 + ((j ^ (r & 7)) << 4));
+              v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(smem + (2 * st + 1) * C::TILE + r * 64 +
+                                                              ((j / 2 ^ (r >> 1 & 3)) << 4) + (j & 1) * 8);
+              v[i][0] = x.x, v[i][1] = x.y;
+            }
+          }
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const int w = kt / 2, e = (kt % 2) * 2;  // word and first byte of element 2 kt
+            const uint32_t even = e == 0 ? 0x4400 : 0x6622, odd = e == 0 ? 0x5511 : 0x7733;
+            mma_16x8x16(o[kt], codes_to_bf16(__byte_perm(v[0][w], v[1][w], even)),
+                        codes_to_bf16(__byte_perm(v[0][w], v[1][w], odd)), codes_to_bf16(__byte_perm(v[2][w], v[3][w], even)),
+                        codes_to_bf16(__byte_perm(v[2][w], v[3][w], odd)), b0, b1);
+          }
+        } else {
+          const int r = warp * 16 + lane % 8 + lane / 16 * 8;
+          // rows past the end may hold anything, NaN too, which 0 would not cancel: keys 2c, 2c + 1 and eight on
+          uint32_t keep[2] = {~0u, ~0u};
+          if (t + 16 > t1) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              keep[i] = (t + 2 * c + 8 * i < t1 ? 0xffffu : 0u) | (t + 2 * c + 8 * i + 1 < t1 ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const int ch = 2 * kt + (lane / 8 & 1);
+            uint32_t a[4];
+            ek::ldmatrix4<true>(a, vt0 + ch / 8 * (C::KEYS * 128) + r * 128 + ((ch % 8 ^ (r & 7)) << 4));
+            mma_16x8x16(o[kt], a[0] & keep[0], a[1] & keep[0], a[2] & keep[1], a[3] & keep[1], b0, b1);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ek::mbar_arrive(empty + st);
+    }
+    if (!ok) m[0] = m[1] = l[0] = l[1] = NAN;  // a wait ran out: the result is NaN and the status is set
+  }
+  __syncthreads();  // all stages are done with
+  if (threadIdx.x == 0 && *abort) g_attention_status = 1;
+  float* s_o = reinterpret_cast<float*>(smem);  // [warp][8][D]
+  if (warp < kWarps) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      s[n] = t + j < t1 ? s[n] * p.scale_log2 : -INFINITY;
-      s[2 + n] = t + j + 8 < t1 ? s[2 + n] * p.scale_log2 : -INFINITY;
-      float top = fmaxf(s[n], s[2 + n]);
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-      const float next = fmaxf(m[n], top);
-      const float base = next == -INFINITY ? 0.f : next;
-      fix[n] = exp2_approx(m[n] - base);
-      grew |= next != m[n];
-      m[n] = next;
-      s[n] = exp2_approx(s[n] - base);
-      s[2 + n] = exp2_approx(s[2 + n] - base);
-      l[n] = l[n] * fix[n] + s[n] + s[2 + n];
-    }
-    if (grew) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(~0u, l[n], x);
+      if (j == 0) s_m[warp * 8 + 2 * c + n] = m[n], s_l[warp * 8 + 2 * c + n] = l[n];
+      float* at = s_o + (warp * 8 + 2 * c + n) * D;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        o[kt][0] *= fix[0], o[kt][1] *= fix[1];
-        o[kt][2] *= fix[0], o[kt][3] *= fix[1];
+        // 8-bit rows: lane/4 holds D / 8 consecutive dimensions
+        at[I8 ? j * (D / 8) + 2 * kt : kt * 16 + j] = o[kt][n];
+        at[I8 ? j * (D / 8) + 2 * kt + 1 : kt * 16 + j + 8] = o[kt][2 + n];
       }
-    }
-    if (I8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = s[i] == 0.f ? 0.f : s[i] * r.vs[i / 2][0];
-    }
-    // probabilities are rounded to bf16 for the product: half a step is 2^-8 of each, as for V itself
-    const uint32_t b0 = transpose_8x8(pack_bf16(s[0], s[1])), b1 = transpose_8x8(pack_bf16(s[2], s[3]));
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      uint32_t a[4];
-      if (I8) {
-        const int w = kt / 2, e = (kt % 2) * 2;  // word and first byte of element 2 kt
-        const uint32_t even = e == 0 ? 0x4400 : 0x6622, odd = e == 0 ? 0x5511 : 0x7733;
-        a[0] = codes_to_bf16(__byte_perm(r.v[0][w], r.v[1][w], even));
-        a[1] = codes_to_bf16(__byte_perm(r.v[0][w], r.v[1][w], odd));
-        a[2] = codes_to_bf16(__byte_perm(r.v[2][w], r.v[3][w], even));
-        a[3] = codes_to_bf16(__byte_perm(r.v[2][w], r.v[3][w], odd));
-      } else {
-        a[0] = __byte_perm(r.v[0][kt], r.v[1][kt], 0x5410);
-        a[1] = __byte_perm(r.v[0][kt], r.v[1][kt], 0x7632);
-        a[2] = __byte_perm(r.v[2][kt], r.v[3][kt], 0x5410);
-        a[3] = __byte_perm(r.v[2][kt], r.v[3][kt], 0x7632);
-      }
-      mma_16x8x16(o[kt], a[0], a[1], a[2], a[3], b0, b1);
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(~0u, l[n], x);
-    if (j == 0) s_m[warp][2 * c + n] = m[n], s_l[warp][2 * c + n] = l[n];
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      s_o[warp][2 * c + n][v_dim<D, I8>(j, 2 * kt)] = o[kt][n];
-      s_o[warp][2 * c + n][v_dim<D, I8>(j, 2 * kt + 1)] = o[kt][2 + n];
     }
   }
   __syncthreads();
   // join the warps
   const long long total_rows = (long long)p.batch * p.q_heads;
   const int part = (shared ? 0 : p.prefix_slots) + slot;
-  for (int i = threadIdx.x; i < 8 * D; i += kWarps * 32) {
-    const int n = i / D, d = i % D;
+  for (int i = threadIdx.x; i < 8 * (D / 4); i += kWarps * 32 + 32) {
+    const int n = i / (D / 4), d = i % (D / 4) * 4;
     int b, h;
     if (!locate(n, b, h)) continue;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][n]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * 8 + n]);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, lsum = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float lsum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2_approx(s_m[w][n] - base);
-      sum += s_o[w][n][d] * f;
-      lsum += s_l[w][n] * f;
+      const float f = exp2_approx(s_m[w * 8 + n] - base);
+      const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 8 + n) * D + d);
+      sum.x += x.x * f, sum.y += x.y * f, sum.z += x.z * f, sum.w += x.w * f;
+      lsum += s_l[w * 8 + n] * f;
     }
     const long long at = part * total_rows + (long long)b * p.q_heads + h;
-    p.part_o[at * D + d] = sum;
+    *reinterpret_cast<float4*>(p.part_o + at * D + d) = sum;
     if (d == 0) p.part_ml[at] = make_float2(top, lsum);
   }
 }
@@ -367,15 +444,13 @@ struct Many {
 };
 
 struct ManyParams {
-  CUtensorMap k, v;
+  RowMap k, v;
   AttnParams a;
-  int k_keys_first, v_keys_first;  // map dimensions: (D, key, head) instead of (D, head, key)
   int rows, wide_blocks, narrow_rows;  // rows of a KV head; blocks of 256; rows left for a narrow block
   int wide_splits, wide_tiles, narrow_splits, narrow_tiles;  // splits of the keys and 128-key tiles of each
   int negate;                   // scale < 0: q is negated and |scale| used
 };
 
-__device__ int g_attention_status;
 
 // Columns from `keys` on of 32 scores become -inf.
 __device__ __forceinline__ void mask_tail(uint32_t (&x)[32], int keys) {
@@ -689,12 +764,11 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         slot(n, is_v, tile, f, e, round, to);
         if (round > 0 && !wait(e, (round - 1) & 1)) break;
         const int key = (tile0 + tile) * 128;
-        const CUtensorMap* map = is_v ? &p.v : &p.k;
-        const bool keys_first = is_v ? p.v_keys_first : p.k_keys_first;
+        const RowMap& map = is_v ? p.v : p.k;
         if (ek::elect_one()) {
           ek::mbar_arrive_expect_tx(f, BYTES);
           for (int blk = 0; blk < (I8 ? 1 : C::BLOCKS); ++blk)
-            ek::tma_load_3d(to + blk * 16384, map, blk * 64, keys_first ? key : head, keys_first ? head : key, f);
+            map.load(to + blk * 16384, blk * 64, head, key, 0, f);
         }
         __syncwarp();
       }
@@ -773,38 +847,57 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 }
 
 // ---------------------------------------------------------------------------
-// One warp per (sequence, query head) joins its items.
+// One warp per (sequence, query head) joins its items: lane i takes the maximum and sum of item i (32 at a time), then
+// the lanes go through the rows of O with 16-byte loads, two items (D = 64) or one at a time.
 template <int D>
 __global__ void __launch_bounds__(128) join(const AttnParams p) {
+  constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
   const long long row = blockIdx.x * 4ll + threadIdx.x / 32, rows = (long long)p.batch * p.q_heads;
-  const int lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32, sub = lane / LANES, piece = lane % LANES;
   if (row >= rows) return;
   const int b = (int)(row / p.q_heads), h = (int)(row % p.q_heads);
   const int len = min(max(p.own_lens[b], 0), p.max_own);
   const int shared = b * p.group + h % p.group < p.wide_rows ? p.wide_slots : p.narrow_slots;
   const int parts = shared + (len + p.own_chunk - 1) / p.own_chunk;
   auto place = [&](int i) { return (long long)(i < shared ? i : i - shared + p.prefix_slots) * rows + row; };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
+  float top = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    const int n = min(32, parts - i0);
+    const float2 ml = lane < n ? __ldg(p.part_ml + place(i0 + lane)) : make_float2(-INFINITY, 0.f);
+    float next = ml.x;
 #pragma unroll
-  for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-  const float base = top == -INFINITY ? 0.f : top;
-  float o[D / 32] = {}, l = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const long long at = place(i);
-    const float2 ml = p.part_ml[at];
-    if (ml.y == 0.f) continue;  // an item without keys has no o
-    const float f = exp2_approx(ml.x - base);
-    l += ml.y * f;
+    for (int x = 16; x; x >>= 1) next = fmaxf(next, __shfl_xor_sync(~0u, next, x));
+    next = fmaxf(next, top);
+    const float base = next == -INFINITY ? 0.f : next, old = exp2_approx(top - base);
+    top = next;
+    // an item without keys has no o
+    const float f = ml.y == 0.f ? 0.f : exp2_approx(ml.x - base);
+    float sum = f == 0.f ? 0.f * ml.y : f * ml.y;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[e] += f * p.part_o[at * D + lane * (D / 32) + e];
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+    l = l * old + sum;
+    o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+    const unsigned holds = __ballot_sync(~0u, lane < n && ml.y != 0.f);
+#pragma unroll 4
+    for (int i = 0; i < n; i += AT_ONCE) {
+      const int k = i + sub;
+      const float fk = __shfl_sync(~0u, f, k & 31);
+      if (k < n && (holds >> k & 1)) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(p.part_o + place(i0 + k) * D) + piece);
+        o.x += fk * x.x, o.y += fk * x.y, o.z += fk * x.z, o.w += fk * x.w;
+      }
+    }
+  }
+  if (AT_ONCE == 2) {
+    o.x += __shfl_xor_sync(~0u, o.x, 16), o.y += __shfl_xor_sync(~0u, o.y, 16);
+    o.z += __shfl_xor_sync(~0u, o.z, 16), o.w += __shfl_xor_sync(~0u, o.w, 16);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: zeros
-  __nv_bfloat16* out = p.out + b * p.out_batch + h * p.out_head + lane * (D / 32);
-#pragma unroll
-  for (int e = 0; e < D / 32; e += 2)
-    *reinterpret_cast<uint32_t*>(out + e) = pack_bf16(o[e] * inv, o[e + 1] * inv);
-  if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+  if (sub == 0)
+    *reinterpret_cast<uint2*>(p.out + b * p.out_batch + h * p.out_head + piece * 4) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) * 0.6931471805599453f + logf(l);
 }
 
 int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -819,10 +912,6 @@ struct Plan {
 
 // Query rows of a KV head from which many_rows takes the prefix.
 constexpr int kManyRows = 17;
-
-bool has_zero_stride(const EkKvTensor& t, int rows, int heads) {
-  return (rows > 1 && t.stride_row == 0) || (heads > 1 && t.stride_head == 0);
-}
 
 int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   using ek::fail;
@@ -851,8 +940,7 @@ int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   const long long own = (long long)a->batch * div_up(group, 8) * a->kv_heads;
   pl.own_chunk = chunk(a->max_own_len, own > 0 ? own : 1);
   pl.own_slots = div_up(a->max_own_len, pl.own_chunk);
-  pl.many = rows >= kManyRows && a->prefix_len > 0 && !has_zero_stride(a->prefix_k, a->prefix_len, a->kv_heads) &&
-            !has_zero_stride(a->prefix_v, a->prefix_len, a->kv_heads);
+  pl.many = rows >= kManyRows && a->prefix_len > 0;
   if (!pl.many) {
     const long long tiles = (long long)div_up(rows, 8) * a->kv_heads;
     pl.prefix_chunk = chunk(a->prefix_len, tiles > 0 ? tiles : 1);
@@ -880,26 +968,45 @@ int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   return EK_SUCCESS;
 }
 
-// Map of the prefix rows of all heads: boxes of 128 keys of one head, 64 bf16 values (128-byte swizzle) or
-// `d` codes wide. The smaller stride comes first. Keys past the end read as zeros.
-int encode_prefix(CUtensorMap* m, const EkKvTensor& t, int keys, int heads, int d, bool i8, int* keys_first) {
+// Map of rows [batch][rows][heads][d]: copies of `box` rows of one head, 64 bf16 values (128-byte swizzle) or `d` codes
+// wide. Rows past the end read as zeros.
+int encode_rows(RowMap& m, const EkKvTensor& t, int batch, int rows, int heads, int d, bool i8, int box,
+                CUtensorMapSwizzle swizzle) {
   ek::EncodeTiledFn enc = ek::get_encoder();
   if (!enc) return ek::fail(EK_E_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const long long size = i8 ? 1 : 2;
-  long long row = t.stride_row * size, head = t.stride_head * size;
-  if (heads == 1) head = d * size;
-  if (keys == 1) row = head * heads;
-  *keys_first = row < head;
-  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)(*keys_first ? keys : heads),
-                              (cuuint64_t)(*keys_first ? heads : keys)};
-  const cuuint64_t strides[2] = {(cuuint64_t)(*keys_first ? row : head), (cuuint64_t)(*keys_first ? head : row)};
-  const cuuint32_t box[3] = {(cuuint32_t)(i8 ? d : 64), *keys_first ? 128u : 1u, *keys_first ? 1u : 128u};
-  const cuuint32_t steps[3] = {1, 1, 1};
-  const CUresult r = enc(m, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, t.data, dims,
-                         strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+  struct Dim {
+    long long n, stride;
+    int8_t* place;
+    bool rows;
+  } dims[3] = {{heads, t.stride_head * size, &m.head, false},
+               {rows, t.stride_row * size, &m.row, true},
+               {batch, t.stride_batch * size, &m.batch, false}};
+  long long widest = d * size;
+  for (Dim& x : dims) {
+    if (x.n == 1 || x.stride == 0) x.n = 1, x.stride = 0;  // not there; a repeated row needs one entry only
+    if (x.stride > widest) widest = x.stride;
+  }
+  for (Dim& x : dims)
+    if (x.n == 1) x.stride = widest;
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (dims[j].stride > dims[j + 1].stride) {
+        const Dim x = dims[j];
+        dims[j] = dims[j + 1], dims[j + 1] = x;
+      }
+  cuuint64_t sizes[4] = {(cuuint64_t)d}, strides[3];
+  cuuint32_t boxes[4] = {(cuuint32_t)(i8 ? d : 64)};
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    *dims[i].place = dims[i].n == 1 ? -1 : i;
+    sizes[i + 1] = (cuuint64_t)dims[i].n, strides[i] = (cuuint64_t)dims[i].stride;
+    boxes[i + 1] = dims[i].rows ? box : 1;
+  }
+  const CUresult r = enc(&m.map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data, sizes,
+                         strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return ek::fail(EK_E_INVALID, "tensor map of the prefix failed (CUresult %d)", (int)r);
+  if (r != CUDA_SUCCESS) return ek::fail(EK_E_INVALID, "tensor map of K or V rows failed (CUresult %d)", (int)r);
   return EK_SUCCESS;
 }
 
@@ -940,17 +1047,19 @@ int take_store(const EkKvTensor& k, const EkKvTensor& v, bool rows, bool i8, con
 }
 
 template <int D, bool I8>
-cudaError_t launch(const AttnParams& p, const ManyParams* many, cudaStream_t st) {
+cudaError_t launch(const FewParams& p, const ManyParams* many, cudaStream_t st) {
   cudaError_t e;
   if (many && (e = launch_many<D, I8>(*many, st)) != cudaSuccess) return e;
-  AttnParams few = p;
-  if (many) few.prefix_tiles = 0;  // the prefix is taken care of
-  const long long items = (long long)few.prefix_slots * few.prefix_tiles * few.kv_heads +
-                          (long long)few.own_slots * few.group_tiles * few.kv_heads * few.batch;
+  const long long items = (long long)p.a.prefix_slots * p.a.prefix_tiles * p.a.kv_heads +
+                          (long long)p.a.own_slots * p.a.group_tiles * p.a.kv_heads * p.a.batch;
   if (items > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  if (items > 0) few_rows<D, I8><<<(unsigned)items, kWarps * 32, 0, st>>>(few);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  join<D><<<div_up((long long)p.batch * p.q_heads, 4), 128, 0, st>>>(p);
+  if (items > 0) {
+    e = cudaFuncSetAttribute(few_rows<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, I8>::SMEM);
+    if (e != cudaSuccess) return e;
+    few_rows<D, I8><<<(unsigned)items, kWarps * 32 + 32, Few<D, I8>::SMEM, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  join<D><<<div_up((long long)p.a.batch * p.a.q_heads, 4), 128, 0, st>>>(p.a);
   return cudaGetLastError();
 }
 
@@ -975,7 +1084,8 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
   if (pl.part_bytes > 0 && (!a->workspace || !ek::aligned16(a->workspace) || a->workspace_bytes < pl.part_bytes))
     return fail(EK_E_INVALID, "workspace of %lld bytes, 16-byte aligned, needed", pl.part_bytes);
   const bool i8 = (a->prefix_len > 0 ? a->prefix_k.scales : a->own_k.scales) != nullptr;
-  AttnParams p;
+  FewParams few;
+  AttnParams& p = few.a;
   if ((rc = take_store(a->prefix_k, a->prefix_v, a->prefix_len > 0, i8, "prefix", p.prefix))) return rc;
   if ((rc = take_store(a->own_k, a->own_v, a->max_own_len > 0, i8, "own", p.own))) return rc;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -998,10 +1108,21 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
   p.wide_slots = pl.wide_splits;
   p.narrow_slots = pl.many ? 2 * pl.narrow_splits : pl.prefix_slots;
   p.scale_log2 = a->scale * kLog2e;
+  const int d = a->head_dim;
+  const CUtensorMapSwizzle wide_rows = CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUtensorMapSwizzle few_swizzle = i8 && d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : wide_rows;
+  auto encode = [&](RowMap& k, RowMap& v, const EkKvTensor& tk, const EkKvTensor& tv, int batch, int rows, int box,
+                    CUtensorMapSwizzle swizzle) {
+    const int r = encode_rows(k, tk, batch, rows, a->kv_heads, d, i8, box, swizzle);
+    return r ? r : encode_rows(v, tv, batch, rows, a->kv_heads, d, i8, box, swizzle);
+  };
+  constexpr int kBox = Few<64, false>::BOX;
+  if (a->max_own_len > 0 &&
+      (rc = encode(few.own_k, few.own_v, a->own_k, a->own_v, a->batch, a->own_capacity, kBox, few_swizzle)))
+    return rc;
   ManyParams m;
   if (pl.many) {
-    if ((rc = encode_prefix(&m.k, a->prefix_k, a->prefix_len, a->kv_heads, a->head_dim, i8, &m.k_keys_first)) ||
-        (rc = encode_prefix(&m.v, a->prefix_v, a->prefix_len, a->kv_heads, a->head_dim, i8, &m.v_keys_first)))
+    if ((rc = encode(m.k, m.v, a->prefix_k, a->prefix_v, 1, a->prefix_len, 128, i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : wide_rows)))
       return rc;
     m.a = p;
     m.rows = a->batch * p.group;
@@ -1011,13 +1132,17 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
     // masked scores are -inf times the scale, so it is kept positive; 1e-30 stands for 0
     m.negate = p.scale_log2 < 0.f;
     m.a.scale_log2 = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
+    p.prefix_tiles = 0;  // nothing of the prefix is left for few_rows
+  } else if (a->prefix_len > 0 &&
+             (rc = encode(few.prefix_k, few.prefix_v, a->prefix_k, a->prefix_v, 1, a->prefix_len, kBox, few_swizzle))) {
+    return rc;
   }
   const ManyParams* many = pl.many ? &m : nullptr;
   ek::DeviceGuard g(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (a->head_dim == 64) e = i8 ? launch<64, true>(p, many, st) : launch<64, false>(p, many, st);
-  else e = i8 ? launch<128, true>(p, many, st) : launch<128, false>(p, many, st);
+  if (a->head_dim == 64) e = i8 ? launch<64, true>(few, many, st) : launch<64, false>(few, many, st);
+  else e = i8 ? launch<128, true>(few, many, st) : launch<128, false>(few, many, st);
   return e == cudaSuccess ? EK_SUCCESS : ek::cuda_fail(e, "ek_prefix_attention launch");
 }
 
