@@ -60,6 +60,10 @@ struct AttnParams {
   float scale_log2;
 };
 
+// Programmatic launches: the next kernel of the stream may start; the one before has ended and its writes are visible.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -131,6 +135,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_consta
   using C = Few<D, I8>;
   constexpr int KT = D / 16;  // 16-wide steps over the dimensions
   const AttnParams& p = fp.a;
+  launch_next();
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* empty = full + C::STAGES;
@@ -466,6 +471,7 @@ __device__ __forceinline__ uint64_t score_pair(const uint32_t (&x)[32], int e) {
 template <int D, bool I8>
 __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __grid_constant__ ManyParams p) {
   using C = Many<D, I8>;
+  launch_next();
   extern __shared__ __align__(1024) uint8_t smem[];  // atoms of the swizzle start on 1024 bytes
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* k_empty = k_full + C::KS;
@@ -521,6 +527,9 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   };
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // for a whole warp, which goes on or gives up together
     return __all_sync(~0u, ek::mbar_wait_bounded(bar, parity, abort)) != 0;
+  };
+  auto spin = [&](uint64_t* bar, uint32_t parity) {  // where the softmax or the tensor core would stand still
+    return __all_sync(~0u, ek::mbar_wait_bounded<true>(bar, parity, abort)) != 0;
   };
   // One arrival per warp: 128 on one barrier are serialised.
   auto arrive = [&](uint64_t* bar) {
@@ -590,11 +599,11 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         ks = sc, vs = sc + 128;
         next_ks = key_scale(use + 1, 0), next_vs = key_scale(use + 1, 1);
       }
-      if (!(ok = wait(s_full + w, use & 1))) break;
+      if (!(ok = spin(s_full + w, use & 1))) break;
       ek::tcgen05_after_sync();
       if (idle) {
         arrive(s_empty);
-        if (use > 0 && !(ok = wait(p_empty + w, (use - 1) & 1))) break;
+        if (use > 0 && !(ok = spin(p_empty + w, (use - 1) & 1))) break;
       } else {
         uint32_t x[4][32];
 #pragma unroll
@@ -632,7 +641,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         const float grown = ek::max3_nan(m, high, high);
         if (use == 0) m = grown;
         // O and P are free once the products of the tile before are done
-        if (use > 0 && !(ok = wait(p_empty + w, (use - 1) & 1))) break;
+        if (use > 0 && !(ok = spin(p_empty + w, (use - 1) & 1))) break;
         ek::tcgen05_after_sync();
         const bool far = grown > m + 8.f || grown != grown;
         if (__any_sync(~0u, far)) {
@@ -797,7 +806,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         // S = Q K^T of product i, once the scores before it have been taken
         for (int i = 0; i < count && (i > 0 || wait(q_full, 0)); ++i) {
           const int w = i % 2, t = wide ? i / 2 : i;
-          if (!wait(k_full + t % C::KS, (t / C::KS) & 1) || (i > 0 && !wait(s_empty, (i - 1) & 1))) break;
+          if (!spin(k_full + t % C::KS, (t / C::KS) & 1) || (i > 0 && !spin(s_empty, (i - 1) & 1))) break;
           ek::tcgen05_after_sync();
           const uint32_t base = ek::smem_u32(smem);
           const uint32_t q = base + (wide ? w * C::TILE : 0), k = base + C::OFF_K + t % C::KS * C::TILE;
@@ -816,7 +825,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         // O += P V of product i
         for (int i = 0; i < count; ++i) {
           const int w = i % 2, t = wide ? i / 2 : i;
-          if (!wait(v_full + t % C::VS, (t / C::VS) & 1) || !wait(p_full + w, (i / 2) & 1)) break;
+          if (!spin(v_full + t % C::VS, (t / C::VS) & 1) || !spin(p_full + w, (i / 2) & 1)) break;
           ek::tcgen05_after_sync();
           const uint32_t v = ek::smem_u32(smem) + C::OFF_V + t % C::VS * C::TILE;
           if (ek::elect_one()) {
@@ -838,6 +847,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     }
   }
   __syncwarp();
+  wait_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort) g_attention_status = 1;
   if (warp == C::SCORES) {
@@ -852,6 +862,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 template <int D>
 __global__ void __launch_bounds__(128) join(const AttnParams p) {
   constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
+  wait_before();
   const long long row = blockIdx.x * 4ll + threadIdx.x / 32, rows = (long long)p.batch * p.q_heads;
   const int lane = threadIdx.x % 32, sub = lane / LANES, piece = lane % LANES;
   if (row >= rows) return;
@@ -864,7 +875,7 @@ __global__ void __launch_bounds__(128) join(const AttnParams p) {
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < parts; i0 += 32) {
     const int n = min(32, parts - i0);
-    const float2 ml = lane < n ? __ldg(p.part_ml + place(i0 + lane)) : make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < n ? __ldcg(p.part_ml + place(i0 + lane)) : make_float2(-INFINITY, 0.f);
     float next = ml.x;
 #pragma unroll
     for (int x = 16; x; x >>= 1) next = fmaxf(next, __shfl_xor_sync(~0u, next, x));
@@ -884,7 +895,7 @@ __global__ void __launch_bounds__(128) join(const AttnParams p) {
       const int k = i + sub;
       const float fk = __shfl_sync(~0u, f, k & 31);
       if (k < n && (holds >> k & 1)) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(p.part_o + place(i0 + k) * D) + piece);
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + place(i0 + k) * D) + piece);
         o.x += fk * x.x, o.y += fk * x.y, o.z += fk * x.z, o.w += fk * x.w;
       }
     }
@@ -1010,21 +1021,6 @@ int encode_rows(RowMap& m, const EkKvTensor& t, int batch, int rows, int heads, 
   return EK_SUCCESS;
 }
 
-template <int D, bool I8>
-cudaError_t launch_many(const ManyParams& p, cudaStream_t st) {
-  static_assert(Many<D, I8>::SMEM <= 227 * 1024, "shared memory");
-  cudaError_t e =
-      cudaFuncSetAttribute(many_rows<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<D, I8>::SMEM);
-  if (e != cudaSuccess) return e;
-  // the warpgroups take more registers out of those that the block is launched with
-  cudaFuncAttributes attr;
-  if ((e = cudaFuncGetAttributes(&attr, many_rows<D, I8>)) != cudaSuccess) return e;
-  if (attr.numRegs != Many<D, I8>::REGS) return cudaErrorLaunchOutOfResources;
-  const int items = (p.wide_blocks * p.wide_splits + (p.narrow_rows ? p.narrow_splits : 0)) * p.a.kv_heads;
-  many_rows<D, I8><<<items, Many<D, I8>::WARPS * 32, Many<D, I8>::SMEM, st>>>(p);
-  return cudaGetLastError();
-}
-
 // Fills one side of `s`; checks alignment and kind when there are rows.
 int take_store(const EkKvTensor& k, const EkKvTensor& v, bool rows, bool i8, const char* name, Store& s) {
   using ek::fail;
@@ -1046,21 +1042,49 @@ int take_store(const EkKvTensor& k, const EkKvTensor& v, bool rows, bool i8, con
   return EK_SUCCESS;
 }
 
+// Launches `kernel`; `overlap`: it may start while the launch before it in the stream still runs (once all of that
+// one's blocks have passed launch_next or ended), and waits for its results itself.
+template <typename P>
+cudaError_t start(void (*kernel)(P), const P& p, long long blocks, int threads, int bytes, bool overlap, cudaStream_t st) {
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  cudaError_t e;
+  if (bytes > 48 * 1024 &&
+      (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess)
+    return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// few_rows, then many_rows beside it, then join. The first is an ordinary launch, so what ran before is done when any
+// of them reads; many_rows reads nothing of few_rows and ends after it (wait_before), join waits for many_rows.
 template <int D, bool I8>
 cudaError_t launch(const FewParams& p, const ManyParams* many, cudaStream_t st) {
+  using M = Many<D, I8>;
+  static_assert(M::SMEM <= 227 * 1024 && Few<D, I8>::SMEM <= 227 * 1024, "shared memory");
   cudaError_t e;
-  if (many && (e = launch_many<D, I8>(*many, st)) != cudaSuccess) return e;
   const long long items = (long long)p.a.prefix_slots * p.a.prefix_tiles * p.a.kv_heads +
                           (long long)p.a.own_slots * p.a.group_tiles * p.a.kv_heads * p.a.batch;
-  if (items > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  if (items > 0) {
-    e = cudaFuncSetAttribute(few_rows<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, I8>::SMEM);
-    if (e != cudaSuccess) return e;
-    few_rows<D, I8><<<(unsigned)items, kWarps * 32 + 32, Few<D, I8>::SMEM, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (items > 0 &&
+      (e = start(few_rows<D, I8>, p, items, kWarps * 32 + 32, Few<D, I8>::SMEM, false, st)) != cudaSuccess)
+    return e;
+  if (many) {
+    // the warpgroups take more registers out of those that the block is launched with
+    cudaFuncAttributes attr;
+    if ((e = cudaFuncGetAttributes(&attr, many_rows<D, I8>)) != cudaSuccess) return e;
+    if (attr.numRegs != M::REGS) return cudaErrorLaunchOutOfResources;
+    const int blocks = (many->wide_blocks * many->wide_splits + (many->narrow_rows ? many->narrow_splits : 0)) * p.a.kv_heads;
+    if ((e = start(many_rows<D, I8>, *many, blocks, M::WARPS * 32, M::SMEM, items > 0, st)) != cudaSuccess) return e;
   }
-  join<D><<<div_up((long long)p.a.batch * p.a.q_heads, 4), 128, 0, st>>>(p.a);
-  return cudaGetLastError();
+  return start(join<D>, p.a, div_up((long long)p.a.batch * p.a.q_heads, 4), 128, 0, items > 0 || many, st);
 }
 
 }  // namespace

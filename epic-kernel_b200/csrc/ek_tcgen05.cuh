@@ -221,12 +221,13 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // ---------------------------------------------------------------- bounded wait
 // Waits for phase `parity` of `bar`. False once *abort is set, by this wait
 // after about two seconds or by another one.
+// SPIN: the thread is not suspended (a suspended one takes some 300 cycles to come back) but takes issue slots.
+template <bool SPIN = false>
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort) {
   uint64_t t0 = 0;
   for (;;) {
-    // test_wait does not suspend the thread: a suspended one takes some 300 cycles to come back
-    for (int i = 0; i < 1024; ++i)
-      if (mbar_test_wait(bar, parity)) return true;
+    for (int i = 0; i < (SPIN ? 1024 : 64); ++i)
+      if (SPIN ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
     uint64_t now;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
