@@ -5,14 +5,13 @@
 // |x| / s <= 127. s has 8 significant bits, as x has, so x / s is either
 // exactly half an integer or at least 1/1020 away from one: 2|x| = (2k + 1) s
 // compares two integers below 2^9 * 2^8 over a common exponent. Adding 2^-12
-// to |x| * (1 / s) (fp32, error below 2^-16) and truncating after + 1/2
-// therefore gives the exact half-away-from-zero code without a division per
-// element.
+// to |x| * (1 / s) (fp32, error below 2^-16) and rounding to nearest therefore
+// gives the exact half-away-from-zero code without a division per element.
 //
 // Bound: bytes (2 B in and 1 B out per element for a write, the reverse for a
 // read, plus 2 B of scale per head). A thread moves 16 elements (two 16-byte
-// loads, one 16-byte store), so 4 (D = 64) or 8 (D = 128) lanes share a head
-// and one maximum needs 2 or 3 shuffles.
+// loads, one 16-byte store) of each of two heads, loaded together, so 4 (D =
+// 64) or 8 (D = 128) lanes share a head and one maximum needs 2 or 3 shuffles.
 #include <cuda_bf16.h>
 
 #include "ek_host.h"
@@ -27,77 +26,89 @@ struct CopyParams {
 };
 
 constexpr int kThreads = 256;
+constexpr int kUnroll = 2;
 
-// Rows of one sequence: blockIdx.x over (row, head), blockIdx.y the sequence, blockIdx.z K or V.
+// Heads of one sequence: blockIdx.x over (row, head), kUnroll * kThreads / LANES of them, blockIdx.y the sequence,
+// blockIdx.z K or V.
 template <int D, bool WRITE>
 __global__ void __launch_bounds__(kThreads) kv_copy(const CopyParams p) {
-  constexpr int LANES = D / 16;
-  const int b = blockIdx.y, kv = blockIdx.z;
-  const long long at = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  const int lane = threadIdx.x % LANES;
-  const bool live = at < (long long)p.length * p.heads;
-  const int i = live ? (int)(at / p.heads) : 0, h = live ? (int)(at % p.heads) : 0;
-  const long long row = (p.start ? (long long)p.start[b] : p.start_all) + i;
-  const bool inside = live && row >= 0 && row < p.capacity;
+  constexpr int LANES = D / 16, PER_BLOCK = kThreads / LANES;
+  const int b = blockIdx.y, kv = blockIdx.z, lane = threadIdx.x % LANES;
   const EkKvTensor& x = p.values[kv];
   const EkKvTensor& c = p.cache[kv];
-  __nv_bfloat16* value = static_cast<__nv_bfloat16*>(x.data) + b * x.stride_batch + i * x.stride_row +
-                         h * x.stride_head + lane * 16;
-  int8_t* code = static_cast<int8_t*>(c.data) + b * c.stride_batch + row * c.stride_row + h * c.stride_head + lane * 16;
-  __nv_bfloat16* scale = static_cast<__nv_bfloat16*>(c.scales) + b * c.scale_stride_batch +
-                         row * c.scale_stride_row + h * c.scale_stride_head;
-  if (WRITE) {
-    uint32_t w[8] = {};
-    if (inside) {
-      const uint4 lo = __ldg(reinterpret_cast<const uint4*>(value));
-      const uint4 hi = __ldg(reinterpret_cast<const uint4*>(value) + 1);
-      w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
+  const long long start = p.start ? (long long)p.start[b] : p.start_all;
+  __nv_bfloat16* value[kUnroll];
+  int8_t* code[kUnroll];
+  __nv_bfloat16* scale[kUnroll];
+  bool live[kUnroll], inside[kUnroll];
+  uint4 lo[kUnroll], hi[kUnroll];
+  float s[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const unsigned at = (blockIdx.x * kUnroll + u) * PER_BLOCK + threadIdx.x / LANES;
+    live[u] = at < (unsigned)p.length * (unsigned)p.heads;
+    const unsigned i = at / (unsigned)p.heads, h = at - i * (unsigned)p.heads;
+    const long long row = start + i;
+    inside[u] = live[u] && row >= 0 && row < p.capacity;
+    value[u] = static_cast<__nv_bfloat16*>(x.data) + b * x.stride_batch + i * x.stride_row + h * x.stride_head + lane * 16;
+    code[u] = static_cast<int8_t*>(c.data) + b * c.stride_batch + row * c.stride_row + h * c.stride_head + lane * 16;
+    scale[u] = static_cast<__nv_bfloat16*>(c.scales) + b * c.scale_stride_batch + row * c.scale_stride_row +
+               h * c.scale_stride_head;
+    lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+    s[u] = 0.f;
+    if (!inside[u]) continue;
+    if (WRITE) {
+      lo[u] = __ldg(reinterpret_cast<const uint4*>(value[u]));
+      hi[u] = __ldg(reinterpret_cast<const uint4*>(value[u]) + 1);
+    } else {
+      lo[u] = __ldg(reinterpret_cast<const uint4*>(code[u]));
+      s[u] = __bfloat162float(*scale[u]);
     }
-    // |x| as integers: NaN > inf > finite
-    unsigned top = 0;
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, max(w[j] << 16 & 0x7fff0000u, w[j] & 0x7fff0000u));
+  for (int u = 0; u < kUnroll; ++u) {
+    uint32_t w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+    if (WRITE) {
+      // |x| as integers: NaN > inf > finite
+      unsigned tops = 0;
 #pragma unroll
-    for (int m = LANES / 2; m; m >>= 1) top = max(top, __shfl_xor_sync(~0u, top, m));
-    const bool finite = top < 0x7f800000u;
-    unsigned s = (__float_as_uint(__uint_as_float(top) / 127.f) + 0xffffu) & 0xffff0000u;
-    s = finite ? max(s, 0x00800000u) : 0x7fff0000u;
-    const float inv = finite ? 1.f / __uint_as_float(s) : 0.f;
-    if (!inside) return;
-    uint32_t out[4];
+      for (int j = 0; j < 8; ++j) tops = __vmaxu2(tops, w[j] & 0x7fff7fffu);
+      unsigned top = max(tops << 16, tops & 0xffff0000u);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t packed = 0;
+      for (int m = LANES / 2; m; m >>= 1) top = max(top, __shfl_xor_sync(~0u, top, m));
+      const bool finite = top < 0x7f800000u;
+      unsigned t = (__float_as_uint(__uint_as_float(top) / 127.f) + 0xffffu) & 0xffff0000u;
+      t = finite ? max(t, 0x00800000u) : 0x7fff0000u;
+      const float inv = finite ? 1.f / __uint_as_float(t) : 0.f;
+      if (!inside[u]) continue;
+      // x / s moved 2^-12 away from zero, then to the nearest whole number by an addition of 1.5 * 2^23: the low byte
+      uint32_t out[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t u = e & 1 ? w[2 * j + e / 2] & 0xffff0000u : w[2 * j + e / 2] << 16;
-        const float a = __uint_as_float(u & 0x7fffffffu);
-        int q = finite ? (int)(a * inv + (0.5f + 0x1p-12f)) : 0;
-        q = u & 0x80000000u ? -q : q;
-        packed |= (uint32_t)(q & 0xff) << (8 * e);
+      for (int j = 0; j < 4; ++j) {
+        uint32_t z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t pair = finite ? w[2 * j + e / 2] : 0u;
+          const uint32_t v = e & 1 ? pair & 0xffff0000u : pair << 16;
+          const float away = __uint_as_float((v & 0x80000000u) | 0x39800000u);
+          z[e] = __float_as_uint(fmaf(__uint_as_float(v), inv, away) + 12582912.f);
+        }
+        out[j] = __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410);
       }
-      out[j] = packed;
-    }
-    *reinterpret_cast<uint4*>(code) = make_uint4(out[0], out[1], out[2], out[3]);
-    if (lane == 0) *scale = __ushort_as_bfloat16((unsigned short)(s >> 16));
-  } else {
-    if (!live) return;
-    uint4 c16 = make_uint4(0, 0, 0, 0);
-    float s = 0.f;
-    if (inside) {
-      c16 = __ldg(reinterpret_cast<const uint4*>(code));
-      s = __bfloat162float(*scale);
-    }
-    const uint32_t w[4] = {c16.x, c16.y, c16.z, c16.w};
-    uint32_t out[8];
+      *reinterpret_cast<uint4*>(code[u]) = make_uint4(out[0], out[1], out[2], out[3]);
+      if (lane == 0) *scale[u] = __ushort_as_bfloat16((unsigned short)(t >> 16));
+    } else if (live[u]) {
+      uint32_t out[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t u = w[j / 2] >> (16 * (j & 1));
-      const __nv_bfloat162 r = __floats2bfloat162_rn((float)(int8_t)(u & 0xff) * s, (float)(int8_t)(u >> 8 & 0xff) * s);
-      out[j] = *reinterpret_cast<const uint32_t*>(&r);
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t v = w[j / 2] >> (16 * (j & 1));
+        const __nv_bfloat162 r =
+            __floats2bfloat162_rn((float)(int8_t)(v & 0xff) * s[u], (float)(int8_t)(v >> 8 & 0xff) * s[u]);
+        out[j] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+      reinterpret_cast<uint4*>(value[u])[0] = make_uint4(out[0], out[1], out[2], out[3]);
+      reinterpret_cast<uint4*>(value[u])[1] = make_uint4(out[4], out[5], out[6], out[7]);
     }
-    reinterpret_cast<uint4*>(value)[0] = make_uint4(out[0], out[1], out[2], out[3]);
-    reinterpret_cast<uint4*>(value)[1] = make_uint4(out[4], out[5], out[6], out[7]);
   }
 }
 
@@ -132,9 +143,9 @@ int copy(const EkKvCopyArgs* a, void* stream, bool write) {
   p.length = a->length;
   p.capacity = a->capacity;
   p.heads = a->kv_heads;
-  const int per_block = kThreads / (a->head_dim / 16);
+  const int per_block = kUnroll * kThreads / (a->head_dim / 16);
   const long long blocks = ((long long)a->length * a->kv_heads + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffll) return fail(EK_E_UNSUPPORTED, "too many rows");
+  if ((long long)a->length * a->kv_heads > 0x7fffffffll) return fail(EK_E_UNSUPPORTED, "length * kv_heads beyond 2^31");
   ek::DeviceGuard g(a->device);
   const dim3 grid((unsigned)blocks, a->batch, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
