@@ -117,6 +117,9 @@ int grow(EkContext* ctx, size_t counters, size_t partials) {
   return EK_SUCCESS;
 }
 
+// Loads the fixed arrays of the allocation-free entry point (the driver allocates them with this file's module).
+void load_static_arrays();
+
 }  // namespace
 
 extern "C" {
@@ -144,6 +147,7 @@ int ek_context_create(int device, EkContext** out) {
     delete ctx;
     return cuda_fail(e, "cudaMemset(status)");
   }
+  load_static_arrays();  // now, so that a later ek_llama_decode_static does not allocate them
   *out = ctx;
   return EK_SUCCESS;
 }
@@ -409,6 +413,11 @@ struct StaticScratch {
 
 std::mutex g_static_mu;
 StaticScratch g_static[kMaxDevices];
+
+void load_static_arrays() {
+  void* at = nullptr;
+  if (cudaGetSymbolAddress(&at, g_static_status) != cudaSuccess) cudaGetLastError();
+}
 
 }  // namespace
 
