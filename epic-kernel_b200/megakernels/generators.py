@@ -6,15 +6,58 @@ token into `hidden_states`, reset the barrier counters, zero the logits, launch
 the megakernel, and take the argmax of the logits, all on the current stream
 with no host synchronisation. With an interpreter that supports the fused
 step (the Llama engine), the gather and the argmax run inside the megakernel
-and a step is one barrier reset plus one launch.
+and a step is one barrier reset plus one launch. With `sampling`, the token is
+drawn from the logits (`ops.sample_tokens`) instead of their argmax.
+
+`ParallelGenerator` decodes several continuations of one prompt at once: the
+prompt's K/V rows are kept once and shared (`ops.shared_prefix_attention`), in
+bf16 or in 8 bits (`ops.KVCacheInt8`). Any continuation can be handed back to
+the model's cache, to go on with the megakernel at batch 1.
 """
+
+from dataclasses import dataclass
 
 import torch
 from torch import Tensor
 
+from megakernels import ops
 from megakernels.mk import MK_Interpreter
 from megakernels.model_types import BatchState
 from megakernels.scheduler import Schedule
+
+
+@dataclass
+class SamplingParams:
+    """How tokens are drawn from the logits (see `ops.sample_tokens`). `generator`
+    is the torch generator of the random numbers, on the logits' device; None
+    uses torch's default one. temperature 0 takes the largest logit."""
+
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    generator: torch.Generator | None = None
+
+
+class _Sampler:
+    """Draws tokens with the random numbers of a generator, which are made for many steps at once."""
+
+    STEPS = 256
+
+    def __init__(self, params: SamplingParams, rows: int):
+        self.params = params
+        self.rows = rows
+        self.step = self.STEPS
+
+    def __call__(self, logits: Tensor, out: Tensor | None = None) -> Tensor:
+        p = self.params
+        if self.step == self.STEPS:
+            self.uniforms = torch.rand((self.STEPS, self.rows), generator=p.generator, device=logits.device)
+            self.step = 0
+        u = self.uniforms[self.step]
+        self.step += 1
+        return ops.sample_tokens(logits, u, temperature=p.temperature, top_k=p.top_k, top_p=p.top_p, min_p=p.min_p,
+                                 out=out)
 
 
 class Generator:
@@ -39,13 +82,15 @@ class Generator:
 
 class MK_Generator(Generator):
     def __init__(self, model, interpreter: MK_Interpreter, schedule: Schedule,
-                 barrier_fill_val: int = 0, skip_mk: bool = False, skip_rest: bool = False):
+                 barrier_fill_val: int = 0, skip_mk: bool = False, skip_rest: bool = False,
+                 sampling: SamplingParams | None = None):
         self.model = model
         self.interpreter = interpreter
         self.schedule = schedule
         self.barrier_fill_val = barrier_fill_val
         self.skip_mk = skip_mk
         self.skip_rest = skip_rest
+        self.sampler = _Sampler(sampling, 1) if sampling is not None else None
         self.fill()
 
     def _fused_step(self) -> bool:
@@ -54,7 +99,8 @@ class MK_Generator(Generator):
         if getattr(self.schedule.globs, "lm_head_instructions", 0) < 1:
             return False
         if not hasattr(self, "_tokens"):
-            self._tokens = torch.zeros(2, 1, dtype=torch.int64, device=self.schedule.globs.hidden_states.device)
+            # two output tokens in turn, and the argmax that a sampled step does not use
+            self._tokens = torch.zeros(3, 1, dtype=torch.int64, device=self.schedule.globs.hidden_states.device)
             self._flip = 0
         return True
 
@@ -77,7 +123,10 @@ class MK_Generator(Generator):
             ids = input_ids.reshape(-1)[:1]
             if ids.dtype != torch.int64:
                 ids = ids.to(torch.int64)
-            self.interpreter.interpret_step(globs, ids, self.model.model.embed_tokens.embed_tokens.weight, out)
+            self.interpreter.interpret_step(globs, ids, self.model.model.embed_tokens.embed_tokens.weight,
+                                            self._tokens[2] if self.sampler else out)
+            if self.sampler:
+                self.sampler(globs.logits.view(1, -1), out=out)
             return out[0]
         if not self.skip_rest:
             emb = self.model.model.embed_tokens(BatchState(input_ids=input_ids))
@@ -89,14 +138,19 @@ class MK_Generator(Generator):
             self.interpreter.interpret(globs)
         if self.skip_rest:
             return input_ids
-        return torch.argmax(globs.logits, dim=-1)
+        return self._pick(globs.logits)
+
+    def _pick(self, logits: Tensor) -> Tensor:
+        if self.sampler:
+            return self.sampler(logits.view(1, -1))[0]
+        return torch.argmax(logits, dim=-1)
 
     def prefill(self, prompt_ids: Tensor, start_pos: int = 0) -> Tensor:
         """Fill the KV cache with the prompt (the model's dense prefill, as
         the reference's model forward does before MK decoding) and return the
-        first generated token (argmax of the last prompt token's logits)."""
-        logits = self.model.prefill(prompt_ids, start_pos)
-        return torch.argmax(logits, dim=-1)
+        first generated token (argmax of, or draw from, the last prompt token's
+        logits)."""
+        return self._pick(self.model.prefill(prompt_ids, start_pos))
 
     def generate(self, output_tokens: Tensor, prompt_len: int, ntok: int,
                  ntok_already_generated: int = 1):
@@ -105,3 +159,115 @@ class MK_Generator(Generator):
             input_ids = output_tokens[:, src : src + 1]
             out = self.run(input_ids, pos_id=prompt_len + ntok_already_generated + i - 1)
             output_tokens[:, src + 1] = out.reshape(-1)
+
+
+class ParallelGenerator(Generator):
+    """Decodes `num_sequences` continuations of one prompt at once.
+
+    The prompt's K/V rows stay in the model's cache (`kv_cache="bf16"`) or are
+    quantised once (`"int8"`); each sequence has a cache of its own, of the same
+    kind, for up to `max_new_tokens` tokens. The projections are dense products,
+    as in the model's prefill. model: a LlamaForCausalLM on a CUDA device."""
+
+    def __init__(self, model, num_sequences: int, max_new_tokens: int, sampling: SamplingParams | None = None,
+                 kv_cache: str = "bf16"):
+        if not hasattr(model, "decode_rows"):
+            raise ValueError(f"ParallelGenerator: {type(model).__name__} has no decode_rows")
+        if model.device.type != "cuda":
+            raise ValueError("ParallelGenerator: the model must be on a CUDA device")
+        if num_sequences < 1 or max_new_tokens < 1:
+            raise ValueError("ParallelGenerator: num_sequences and max_new_tokens must be positive")
+        if kv_cache not in ("bf16", "int8"):
+            raise ValueError(f"kv_cache {kv_cache!r}: must be 'bf16' or 'int8'")
+        c = model.config
+        self.model = model
+        self.num_sequences = num_sequences
+        self.max_new_tokens = max_new_tokens
+        self.sampler = _Sampler(sampling or SamplingParams(), num_sequences)
+        self.int8 = kv_cache == "int8"
+        self.prompt_len = 0
+        self.new_tokens = 0  # tokens in the sequences' own caches
+        self.logits: Tensor | None = None  # of the last step, [num_sequences, vocab]
+        shape = (c.num_hidden_layers * num_sequences, max_new_tokens, c.num_key_value_heads, c.head_dim)
+        if self.int8:
+            own = ops.KVCacheInt8.empty(*shape, device=model.device)
+            self.own = [ops.KVCacheInt8(*(t.unflatten(0, (c.num_hidden_layers, num_sequences))[l]
+                                          for t in own._tensors())) for l in range(c.num_hidden_layers)]
+        else:
+            k, v = (torch.zeros(shape, dtype=torch.bfloat16, device=model.device)
+                    .unflatten(0, (c.num_hidden_layers, num_sequences)) for _ in range(2))
+            self.own = list(zip(k, v))
+        self.prefix: list = []
+
+    def prefill(self, prompt_ids: Tensor) -> Tensor:
+        """Run the prompt through the model, keep its K/V rows as the shared
+        prefix, and return the first token of every sequence (`[num_sequences]`
+        int64). Starts over: earlier continuations are dropped."""
+        logits = self.model.prefill(prompt_ids, 0)
+        n = self.prompt_len = prompt_ids.numel()
+        self.new_tokens = 0
+        k, v = (t[:, 0, :n] for t in self.model.stacked_kv_cache)  # [L, n, Hkv, D]
+        if self.int8:
+            prefix = ops.KVCacheInt8.empty(*k.shape, device=k.device)
+            ops.kv_cache_write(prefix, k, v, 0)
+            self.prefix = [prefix.sequence(l) for l in range(k.shape[0])]
+        else:
+            self.prefix = list(zip(k, v))
+        return self.sampler(logits.view(1, -1).expand(self.num_sequences, -1))
+
+    def run(self, input_ids: Tensor) -> Tensor:
+        """One step: the sequences' last tokens `[num_sequences]` in, their next
+        ones out. `logits` keeps what they were drawn from."""
+        if not self.prefix:
+            raise ValueError("ParallelGenerator.run: prefill first")
+        if self.new_tokens == self.max_new_tokens:
+            raise ValueError(f"ParallelGenerator.run: the caches hold {self.max_new_tokens} new tokens")
+        ids = input_ids.reshape(-1)
+        if ids.numel() != self.num_sequences:
+            raise ValueError(f"input_ids: {ids.numel()} tokens, expected {self.num_sequences}")
+        at = self.new_tokens
+        if self.prompt_len + at >= self.model.max_len():
+            raise ValueError("ParallelGenerator.run: beyond the model's positions")
+        lens = torch.full((self.num_sequences,), at + 1, dtype=torch.int32, device=self.model.device)
+        pos = torch.full((self.num_sequences,), self.prompt_len + at, dtype=torch.int64, device=self.model.device)
+
+        def attend(l, q, k, v):
+            own = self.own[l]
+            if self.int8:
+                ops.kv_cache_write(own, k.unsqueeze(1), v.unsqueeze(1), at)
+            else:
+                own[0][:, at] = k
+                own[1][:, at] = v
+            return ops.shared_prefix_attention(q, self.prefix[l], own, lens, max_own_len=at + 1)
+
+        self.logits = self.model.decode_rows(ids, pos, attend)
+        self.new_tokens = at + 1
+        return self.sampler(self.logits)
+
+    def generate(self, output_tokens: Tensor, prompt_len: int, ntok: int, ntok_already_generated: int = 1):
+        """Append `ntok` tokens per sequence to `output_tokens`
+        `[num_sequences, ...]`, whose column ntok_already_generated - 1 holds the
+        last ones (as `prefill` returned them, the first time)."""
+        if prompt_len != self.prompt_len or ntok_already_generated != self.new_tokens + 1:
+            raise ValueError(f"prompt_len {prompt_len} / ntok_already_generated {ntok_already_generated}: the caches "
+                             f"hold a prompt of {self.prompt_len} and {self.new_tokens} new tokens")
+        for i in range(ntok):
+            src = ntok_already_generated + i - 1
+            output_tokens[:, src + 1] = self.run(output_tokens[:, src])
+
+    def hand_over(self, index: int) -> int:
+        """Copy the rows of sequence `index` behind the prompt in the model's
+        cache, so that `MK_Generator` goes on with it; returns the next position
+        (prompt and new tokens)."""
+        if not 0 <= index < self.num_sequences:
+            raise ValueError(f"sequence {index} of {self.num_sequences}")
+        n, end = self.new_tokens, self.prompt_len + self.new_tokens
+        k_cache, v_cache = self.model.stacked_kv_cache
+        for l, own in enumerate(self.own):
+            k, v = k_cache[l, :1, self.prompt_len : end], v_cache[l, :1, self.prompt_len : end]
+            if self.int8:
+                ops.kv_cache_read(own.sequence(index), 0, n, out=(k, v))
+            else:
+                k.copy_(own[0][index : index + 1, :n])
+                v.copy_(own[1][index : index + 1, :n])
+        return end

@@ -309,14 +309,42 @@ class LlamaForCausalLM(nn.Module):
         causal mask); the decode megakernel then continues at start_pos + n.
         Rounding follows the decode path: bf16 activations between ops, fp32
         accumulation inside each product, RMSNorm as the interpreter's."""
-        c, sp = self.config, self.stacked_params
         k_cache, v_cache = self.stacked_kv_cache
         ids = input_ids.reshape(-1).to(self.device)
-        n, D = ids.numel(), c.head_dim
-        Hq, Hkv = c.num_attention_heads, c.num_key_value_heads
+        n, D = ids.numel(), self.config.head_dim
         end = start_pos + n
         assert n >= 1 and end <= self.max_len(), "prompt beyond the KV cache"
         pos = torch.arange(start_pos, end, device=self.device)
+        # causal mask with the cached prefix: query i sees keys 0 .. start_pos + i
+        mask = torch.arange(end, device=self.device).unsqueeze(0) <= pos.unsqueeze(1)  # [n, end]
+
+        def attend(l, q, k, v):
+            k_cache[l, 0, start_pos:end] = k
+            v_cache[l, 0, start_pos:end] = v
+            keys = k_cache[l, 0, :end].transpose(0, 1).unsqueeze(0)  # [1, Hkv, end, D]
+            vals = v_cache[l, 0, :end].transpose(0, 1).unsqueeze(0)
+            o = F.scaled_dot_product_attention(q.transpose(0, 1).unsqueeze(0), keys, vals, attn_mask=mask,
+                                               scale=1.0 / math.sqrt(D), enable_gqa=True)
+            return o[0].transpose(0, 1)
+
+        h = self._layers(ids, pos, attend)
+        self.prefill_hidden = h[-1].clone()
+        return self.lm_head.lm_head(self.lm_head.input_norm(h[-1]))
+
+    @torch.no_grad()
+    def decode_rows(self, input_ids: Tensor, positions: Tensor, attend) -> Tensor:
+        """One token of each of n sequences (ids and positions `[n]`) through the
+        model as dense products; returns the logits `[n, vocab]`. `attend(layer,
+        q, k, v)` gets the rows after RoPE (`[n, heads, D]`), appends k and v to
+        its caches and returns the attention's output `[n, num_q_heads, D]`."""
+        h = self._layers(input_ids.to(self.device), positions.to(self.device), attend)
+        return self.lm_head.lm_head(self.lm_head.input_norm(h))
+
+    def _layers(self, ids: Tensor, pos: Tensor, attend) -> Tensor:
+        """Hidden states `[n, H]` of n rows behind the last layer."""
+        c, sp = self.config, self.stacked_params
+        n, D = ids.numel(), c.head_dim
+        Hq, Hkv = c.num_attention_heads, c.num_key_value_heads
         cos, sin = self.model.rope_cos[pos].unsqueeze(1), self.model.rope_sin[pos].unsqueeze(1)  # [n, 1, D]
 
         def norm(x, w):
@@ -330,26 +358,18 @@ class LlamaForCausalLM(nn.Module):
                 rot = torch.cat((-x[..., D // 2 :], x[..., : D // 2]), dim=-1)
             return (x * cos + rot * sin).to(x.dtype)
 
-        # causal mask with the cached prefix: query i sees keys 0 .. start_pos + i
-        mask = torch.arange(end, device=self.device).unsqueeze(0) <= pos.unsqueeze(1)  # [n, end]
         h = self.model.embed_tokens.embed_tokens.weight[ids]  # [n, H]
         for l in range(c.num_hidden_layers):
             qkv = norm(h, sp.attn_ln_weight[l]) @ sp.qkv_proj[l].T
             q = rope(qkv[:, : Hq * D].view(n, Hq, D))
             k = rope(qkv[:, Hq * D : (Hq + Hkv) * D].view(n, Hkv, D))
             v = qkv[:, (Hq + Hkv) * D :].view(n, Hkv, D)
-            k_cache[l, 0, start_pos:end] = k
-            v_cache[l, 0, start_pos:end] = v
-            keys = k_cache[l, 0, :end].transpose(0, 1).unsqueeze(0)  # [1, Hkv, end, D]
-            vals = v_cache[l, 0, :end].transpose(0, 1).unsqueeze(0)
-            o = F.scaled_dot_product_attention(q.transpose(0, 1).unsqueeze(0), keys, vals, attn_mask=mask,
-                                               scale=1.0 / math.sqrt(D), enable_gqa=True)
-            h = h + o[0].transpose(0, 1).reshape(n, Hq * D) @ sp.o_proj[l].T
+            o = attend(l, q, k, v)
+            h = h + o.reshape(n, Hq * D) @ sp.o_proj[l].T
             x = norm(h, sp.mlp_ln_weight[l])
             up, gate = x @ sp.up_proj[l].T, x @ sp.gate_proj[l].T
             h = h + (F.silu(gate) * up) @ sp.down_proj[l].T
-        self.prefill_hidden = h[-1].clone()
-        return self.lm_head.lm_head(self.lm_head.input_norm(h[-1]))
+        return h
 
     def setup_caches(self):
         shape = (
