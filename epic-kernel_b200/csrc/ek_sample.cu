@@ -14,10 +14,13 @@
 // pass then adds up all weights exactly (which shows whether those bins hold
 // the cut; if not, all logits are searched) and lists the logits of those bins,
 // which go into histograms over their order-preserving integer keys until a
-// bin is one value. When few tokens are left, they are listed instead, and one block
-// ranks them by counting, n^2 comparisons for n <= 512. For top-k <= 512 the
-// bins are filled with the largest logit of each thread only: at least k
-// logits lie at or above the bin where k of those maxima are reached.
+// bin is one value. When few tokens are left, they are listed instead, and one
+// block ranks them by counting, n^2 comparisons for n <= 512. For top-k <= 512
+// the bins are filled with the largest logit of each thread only: at least k
+// logits lie at or above the bin where k of those maxima are reached. bf16
+// logits take few values: without top-k their weights come from a table of
+// values, and for top-p a count per value gives the cut in one pass (64 rows of
+// 128256 logits with top-p 0.9: 66 us before the table, 44 with it).
 //
 // A row is spread over a cluster of 1 to 8 blocks that hold it in shared
 // memory, so it is read from HBM once; the blocks exchange maxima, histograms
@@ -43,6 +46,9 @@ constexpr int kBatch = 4;
 constexpr int kList = 512;   // tokens that one block ranks by counting
 constexpr int kRoom = 1024;  // a block's list; also room for all of one of 512 ranges of the index
 constexpr int kRaw = 4096;   // logits listed against a maximum that still grows
+// Table of bf16 values, 2^-9 <= |l| < 2^7, by falling value: 2048 positive, 2048 negative.
+constexpr int kValues = 4096;
+constexpr int kTableBytes = kValues * (sizeof(unsigned) + sizeof(unsigned long long));  // counts, weights
 constexpr int kMaxVocab = kMaxCluster * kMaxBytes / 4;
 using u64 = unsigned long long;
 
@@ -58,6 +64,7 @@ struct SampleParams {
   float temperature_all, top_p_all, min_p_all;
   int top_k_all, vocab, weight_bits;
   int slice;  // elements per block, a multiple of 16
+  int table;  // bytes of the slice when a table of values follows it, else 0
 };
 
 __device__ __forceinline__ float as_float(float x) { return x; }
@@ -162,6 +169,17 @@ __device__ u64 block_scan(u64 v, Shared<kThreads>& sh) {
   }
   const u64 earlier = __shfl_sync(~0u, t, (warp + 31) % 32);
   return warp ? v + earlier : v;
+}
+
+// Place of a bf16 value (its 16 bits) in the table; outside [0, kValues) halves for tiny values (callers check).
+__device__ __forceinline__ int place_of(unsigned bits) {
+  const int m = (int)(bits & 0x7fffu) - 0x3b00;
+  return bits & 0x8000u ? kValues / 2 + m : kValues / 2 - 1 - m;
+}
+__device__ __forceinline__ bool tabled(unsigned bits) { return (bits & 0x7fffu) >= 0x3b00u; }  // (below 2^7 by the caller)
+__device__ __forceinline__ float value_at(int place) {
+  const unsigned bits = place < kValues / 2 ? 0x3b00u + (kValues / 2 - 1 - place) : 0x8000u | (0x3b00u + place - kValues / 2);
+  return __uint_as_float(bits << 16);
 }
 
 template <typename T>
@@ -583,8 +601,94 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   bool listed = false;       // sh.list holds this block's logits in question
   unsigned k_cut = 0;  // top-k keeps keys above, and k_ties equal ones
   u64 k_ties = 0;
+  // bf16 logits take few values: a table of their weights, and for top-p a count per value, which gives the cut at once
+  bool by_value = false;
+  unsigned* counts_at = reinterpret_cast<unsigned*>(reinterpret_cast<uint8_t*>(dynamic) + p.table);
+  u64* weight_at = reinterpret_cast<u64*>(counts_at + kValues);
+  const bool table = sizeof(T) == 2 && RESIDENT && p.table && !use_k && top < 128.f && low > -128.f;
+  if (table && !use_p) {
+    for (int i = tid; i < kValues; i += kThreads) {
+      const float l = value_at(i);
+      weight_at[i] = l >= low && l <= top ? weight(l) : 0;
+    }
+    __syncthreads();
+    by_value = true;
+  } else if (table) {
+    constexpr int PER = kValues / kThreads;
+    for (int i = tid; i < kValues / 4; i += kThreads) reinterpret_cast<uint4*>(counts_at)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    u64 tiny = 0;
+#pragma unroll 2
+    for (int i = tid; i < vectors; i += kThreads) {
+      const V16 v = vec(i);
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float l = as_float(v.x[e]);
+        const unsigned bits = __float_as_uint(l) >> 16;
+        any |= l >= low && !tabled(bits);
+        if (l >= low && tabled(bits)) atomicAdd(counts_at + place_of(bits), 1u);
+      }
+      if (any) {
+#pragma unroll 1
+        for (int e = i * N; e < (i + 1) * N; ++e) {
+          const float l = as_float(slice[e]);
+          if (l >= low && !tabled(__float_as_uint(l) >> 16)) tiny += weight(l);
+        }
+      }
+    }
+    const u64 block_tiny = block_scan(tiny, sh);
+    if (tid == kThreads - 1)
+      for (int r = 0; r < C; ++r) *peer(&sh.block_total[rank], r) = block_tiny;
+    if (tid == 0) sh.found_bin = -1;
+    sync();
+    tiny = 0;
+    for (int r = 0; r < C; ++r) tiny += sh.block_total[r];
+    u64 n[PER], w[PER], mine = 0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) n[e] = 0;
+    for (int r = 0; r < C; ++r) {
+      const unsigned* other = peer(counts_at, r) + tid * PER;
+#pragma unroll
+      for (int e = 0; e < PER; e += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(other + e);
+        n[e] += x.x, n[e + 1] += x.y, n[e + 2] += x.z, n[e + 3] += x.w;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      w[e] = n[e] ? weight(value_at(tid * PER + e)) : 0;
+      weight_at[tid * PER + e] = w[e];
+      mine += n[e] * w[e];
+    }
+    const u64 upto = block_scan(mine, sh);
+    if (tid == kThreads - 1) sh.found_before = upto;
+    __syncthreads();
+    const u64 goal = share(sh.found_before + tiny);
+    u64 before = upto - mine + (tid * PER >= kValues / 2 ? tiny : 0);  // the tiny values lie between the halves
+    if (before < goal && goal <= before + mine) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const u64 all = n[e] * w[e];
+        if (before < goal && goal <= before + all) {
+          sh.found_bin = (int)key_of<T>(value_at(tid * PER + e));
+          sh.total[0] = quotient_up(goal - before, w[e]);
+        }
+        before += all;
+      }
+    }
+    __syncthreads();
+    by_value = sh.found_bin >= 0;  // else the cut is among the tiny values: the general search finds it
+    if (by_value) {
+      const unsigned key = (unsigned)sh.found_bin;
+      const u64 r = sh.total[0];
+      if (key > cut) cut = key, ties = r;
+      else if (key == cut) ties = min(ties, r);
+    }
+    __syncthreads();
+  }
   for (int stage = 0; stage < 2; ++stage) {  // 0: top-k; 1: top-p among what top-k left
-    if (stage == 0 ? !use_k : !use_p) continue;
+    if (stage == 0 ? !use_k : !use_p || by_value) continue;
     // the lowest logit that takes part; NaN (none) above an infinite k_cut
     const float next = value_of<T>(k_cut + 1);
     const float lowest = stage == 0 || k_cut == 0 || next <= low ? low : next;
@@ -780,6 +884,32 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
         }
       });
     }
+  } else if (by_value) {
+#pragma unroll 2
+    for (int i = v0 + lane; i < v1; i += 32) {
+      const V16 v = vec(i);
+      u64 w[N];
+      bool tiny = false;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float l = as_float(v.x[e]);
+        const unsigned bits = __float_as_uint(l) >> 16;
+        const bool in = l > cut_value;
+        tied += l == cut_value;
+        tiny |= in && !tabled(bits);
+        w[e] = 0;
+        if (in && tabled(bits)) w[e] = weight_at[place_of(bits)];
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) above += w[e];
+      if (tiny) {
+#pragma unroll 1
+        for (int e = i * N; e < (i + 1) * N; ++e) {
+          const float l = as_float(slice[e]);
+          if (l > cut_value && !tabled(__float_as_uint(l) >> 16)) above += weight(l);
+        }
+      }
+    }
   } else {
     for_each_by_warp([&](int, const float (&l)[kBatch]) {
       bool any = false;
@@ -847,6 +977,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   }
   const int from = __ffs(__ballot_sync(~0u, owner >= 0)) - 1;
   owner = __shfl_sync(~0u, owner, from);
+  auto weight_of = [&](float l) {
+    const unsigned bits = __float_as_uint(l) >> 16;
+    return by_value && tabled(bits) ? weight_at[place_of(bits)] : weight(l);
+  };
   if (owner == rank * kWarps + warp) {
     u64 sum = __shfl_sync(~0u, owner_before, from), seen = __shfl_sync(~0u, owner_ties, from);
     for (int i0 = v0; i0 < v1; i0 += 32) {
@@ -860,7 +994,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
         for (int e = 0; e < N; ++e) {
           const float l = as_float(v.x[e]);
           mine += l == cut_value;
-          if (l > cut_value) heavy += weight(l);
+          if (l > cut_value) heavy += weight_of(l);
         }
       }
       unsigned tb = mine;
@@ -884,7 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float l = as_float(v.x[e]);
-          if (l > cut_value) at += weight(l);
+          if (l > cut_value) at += weight_of(l);
           else if (l == cut_value && tt++ < ties) at += unit;
           if (pick < 0 && at > goal) pick = e;
         }
@@ -942,8 +1076,12 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
     return launch<T, false, 512>(p, batch, 1, kRaw * sizeof(u64), st);
   }
   p.slice = slice(cluster);
-  if (threads == 1024) return launch<T, true, 1024>(p, batch * cluster, cluster, p.slice * size, st);
-  return launch<T, true, 512>(p, batch * cluster, cluster, p.slice * size, st);
+  // The table of values: where it does not take the second block off an SM, and a block has more elements than it.
+  const int bytes = p.slice * size;
+  if (size == 2 && p.slice >= 4096 && (threads == 1024 || bytes <= 36 * 1024)) p.table = bytes;
+  const int all = bytes + (p.table ? kTableBytes : 0);
+  if (threads == 1024) return launch<T, true, 1024>(p, batch * cluster, cluster, all, st);
+  return launch<T, true, 512>(p, batch * cluster, cluster, all, st);
 }
 
 }  // namespace
@@ -956,7 +1094,7 @@ extern "C" int ek_sample(const EkSampleArgs* a, void* stream) {
   if (a->batch > (1 << 27)) return fail(EK_E_UNSUPPORTED, "batch %d", a->batch);
   if (a->batch == 0) return EK_SUCCESS;
   if (!a->logits || !a->uniforms || !a->tokens) return fail(EK_E_INVALID, "NULL pointer argument");
-  SampleParams p;
+  SampleParams p = {};
   p.logits = a->logits;
   p.row_stride = a->row_stride;
   p.uniforms = a->uniforms;
