@@ -606,14 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   unsigned* counts_at = reinterpret_cast<unsigned*>(reinterpret_cast<uint8_t*>(dynamic) + p.table);
   u64* weight_at = reinterpret_cast<u64*>(counts_at + kValues);
   const bool table = sizeof(T) == 2 && RESIDENT && p.table && !use_k && top < 128.f && low > -128.f;
-  if (table && !use_p) {
+  if (table && !use_p && !(min_p > 0.f)) {  // min-p leaves too few weights
     for (int i = tid; i < kValues; i += kThreads) {
       const float l = value_at(i);
       weight_at[i] = l >= low && l <= top ? weight(l) : 0;
     }
     __syncthreads();
     by_value = true;
-  } else if (table) {
+  } else if (table && use_p) {
     constexpr int PER = kValues / kThreads;
     for (int i = tid; i < kValues / 4; i += kThreads) reinterpret_cast<uint4*>(counts_at)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
@@ -1058,16 +1058,20 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
   auto fits = [&](int n) { return slice(n) <= kMaxElements && slice(n) * size <= kMaxBytes; };
   // Blocks per row: up to 8 that keep 2048 elements each and run at once with the other rows' (what fits of
   // clusters of 2, 4 and 8: 148, 71 and 33 with two blocks of 512 threads on an SM, 74, 33 and 15 with one of 1024).
+  // Rows whose cut or weights come from the table of values (bf16, no top-k, top-p) take blocks of 1024: with the
+  // table two blocks of 512 do not fit an SM. More than 4 give nothing there, since each block adds up all blocks'
+  // counts (33 rows of 128256: 37 us on 4 x 1024, 55 on 8 x 512 without the table; one row 39 and 37 on 4 and 8).
+  const bool by_value = size == 2 && !p.top_k && (p.top_k_all <= 0 || p.top_k_all >= p.vocab) && (p.top_p || p.top_p_all < 1.f);
   int cluster = 1, threads = 512;
   while (cluster < kMaxCluster && p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 148 : cluster == 2 ? 71 : 33))
     cluster *= 2;
-  if (slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
-    // Much work per block: 1024 threads. 64 rows of 128256 bf16 logits with top-p take 66 us on 2 x 1024 threads
-    // and 75 us on 4 x 512; one row with top-k takes 15.9 us on 8 x 1024 and 13.8 us on 8 x 512.
+  if (by_value || slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
+    // Much work per block: 1024 threads (one row of 128256 with top-k takes 15.9 us on 8 x 1024 and 13.8 us on 8 x
+    // 512; 40 plain rows 37 us on 2 x 1024, 39 on 4 x 512).
     threads = 1024;
     cluster = 1;
     while (cluster < kMaxCluster &&
-           ((p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 74 : cluster == 2 ? 33 : 15)) ||
+           ((p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 74 : cluster == 2 ? 33 : by_value ? 0 : 15)) ||
             (!fits(cluster) && batch < 148)))
       cluster *= 2;
   }
@@ -1076,9 +1080,9 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
     return launch<T, false, 512>(p, batch, 1, kRaw * sizeof(u64), st);
   }
   p.slice = slice(cluster);
-  // The table of values: where it does not take the second block off an SM, and a block has more elements than it.
+  // The table of values goes behind the slice of a block that has its SM to itself.
   const int bytes = p.slice * size;
-  if (size == 2 && p.slice >= 4096 && (threads == 1024 || bytes <= 36 * 1024)) p.table = bytes;
+  if (size == 2 && threads == 1024) p.table = bytes;
   const int all = bytes + (p.table ? kTableBytes : 0);
   if (threads == 1024) return launch<T, true, 1024>(p, batch * cluster, cluster, all, st);
   return launch<T, true, 512>(p, batch * cluster, cluster, all, st);
