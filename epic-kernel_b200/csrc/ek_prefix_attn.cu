@@ -857,20 +857,26 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 }
 
 // ---------------------------------------------------------------------------
-// One warp per (sequence, query head) joins its items: lane i takes the maximum and sum of item i (32 at a time), then
-// the lanes go through the rows of O with 16-byte loads, two items (D = 64) or one at a time.
-template <int D>
-__global__ void __launch_bounds__(128) join(const AttnParams p) {
+// A warp, or W warps of a block, per (sequence, query head) join its items: of 32 items, lane i takes the maximum and
+// sum of item i, then the lanes go through the rows of O with 16-byte loads, two items (D = 64) or one at a time. Warp
+// w of W takes every W-th item.
+constexpr int kJoinWarps = 8;
+
+template <int D, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) join(const AttnParams p) {
   constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
   wait_before();
-  const long long row = blockIdx.x * 4ll + threadIdx.x / 32, rows = (long long)p.batch * p.q_heads;
-  const int lane = threadIdx.x % 32, sub = lane / LANES, piece = lane % LANES;
-  if (row >= rows) return;
+  const long long row = W == 1 ? blockIdx.x * 4ll + threadIdx.x / 32 : blockIdx.x, rows = (long long)p.batch * p.q_heads;
+  const int lane = threadIdx.x % 32, sub = lane / LANES, piece = lane % LANES, warp = W == 1 ? 0 : threadIdx.x / 32;
+  if (W == 1 && row >= rows) return;
   const int b = (int)(row / p.q_heads), h = (int)(row % p.q_heads);
   const int len = min(max(p.own_lens[b], 0), p.max_own);
   const int shared = b * p.group + h % p.group < p.wide_rows ? p.wide_slots : p.narrow_slots;
-  const int parts = shared + (len + p.own_chunk - 1) / p.own_chunk;
-  auto place = [&](int i) { return (long long)(i < shared ? i : i - shared + p.prefix_slots) * rows + row; };
+  const int all = shared + (len + p.own_chunk - 1) / p.own_chunk, parts = (all - warp + W - 1) / W;
+  auto place = [&](int j) {
+    const int i = j * W + warp;
+    return (long long)(i < shared ? i : i - shared + p.prefix_slots) * rows + row;
+  };
   float top = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < parts; i0 += 32) {
@@ -890,7 +896,7 @@ __global__ void __launch_bounds__(128) join(const AttnParams p) {
     l = l * old + sum;
     o.x *= old, o.y *= old, o.z *= old, o.w *= old;
     const unsigned holds = __ballot_sync(~0u, lane < n && ml.y != 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < n; i += AT_ONCE) {
       const int k = i + sub;
       const float fk = __shfl_sync(~0u, f, k & 31);
@@ -903,6 +909,24 @@ __global__ void __launch_bounds__(128) join(const AttnParams p) {
   if (AT_ONCE == 2) {
     o.x += __shfl_xor_sync(~0u, o.x, 16), o.y += __shfl_xor_sync(~0u, o.y, 16);
     o.z += __shfl_xor_sync(~0u, o.z, 16), o.w += __shfl_xor_sync(~0u, o.w, 16);
+  }
+  if (W > 1) {
+    __shared__ float4 warp_o[W][LANES];
+    __shared__ float2 warp_ml[W];
+    if (sub == 0) warp_o[warp][piece] = o;
+    if (lane == 0) warp_ml[warp] = make_float2(top, l);
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 0; w < W; ++w) top = fmaxf(top, warp_ml[w].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    l = 0.f, o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = exp2_approx(warp_ml[w].x - base);
+      const float4 x = warp_o[w][piece];
+      l += f * warp_ml[w].y;
+      o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: zeros
   if (sub == 0)
@@ -921,8 +945,13 @@ struct Plan {
   long long part_bytes;
 };
 
-// Query rows of a KV head from which many_rows takes the prefix.
-constexpr int kManyRows = 17;
+// many_rows takes the prefix from here on: more than two tiles of 8 query rows per KV head, and that many elements of
+// K that few_rows would go through, its tiles of 8 rows times the prefix. Times of whole calls in us, few against many:
+// 16 heads of 128, bf16, 32768 rows of prefix: 68 / 70 at 16 query rows, 84 / 72 at 24; 4096 rows: 31 / 31 at 32
+// (2^25 elements), 37 / 33 at 48. 8 heads, 8192 rows, 32 query rows (2^25): 25 / 25 bf16, 33 / 31 int8. int8, 16 heads,
+// 32768 rows: 90 / 106 at 16 query rows, 125 / 108 at 24. 8 heads, 512 rows: 22 / 31 at 256 query rows, 59 / 49 at 1024.
+constexpr int kManyFrom = 17;
+constexpr long long kManyElements = 1ll << 25;
 
 int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   using ek::fail;
@@ -941,36 +970,38 @@ int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   if (e != cudaSuccess) return ek::cuda_fail(e, "cudaDeviceGetAttribute");
   std::memset(&pl, 0, sizeof(pl));
   const int group = a->q_heads / a->kv_heads, rows = a->batch * group;
-  // few_rows: items that fill the GPU about once
-  const long long want = 4ll * sms;
-  auto chunk = [&](long long len, long long items) {
-    const long long splits = items < want ? div_up(want, items) : 1;
+  // few_rows: items that fill the GPU once: four blocks fit an SM, three with bf16 rows of 128. One sequence, 32 query
+  // heads of 128, 32768 rows of prefix, for 1, 2, 3, 4 and 6 items per SM: bf16 47, 39, 39, 44, 43 us, int8 61, 43, 39,
+  // 37, 43 us.
+  const bool i8 = (a->prefix_len > 0 ? a->prefix_k.scales : a->own_k.scales) != nullptr;
+  const long long want = (a->head_dim == 128 && !i8 ? 3ll : 4ll) * sms;
+  auto chunk = [&](long long len, long long splits) {
     const long long c = div_up(div_up(len, splits), 64) * 64ll;
     return (int)(c < 64 ? 64 : c);
   };
   const long long own = (long long)a->batch * div_up(group, 8) * a->kv_heads;
-  pl.own_chunk = chunk(a->max_own_len, own > 0 ? own : 1);
+  pl.own_chunk = chunk(a->max_own_len, own > 0 ? div_up(want, own) : 1);  // of unequal lengths: rather more
   pl.own_slots = div_up(a->max_own_len, pl.own_chunk);
-  pl.many = rows >= kManyRows && a->prefix_len > 0;
+  const long long tiles = (long long)div_up(rows, 8) * a->kv_heads;
+  pl.many = rows >= kManyFrom && tiles * a->prefix_len * a->head_dim >= kManyElements;
   if (!pl.many) {
-    const long long tiles = (long long)div_up(rows, 8) * a->kv_heads;
-    pl.prefix_chunk = chunk(a->prefix_len, tiles > 0 ? tiles : 1);
+    pl.prefix_chunk = chunk(a->prefix_len, tiles > 0 && tiles < want ? want / tiles : 1);
     pl.prefix_slots = div_up(a->prefix_len, pl.prefix_chunk);
   } else {
     // Blocks of 256 rows (wide), and one of the rest, which is narrow up to 128 rows. A wide tile costs two
     // units, a narrow one one; the smallest share of units whose items all run at once.
     pl.wide_blocks = rows / 256 + (rows % 256 > 128);
     pl.narrow_rows = rows % 256 > 128 ? 0 : rows % 256;
-    const long long tiles = div_up(a->prefix_len, 128), narrow = pl.narrow_rows ? 1 : 0;
-    const long long units = (2ll * pl.wide_blocks + narrow) * tiles * a->kv_heads;
+    const long long keys = div_up(a->prefix_len, 128), narrow = pl.narrow_rows ? 1 : 0;
+    const long long units = (2ll * pl.wide_blocks + narrow) * keys * a->kv_heads;
     const long long blocks = (pl.wide_blocks + narrow) * a->kv_heads;
     const long long most = blocks <= sms ? sms : 4 * blocks;
     long long share = div_up(units, most);
     for (;; ++share) {
       pl.wide_tiles = div_up(share, 2), pl.narrow_tiles = (int)share;
-      pl.wide_splits = div_up(tiles, pl.wide_tiles), pl.narrow_splits = div_up(tiles, pl.narrow_tiles);
+      pl.wide_splits = div_up(keys, pl.wide_tiles), pl.narrow_splits = div_up(keys, pl.narrow_tiles);
       if (((long long)pl.wide_blocks * pl.wide_splits + narrow * pl.narrow_splits) * a->kv_heads <= most) break;
-      if (share >= 2 * tiles) break;
+      if (share >= 2 * keys) break;
     }
     const int wide_slots = pl.wide_blocks ? pl.wide_splits : 0, narrow_slots = narrow ? 2 * pl.narrow_splits : 0;
     pl.prefix_slots = wide_slots > narrow_slots ? wide_slots : narrow_slots;
@@ -1084,7 +1115,12 @@ cudaError_t launch(const FewParams& p, const ManyParams* many, cudaStream_t st) 
     const int blocks = (many->wide_blocks * many->wide_splits + (many->narrow_rows ? many->narrow_splits : 0)) * p.a.kv_heads;
     if ((e = start(many_rows<D, I8>, *many, blocks, M::WARPS * 32, M::SMEM, items > 0, st)) != cudaSuccess) return e;
   }
-  return start(join<D>, p.a, div_up((long long)p.a.batch * p.a.q_heads, 4), 128, 0, items > 0 || many, st);
+  // Few rows of many items get a block each. Whole calls, a warp against a block per row: 32 rows 47 / 39 us (one
+  // sequence, 32768 rows of prefix, D = 128), 512 rows 41 / 35, 1952 rows 86 / 84, 4096 rows 84 / 91.
+  const long long rows = (long long)p.a.batch * p.a.q_heads;
+  if (rows <= 2048 && p.a.prefix_slots + p.a.own_slots > 8)
+    return start(join<D, kJoinWarps>, p.a, (int)rows, kJoinWarps * 32, 0, items > 0 || many, st);
+  return start(join<D, 1>, p.a, div_up(rows, 4), 128, 0, items > 0 || many, st);
 }
 
 }  // namespace
