@@ -505,9 +505,9 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 
   if (warp == C::SCORES) ek::tmem_alloc(tmem_at, 512);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::KS; ++i) ek::mbar_init(k_full + i, I8 ? 128 : 1), ek::mbar_init(k_empty + i, 1);
-    for (int i = 0; i < C::VS; ++i) ek::mbar_init(v_full + i, I8 ? 128 : 1), ek::mbar_init(v_empty + i, 1);
-    for (int i = 0; i < C::RAW_STAGES; ++i) ek::mbar_init(raw_full + i, 1), ek::mbar_init(raw_empty + i, 128);
+    for (int i = 0; i < C::KS; ++i) ek::mbar_init(k_full + i, I8 ? 4 : 1), ek::mbar_init(k_empty + i, 1);
+    for (int i = 0; i < C::VS; ++i) ek::mbar_init(v_full + i, I8 ? 4 : 1), ek::mbar_init(v_empty + i, 1);
+    for (int i = 0; i < C::RAW_STAGES; ++i) ek::mbar_init(raw_full + i, 1), ek::mbar_init(raw_empty + i, 4);
     for (int i = 0; i < 2; ++i) ek::mbar_init(s_full + i, 1), ek::mbar_init(p_full + i, 4), ek::mbar_init(p_empty + i, 1);
     ek::mbar_init(s_empty, 4), ek::mbar_init(q_full, 8), ek::mbar_init(drained, 2);
     *abort = 0;
@@ -528,8 +528,10 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // for a whole warp, which goes on or gives up together
     return __all_sync(~0u, ek::mbar_wait_bounded(bar, parity, abort)) != 0;
   };
-  auto spin = [&](uint64_t* bar, uint32_t parity) {  // where the softmax or the tensor core would stand still
-    return __all_sync(~0u, ek::mbar_wait_bounded<true>(bar, parity, abort)) != 0;
+  // Where the softmax or the tensor core would stand still. With 8-bit rows polls would slow the widening warps, which
+  // the others wait for (256 x 24 heads of 128, 32768 rows: 218 us with polls, 160 without).
+  auto spin = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(~0u, ek::mbar_wait_bounded<!I8>(bar, parity, abort)) != 0;
   };
   // One arrival per warp: 128 on one barrier are serialised.
   auto arrive = [&](uint64_t* bar) {
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
       if (tile >= stages && !wait((is_v ? v_empty : k_empty) + cs, (tile / stages - 1) & 1)) break;
       const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW;
       uint8_t* to = smem + (is_v ? C::OFF_V : C::OFF_K) + cs * C::TILE;
-#pragma unroll 4
+#pragma unroll 2
       for (int i = t; i < 128 * D / 16; i += 128) {
         const int r = i / (D / 16), piece = i % (D / 16);
         const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 16);
@@ -749,8 +751,8 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         }
       }
       ek::fence_proxy_async_smem();
-      ek::mbar_arrive((is_v ? v_full : k_full) + cs);
-      ek::mbar_arrive(raw_empty + rs);
+      arrive((is_v ? v_full : k_full) + cs);
+      arrive(raw_empty + rs);
     }
   } else {
     ek::registers_down<C::OTHER_REGS>();
