@@ -16,8 +16,8 @@
 // which go into histograms over their order-preserving integer keys until a
 // bin is one value. When few tokens are left, they are listed instead, and one
 // block ranks them by counting, n^2 comparisons for n <= 512. For top-k <= 512
-// the bins are filled with the largest logit of each thread only: at least k
-// logits lie at or above the bin where k of those maxima are reached. bf16
+// the bins are filled with the largest logit of each thread only (with all of a
+// short row): at least k logits lie at or above the bin where k are reached. bf16
 // logits take few values: without top-k their weights come from a table of
 // values, and for top-p a count per value gives the cut in one pass (64 rows of
 // 128256 logits with top-p 0.9: 66 us before the table, 44 with it).
@@ -553,9 +553,25 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     if (at < kRoom) sh.list[at] = (u64)~key << 32 | (unsigned)index;
   };
 
+  if (p.vocab <= 128) {  // C is 1; 10 to 14 us instead of 20 to 37. At 512 ranking takes 43 us, the rest 12 to 35.
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    for_each([&](int i, float l) {
+      if (l >= low) append(key_of<T>(l), i);
+    });
+    __syncthreads();
+    finish(sh.listed, 0);
+    return;
+  }
   if (use_k && k <= kList) {  // at least k logits lie in the bins down to that of the k-th largest thread maximum
     if (tid == 0) sh.listed = 0;
-    if (mine_top >= low) atomicAdd(&sh.hist[buffer][0][bin_of(mine_top)], 1u);
+    if (vectors <= kThreads) {  // short rows have too few maxima: all logits (129 logits, k = 20: 37 -> 13 us)
+      for_each([&](int, float l) {
+        if (l >= low) atomicAdd(&sh.hist[buffer][0][bin_of(l)], 1u);
+      });
+    } else if (mine_top >= low) {
+      atomicAdd(&sh.hist[buffer][0][bin_of(mine_top)], 1u);
+    }
     sync();
     const u64 count_here = collect(false);
     const u64 sum = block_scan(count_here, sh);
@@ -1065,7 +1081,12 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
   int cluster = 1, threads = 512;
   while (cluster < kMaxCluster && p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 148 : cluster == 2 ? 71 : 33))
     cluster *= 2;
-  if (by_value || slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
+  // Beyond 148 rows two blocks of 512 with the table share an SM while the row leaves room (155 rows of 19592: 39 us,
+  // 51 on 1 x 1024; 32000: 66 and 61).
+  const bool pairs = by_value && batch > 148 && slice(1) * size <= 40 * 1024;
+  if (pairs) {
+    cluster = 1;
+  } else if (by_value || slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
     // Much work per block: 1024 threads (one row of 128256 with top-k takes 15.9 us on 8 x 1024 and 13.8 us on 8 x
     // 512; 40 plain rows 37 us on 2 x 1024, 39 on 4 x 512).
     threads = 1024;
@@ -1080,9 +1101,9 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
     return launch<T, false, 512>(p, batch, 1, kRaw * sizeof(u64), st);
   }
   p.slice = slice(cluster);
-  // The table of values goes behind the slice of a block that has its SM to itself.
+  // The table of values goes behind the slice.
   const int bytes = p.slice * size;
-  if (size == 2 && threads == 1024) p.table = bytes;
+  if (size == 2 && (threads == 1024 || pairs)) p.table = bytes;
   const int all = bytes + (p.table ? kTableBytes : 0);
   if (threads == 1024) return launch<T, true, 1024>(p, batch * cluster, cluster, all, st);
   return launch<T, true, 512>(p, batch * cluster, cluster, all, st);
