@@ -14,8 +14,8 @@
 // pass then adds up all weights exactly (which shows whether those bins hold
 // the cut; if not, all logits are searched) and lists the logits of those bins,
 // which go into histograms over their order-preserving integer keys until a
-// bin is one value. When few tokens are left, they are listed instead, and one
-// block ranks them by counting, n^2 comparisons for n <= 512. For top-k <= 512
+// bin is one value. When few tokens are left, up to 512, they are listed
+// instead, and one block ranks them. For top-k <= 512
 // the bins are filled with the largest logit of each thread only (with all of a
 // short row): at least k logits lie at or above the bin where k are reached. bf16
 // logits take few values: without top-k their weights come from a table of
@@ -43,7 +43,8 @@ constexpr int kMaxCluster = 8;
 constexpr int kMaxElements = 65536;    // per block: a bin's 16-bit limbs add up below 2^32
 constexpr int kMaxBytes = 176 * 1024;  // of logits per block
 constexpr int kBatch = 4;
-constexpr int kList = 512;   // tokens that one block ranks by counting
+constexpr int kList = 512;   // tokens that one block ranks
+constexpr int kCount = 160;  // so many by counting, more by sorting (a row of 2000: 14 and 16 us at k = 64, 25 and 18 at 256)
 constexpr int kRoom = 1024;  // a block's list; also room for all of one of 512 ranges of the index
 constexpr int kRaw = 4096;   // logits listed against a maximum that still grows
 // Table of bf16 values, 2^-9 <= |l| < 2^7, by falling value: 2048 positive, 2048 negative.
@@ -410,9 +411,58 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     cut = max(cut, key_of<T>(fminf(l, top)));
   }
 
-  // Finishes the row from the n listed tokens, which are all that may stay. `goal`: the weight for top-p, 0 if
+  // Finishes the row from the n <= kList listed tokens, which are all that may stay. `goal`: the weight for top-p, 0 if
   // it follows from the list.
+  auto finish_sorted = [&](int n, u64 goal) {
+    // `own` of threads 0 .. n - 1 in rising order (bitonic; exchanges within a warp by shuffles)
+    auto sort = [&](u64 own) {
+      for (int size = 2; size < 2 * n; size *= 2)
+        for (int j = size / 2; j > 0; j /= 2) {
+          u64 other;
+          if (j < 32) {
+            other = __shfl_xor_sync(~0u, own, j);
+          } else {
+            __syncthreads();
+            if (tid < kList) sh.list[tid] = own;
+            __syncthreads();
+            other = tid < kList ? sh.list[tid ^ j] : ~0ull;
+          }
+          if ((own < other) == (((tid & j) != 0) == ((tid & size) == 0))) own = other;
+        }
+      return own;
+    };
+    __syncthreads();
+    // by falling logit, then by rising index
+    const u64 own = sort(tid < n ? sh.list[tid] : ~0ull);
+    const unsigned key = ~(unsigned)(own >> 32);
+    bool stay = tid < n && (!use_k || tid < k);
+    const u64 w = stay ? weight(value_of<T>(key)) : 0;
+    if (use_p) {
+      const u64 upto = block_scan(w, sh);
+      if (goal == 0) {
+        if (tid == kThreads - 1) sh.found_before = upto;
+        __syncthreads();
+        goal = share(sh.found_before);
+      }
+      stay = stay && upto - w < goal;
+    }
+    stay = stay && key >= cut;
+    // what stays, by rising index
+    if (tid < kList) sh.list_weight[tid] = w;
+    const u64 next = sort(stay ? own << 32 | (unsigned)tid : ~0ull);
+    __syncthreads();
+    const u64 its = next != ~0ull ? sh.list_weight[(unsigned)next] : 0, upto = block_scan(its, sh);
+    if (tid == kThreads - 1) sh.found_before = upto;
+    __syncthreads();
+    const u64 t = target(sh.found_before);
+    if (upto - its <= t && t < upto) p.tokens[b] = (long long)(next >> 32);
+  };
+  // The same by counting, for each token, those ahead of it.
   auto finish = [&](int n, u64 goal) {
+    if (n > kCount) {
+      finish_sorted(n, goal);
+      return;
+    }
     int parts = 1;  // neighbouring lanes that share a token
     while (parts < 32 && n * parts * 2 <= kThreads) parts *= 2;
     const int i = tid / parts, sub = tid % parts;
@@ -423,8 +473,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     __syncthreads();
     int rank_of = 0;
     u64 before = 0;
-    for (int j = sub; j < n && (use_k || use_p); j += parts)
-      if (sh.list[j] < own) ++rank_of, before += sh.list_weight[j];
+    if (use_k || use_p) {
+#pragma unroll 8
+      for (int j = sub; j < n; j += parts) {
+        const u64 x = sh.list_weight[j];
+        const bool ahead = sh.list[j] < own;
+        rank_of += ahead, before += ahead ? x : 0;
+      }
+    }
     for (int m = 1; m < parts; m <<= 1) {
       rank_of += __shfl_xor_sync(~0u, rank_of, m);
       before += __shfl_xor_sync(~0u, before, m);
@@ -442,20 +498,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     stay = stay && key >= cut;
     __syncthreads();
     if (i < n && sub == 0) sh.list_weight[i] = stay ? w : 0;
+    const u64 sum = block_scan(stay && sub == 0 ? w : 0, sh);
+    if (tid == kThreads - 1) sh.found_before = sum;
     __syncthreads();
-    u64 total = 0;
+    if (!__any_sync(~0u, stay)) return;
     before = 0;
+#pragma unroll 8
     for (int j = sub; j < n; j += parts) {
       const u64 x = sh.list_weight[j];
-      total += x;
-      if ((unsigned)sh.list[j] < (unsigned)own) before += x;
+      before += (unsigned)sh.list[j] < (unsigned)own ? x : 0;
     }
-    for (int m = 1; m < parts; m <<= 1) {
-      total += __shfl_xor_sync(~0u, total, m);
-      before += __shfl_xor_sync(~0u, before, m);
-    }
+    for (int m = 1; m < parts; m <<= 1) before += __shfl_xor_sync(~0u, before, m);
     if (stay && sub == 0) {
-      const u64 t = target(total);
+      const u64 t = target(sh.found_before);
       if (before <= t && t < before + w) p.tokens[b] = (long long)(unsigned)own;
     }
   };
@@ -553,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     if (at < kRoom) sh.list[at] = (u64)~key << 32 | (unsigned)index;
   };
 
-  if (p.vocab <= 128) {  // C is 1; 10 to 14 us instead of 20 to 37. At 512 ranking takes 43 us, the rest 12 to 35.
+  if (p.vocab <= 128) {  // C is 1
     if (tid == 0) sh.listed = 0;
     __syncthreads();
     for_each([&](int i, float l) {
