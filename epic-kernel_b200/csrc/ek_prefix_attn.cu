@@ -965,6 +965,8 @@ int make_plan(const EkPrefixAttnArgs* a, Plan& pl) {
   if (a->prefix_len < 0 || a->own_capacity < 0 || a->max_own_len < 0 || a->max_own_len > a->own_capacity)
     return fail(EK_E_INVALID, "bad lengths prefix_len=%d own_capacity=%d max_own_len=%d", a->prefix_len,
                 a->own_capacity, a->max_own_len);
+  if (a->prefix_len > 1 << 30 || a->own_capacity > 1 << 30)
+    return fail(EK_E_UNSUPPORTED, "more than %d rows", 1 << 30);
   if ((long long)a->batch * a->q_heads > (1 << 22))
     return fail(EK_E_UNSUPPORTED, "batch * q_heads beyond %d", 1 << 22);
   int sms = 0;
@@ -1028,7 +1030,7 @@ int encode_rows(RowMap& m, const EkKvTensor& t, int batch, int rows, int heads, 
                {batch, t.stride_batch * size, &m.batch, false}};
   long long widest = d * size;
   for (Dim& x : dims) {
-    if (x.n == 1 || x.stride == 0) x.n = 1, x.stride = 0;  // not there; a repeated row needs one entry only
+    if (x.n == 1 || x.stride == 0) x.n = 1, x.stride = 0;  // not there: a repeated head or sequence
     if (x.stride > widest) widest = x.stride;
   }
   for (Dim& x : dims)
@@ -1055,13 +1057,14 @@ int encode_rows(RowMap& m, const EkKvTensor& t, int batch, int rows, int heads, 
 }
 
 // Fills one side of `s`; checks alignment and kind when there are rows.
-int take_store(const EkKvTensor& k, const EkKvTensor& v, bool rows, bool i8, const char* name, Store& s) {
+int take_store(const EkKvTensor& k, const EkKvTensor& v, int rows, bool i8, const char* name, Store& s) {
   using ek::fail;
-  if (rows) {
+  if (rows > 0) {
     const int unit = i8 ? 16 : 8;
     for (const EkKvTensor* t : {&k, &v}) {
       if (!t->data || !ek::aligned16(t->data) || t->stride_batch % unit || t->stride_row % unit || t->stride_head % unit)
         return fail(EK_E_INVALID, "%s rows must be 16-byte aligned with strides of 16 bytes", name);
+      if (rows > 1 && t->stride_row == 0) return fail(EK_E_INVALID, "%s rows with a stride of 0", name);
       if ((t->scales != nullptr) != i8) return fail(EK_E_INVALID, "prefix and own rows must be of one kind");
     }
   }
@@ -1145,11 +1148,12 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
     return fail(EK_E_INVALID, "out must be 16-byte aligned with strides of 16 bytes");
   if (pl.part_bytes > 0 && (!a->workspace || !ek::aligned16(a->workspace) || a->workspace_bytes < pl.part_bytes))
     return fail(EK_E_INVALID, "workspace of %lld bytes, 16-byte aligned, needed", pl.part_bytes);
+  ek::DeviceGuard g(a->device);
   const bool i8 = (a->prefix_len > 0 ? a->prefix_k.scales : a->own_k.scales) != nullptr;
   FewParams few;
   AttnParams& p = few.a;
-  if ((rc = take_store(a->prefix_k, a->prefix_v, a->prefix_len > 0, i8, "prefix", p.prefix))) return rc;
-  if ((rc = take_store(a->own_k, a->own_v, a->max_own_len > 0, i8, "own", p.own))) return rc;
+  if ((rc = take_store(a->prefix_k, a->prefix_v, a->prefix_len, i8, "prefix", p.prefix))) return rc;
+  if ((rc = take_store(a->own_k, a->own_v, a->max_own_len > 0 ? a->own_capacity : 0, i8, "own", p.own))) return rc;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.q_batch = a->q_stride_batch, p.q_head = a->q_stride_head;
   p.out = static_cast<__nv_bfloat16*>(a->out);
@@ -1200,7 +1204,6 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
     return rc;
   }
   const ManyParams* many = pl.many ? &m : nullptr;
-  ek::DeviceGuard g(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (a->head_dim == 64) e = i8 ? launch<64, true>(few, many, st) : launch<64, false>(few, many, st);

@@ -35,6 +35,7 @@ struct Api {
 [[noreturn]] void refuse(const std::string& why) { throw py::value_error(why); }
 
 void check(int rc, const char* what) {
+  if (rc == EK_E_INVALID || rc == EK_E_UNSUPPORTED) refuse(std::string(what) + ": " + api.last_error());
   if (rc != 0)
     throw std::runtime_error(std::string(what) + " failed (code " + std::to_string(rc) + "): " + api.last_error());
 }
@@ -90,6 +91,11 @@ void no_overlap(const Tensor& t, const char* name) {
   }
 }
 
+// K and V are written by different blocks.
+void apart(const Tensor& k, const Tensor& v, const char* what) {
+  if (k.numel() && k.data_ptr() == v.data_ptr()) refuse(std::string(what) + ": K and V are the same memory");
+}
+
 int64_t step(const Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
 
 // Descriptor of [batch, row, head, D] rows; a 3-D tensor has no batch.
@@ -105,6 +111,11 @@ EkKvTensor describe(const Tensor& data, const Tensor* scales) {
     r.scale_stride_head = step(*scales, 2);
   }
   return r;
+}
+
+// Rows [.., row, head, D] that copies of several rows can take: one row shown as many would need a stride of 0.
+void distinct_rows(const Tensor& t, const char* name) {
+  if (t.size(-3) > 1 && t.stride(-3) == 0) refuse(std::string(name) + ": a row repeated by expand; make it contiguous");
 }
 
 int fit32(int64_t n, const char* name) {
@@ -150,8 +161,9 @@ void kv_copy(bool write, const py::tuple& cache, py::handle ko, py::handle vo, p
   if (write) {
     no_overlap(*c.kc, "k_codes"), no_overlap(*c.ks, "k_scales");
     no_overlap(*c.vc, "v_codes"), no_overlap(*c.vs, "v_scales");
+    apart(*c.kc, *c.vc, "cache codes"), apart(*c.ks, *c.vs, "cache scales");
   } else {
-    no_overlap(k, "out[0]"), no_overlap(v, "out[1]");
+    no_overlap(k, "out[0]"), no_overlap(v, "out[1]"), apart(k, v, "out");
   }
   EkKvCopyArgs a = {};
   a.k_values = describe(k, nullptr), a.v_values = describe(v, nullptr);
@@ -191,6 +203,8 @@ py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& ow
     if (p.kc->size(0) != 1) refuse("prefix: batch " + std::to_string(p.kc->size(0)) + ", expected 1");
     a.prefix_k = describe(*p.kc, p.ks), a.prefix_v = describe(*p.vc, p.vs);
     a.own_k = describe(*o.kc, o.ks), a.own_v = describe(*o.vc, o.vs);
+    distinct_rows(*p.kc, "prefix k_codes"), distinct_rows(*p.vc, "prefix v_codes");
+    distinct_rows(*o.kc, "own k_codes"), distinct_rows(*o.vc, "own v_codes");
     pk = p.kc, ok = o.kc;
     prefix_len = pk->size(1);
   } else {
@@ -202,6 +216,8 @@ py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& ow
     if (pk->sizes() != pv.sizes() || ok->sizes() != ov.sizes()) refuse("k and v must have the same shape");
     a.prefix_k = describe(*pk, nullptr), a.prefix_v = describe(pv, nullptr);
     a.own_k = describe(*ok, nullptr), a.own_v = describe(ov, nullptr);
+    distinct_rows(*pk, "prefix k"), distinct_rows(pv, "prefix v");
+    distinct_rows(*ok, "own k"), distinct_rows(ov, "own v");
     prefix_len = pk->size(0);
   }
   const int64_t kv_heads = ok->size(2), rows = ok->size(1);
@@ -238,7 +254,7 @@ py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& ow
   a.scale = (float)s;
   a.device = q.device().index();
   a.workspace_bytes = api.attention_workspace(&a);
-  if (a.workspace_bytes < 0) check(1, "ek_prefix_attention_workspace");
+  if (a.workspace_bytes < 0) refuse(std::string("shared_prefix_attention: ") + api.last_error());
   Tensor workspace = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte));
   a.workspace = workspace.data_ptr();
   check(api.attention(&a, stream_of(q)), "ek_prefix_attention");

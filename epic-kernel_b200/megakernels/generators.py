@@ -51,6 +51,8 @@ class _Sampler:
 
     def __call__(self, logits: Tensor, out: Tensor | None = None) -> Tensor:
         p = self.params
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("sampling cannot be captured: a replay would use the same random numbers again")
         if self.step == self.STEPS:
             self.uniforms = torch.rand((self.STEPS, self.rows), generator=p.generator, device=logits.device)
             self.step = 0
@@ -164,8 +166,8 @@ class MK_Generator(Generator):
 class ParallelGenerator(Generator):
     """Decodes `num_sequences` continuations of one prompt at once.
 
-    The prompt's K/V rows stay in the model's cache (`kv_cache="bf16"`) or are
-    quantised once (`"int8"`); each sequence has a cache of its own, of the same
+    The prompt's K/V rows stay in the model's cache (`kv_cache="bf16"`: nothing
+    else may write them meanwhile) or are quantised once (`"int8"`); each sequence has a cache of its own, of the same
     kind, for up to `max_new_tokens` tokens. The projections are dense products,
     as in the model's prefill. model: a LlamaForCausalLM on a CUDA device."""
 

@@ -165,8 +165,9 @@ def shared_prefix_attention(q: Tensor, prefix, own, own_lens: Tensor, *, scale: 
 
     Returns bf16 `[batch, q_heads, head_dim]` (`out` if given), with
     `return_lse` also the natural log of the softmax sum, f32 `[batch, q_heads]`.
-    A row without any key gives zeros and -inf. Only the first own_lens[b] rows
-    are read. Scores, softmax and sums are fp32; the probabilities are rounded
+    A row without any key gives zeros and -inf. What lies behind the first
+    own_lens[b] rows has no effect, NaN included. Caches may repeat heads or
+    sequences (expand), not rows. Scores, softmax and sums are fp32; the probabilities are rounded
     to bf16 for the product with V."""
     return _native().attention(q, _tensors_of(prefix, "prefix"), _tensors_of(own, "own"), own_lens, scale,
                                max_own_len, out, return_lse)

@@ -164,3 +164,28 @@ def test_generator_refuses():
         gen.hand_over(2)
     with pytest.raises(ValueError, match="ntok_already_generated"):
         gen.generate(torch.zeros(2, 4, dtype=torch.int64, device="cuda"), PROMPT, 1, 1)
+
+
+def test_a_second_prompt_starts_over():
+    """After longer use, a shorter prompt gives what a new generator gives."""
+    for kind in ("bf16", "int8"):
+        model, gen, _, _ = generate(kind, 3)
+        fresh = type(gen)(model, 3, NEW, sampling=params(seed=9, top_k=20), kv_cache=kind)
+        gen.sampler = type(gen.sampler)(params(seed=9, top_k=20), 3)
+        got = []
+        for g in (gen, fresh):
+            out = torch.zeros(3, NEW + 1, dtype=torch.int64, device="cuda")
+            out[:, 0] = g.prefill(ids(17, seed=4))
+            g.generate(out, 17, NEW)
+            got.append(out)
+        assert torch.equal(*got)
+
+
+def test_sampled_steps_are_not_captured():
+    gen = generate("bf16", 2)[1]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            gen.sampler(gen.logits)
+    torch.cuda.synchronize()
+    assert gen.sampler(gen.logits).shape == (2,)

@@ -151,3 +151,31 @@ def test_cache_refuses_on_the_gpu():
     refuses("overlap", ops.kv_cache_write, expanded, k, k, 0)
     assert ops.kv_cache_read(cache, 6, 0)[0].shape == (2, 0, 2, 64)
     ops.kv_cache_write(cache, k[:, :0], k[:, :0], 6)
+
+
+@pytest.mark.gpu
+def test_memory_shared_within_a_call_is_refused():
+    q, lens = cuda(3, 8, 64), cuda(3, dtype=torch.int32)
+    prefix, own = (cuda(5, 2, 64), cuda(5, 2, 64)), (cuda(3, 6, 2, 64), cuda(3, 6, 2, 64))
+    row = cuda(1, 2, 64).expand(5, 2, 64)  # one row shown as five
+    refuses("prefix k: a row repeated", ops.shared_prefix_attention, q, (row, prefix[1]), own, lens)
+    refuses("own v: a row repeated", ops.shared_prefix_attention, q, prefix, (own[0], cuda(3, 1, 2, 64).expand(3, 6, 2, 64)), lens)
+    c = ops.KVCacheInt8.empty(3, 6, 2, 64)
+    one = ops.KVCacheInt8(*(t[:, :1].expand(t.shape) for t in c._tensors()))
+    refuses("own k_codes: a row repeated", ops.shared_prefix_attention, q, c.sequence(0), one, lens)
+    same = ops.KVCacheInt8(c.k_codes, c.k_scales, c.k_codes, c.v_scales)
+    k = cuda(3, 1, 2, 64)
+    refuses("same memory", ops.kv_cache_write, same, k, k, 0)
+    refuses("same memory", ops.kv_cache_read, c, 0, 1, out=(k, k))
+
+
+@pytest.mark.gpu
+def test_sizes_beyond_the_kernels_are_value_errors():
+    many = ops.KVCacheInt8.empty(65536, 1, 1, 64)
+    k = cuda(65536, 1, 1, 64)
+    refuses("batch 65536", ops.kv_cache_write, many, k, k, 0)
+    refuses("batch 65536", ops.kv_cache_read, many, 0, 1)
+    n = (1 << 22) + 1
+    q, lens = cuda(1, 1, 64).expand(n, 1, 64), cuda(n, dtype=torch.int32)
+    prefix, own = (cuda(5, 1, 64), cuda(5, 1, 64)), tuple(cuda(1, 1, 1, 64).expand(n, 1, 1, 64) for _ in range(2))
+    refuses("batch \\* q_heads", ops.shared_prefix_attention, q, prefix, own, lens)
