@@ -20,7 +20,7 @@
 // short row): at least k logits lie at or above the bin where k are reached. bf16
 // logits take few values: without top-k their weights come from a table of
 // values, and for top-p a count per value gives the cut in one pass (64 rows of
-// 128256 logits with top-p 0.95: 66 us before the table, 45 with it).
+// 128256 logits with top-p 0.95: 66 us before the table, 44 with it).
 //
 // A row is spread over a cluster of 1 to 8 blocks that hold it in shared
 // memory, so it is read from HBM once; the blocks exchange maxima, histograms
@@ -301,11 +301,21 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     }
   } else {
     constexpr int U = 4;
-    for (int i = tid; i - lane < vectors; i += U * kThreads) {  // whole warps
-      V16 v[U];
+    V16 v[U], next[U];
+    auto load = [&](V16 (&x)[U], int i) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < vectors) v[u] = fetch(i + u * kThreads);
+        if (i + u * kThreads < vectors) x[u] = fetch(i + u * kThreads);
+    };
+    if (!RESIDENT) load(next, tid);  // long slices: the next loads are under way while these are looked at
+    for (int i = tid; i - lane < vectors; i += U * kThreads) {  // whole warps
+      if (RESIDENT) {
+        load(v, i);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
+        load(next, i + U * kThreads);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i + u * kThreads < vectors) {
@@ -459,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   };
   // The same by counting, for each token, those ahead of it.
   auto finish = [&](int n, u64 goal) {
-    if (n > kCount) {
+    if (kThreads == 1024 || n > kCount) {  // 1024 threads have no registers for both (64 rows, top-p: 48 us, 44 without)
       finish_sorted(n, goal);
       return;
     }
