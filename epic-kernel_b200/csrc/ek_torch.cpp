@@ -151,10 +151,7 @@ Cache take_cache(const py::tuple& t, const char* name, const Tensor* like = null
 
 void check_cache(const py::tuple& t) { take_cache(t, "cache"); }
 
-void kv_copy(bool write, const py::tuple& cache, py::handle ko, py::handle vo, py::handle start) {
-  const Cache c = take_cache(cache, "cache");
-  const Tensor& k = rows16(need(ko.ptr(), write ? "k" : "out[0]", at::kBFloat16, 4, c.kc), write ? "k" : "out[0]");
-  const Tensor& v = rows16(need(vo.ptr(), write ? "v" : "out[1]", at::kBFloat16, 4, c.kc), write ? "v" : "out[1]");
+void kv_copy(bool write, const Cache& c, const Tensor& k, const Tensor& v, py::handle start) {
   if (k.sizes() != v.sizes() || k.size(0) != c.kc->size(0) || k.sizes().slice(2) != c.kc->sizes().slice(2))
     refuse("k " + shape_of(k) + " / v " + shape_of(v) + ": expected [batch, rows, kv_heads, head_dim] as in the cache " +
            shape_of(*c.kc));
@@ -186,6 +183,32 @@ void kv_copy(bool write, const py::tuple& cache, py::handle ko, py::handle vo, p
   if (a.kv_heads == 0 || a.batch == 0 || a.length == 0) return;
   a.device = c.kc->device().index();
   check((write ? api.kv_write : api.kv_read)(&a, stream_of(k)), write ? "ek_kv_write" : "ek_kv_read");
+}
+
+void kv_write(const py::tuple& cache, py::handle ko, py::handle vo, py::handle start) {
+  const Cache c = take_cache(cache, "cache");
+  const Tensor& k = rows16(need(ko.ptr(), "k", at::kBFloat16, 4, c.kc), "k");
+  const Tensor& v = rows16(need(vo.ptr(), "v", at::kBFloat16, 4, c.kc), "v");
+  kv_copy(true, c, k, v, start);
+}
+
+py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::handle out) {
+  const Cache c = take_cache(cache, "cache");
+  if (length < 0) refuse("length " + std::to_string(length));
+  if (out.is_none()) {
+    const Tensor both = at::empty({2, c.kc->size(0), length, c.kc->size(2), c.kc->size(3)}, c.ks->options());
+    const Tensor k = both.select(0, 0), v = both.select(0, 1);
+    kv_copy(false, c, k, v, start);
+    return py::make_tuple(k, v);
+  }
+  const py::sequence pair = py::reinterpret_borrow<py::sequence>(out);
+  if (pair.size() != 2) refuse("out: expected a (k, v) pair");
+  const py::object ko = pair[0], vo = pair[1];
+  const Tensor& k = rows16(need(ko.ptr(), "out[0]", at::kBFloat16, 4, c.kc), "out[0]");
+  const Tensor& v = rows16(need(vo.ptr(), "out[1]", at::kBFloat16, 4, c.kc), "out[1]");
+  if (k.size(1) != length) refuse("out: " + std::to_string(k.size(1)) + " rows, expected " + std::to_string(length));
+  kv_copy(false, c, k, v, start);
+  return py::make_tuple(ko, vo);
 }
 
 py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& own, py::handle lens_o,
@@ -352,7 +375,8 @@ void bind(const py::dict& d) {
 PYBIND11_MODULE(_ekops, m) {
   m.def("bind", &bind);
   m.def("check_cache", &check_cache);
-  m.def("kv_copy", &kv_copy);
+  m.def("kv_write", &kv_write);
+  m.def("kv_read", &kv_read);
   m.def("attention", &attention);
   m.def("sample", &sample);
 }

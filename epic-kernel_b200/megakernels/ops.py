@@ -120,7 +120,7 @@ def kv_cache_write(cache: KVCacheInt8, k: Tensor, v: Tensor, start: int | Tensor
     Per (row, head): scale = max|x| / 127 rounded up to bf16 (at least 2^-126),
     code = x / scale rounded half away from zero, so a value is off by at most
     half a scale. A head holding a NaN or an infinity reads back as NaN."""
-    _native().kv_copy(True, _cache_tensors(cache), k, v, start)
+    _native().kv_write(_cache_tensors(cache), k, v, start)
 
 
 def kv_cache_read(cache: KVCacheInt8, start: int | Tensor, length: int,
@@ -129,19 +129,7 @@ def kv_cache_read(cache: KVCacheInt8, start: int | Tensor, length: int,
     (k, v) of `[batch, length, kv_heads, head_dim]`, into `out` if given (two
     bf16 tensors, which may be views into the model's cache). `start` as in
     `kv_cache_write`; with a tensor, rows outside the cache read as zeros."""
-    tensors = _cache_tensors(cache)
-    if length < 0:
-        raise ValueError(f"length {length}")
-    if out is None:
-        codes = tensors[0]
-        b, _, h, d = codes.shape
-        both = torch.empty((2, b, length, h, d), dtype=torch.bfloat16, device=codes.device)
-        out = both[0], both[1]
-    k, v = out
-    if k.dim() > 1 and k.shape[1] != length:
-        raise ValueError(f"out: {k.shape[1]} rows, expected {length}")
-    _native().kv_copy(False, tensors, k, v, start)
-    return k, v
+    return _native().kv_read(_cache_tensors(cache), start, length, out)
 
 
 def shared_prefix_attention(q: Tensor, prefix, own, own_lens: Tensor, *, scale: float | None = None,
