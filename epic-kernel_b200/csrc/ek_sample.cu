@@ -1188,7 +1188,8 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
     cluster *= 2;
   // Beyond 148 rows two blocks of 512 with the table share an SM while the row leaves room (155 rows of 19592: 33 us,
   // 42 on 1 x 1024; 32000: 61 and 51).
-  const bool pairs = by_value && batch > 148 && slice(1) * size <= 40 * 1024;
+  const int block_bytes = slice(1) * size + kTableBytes + (int)sizeof(Shared<512>) + 1024;
+  const bool pairs = by_value && batch > 148 && 2 * block_bytes <= 228 * 1024;
   if (pairs) {
     cluster = 1;
   } else if (by_value || slice(cluster) >= 32000 || slice(cluster) * size > 72 * 1024) {
