@@ -957,10 +957,10 @@ struct Plan {
 };
 
 // many_rows takes the prefix from here on: more than two tiles of 8 query rows per KV head, and that many elements of
-// K that few_rows would go through, its tiles of 8 rows times the prefix. Times of whole calls in us, few against many:
-// 16 heads of 128, bf16, 32768 rows of prefix: 68 / 70 at 16 query rows, 84 / 72 at 24; 4096 rows: 31 / 31 at 32
-// (2^25 elements), 37 / 33 at 48. 8 heads, 8192 rows, 32 query rows (2^25): 25 / 25 bf16, 33 / 31 int8. int8, 16 heads,
-// 32768 rows: 90 / 106 at 16 query rows, 125 / 108 at 24. 8 heads, 512 rows: 22 / 31 at 256 query rows, 59 / 49 at 1024.
+// K that few_rows would go through, its tiles of 8 rows times the prefix. Times of whole calls in us, few against many,
+// heads of 128: 16 KV heads, bf16, 32768 rows of prefix: 70 / 72 at 16 query rows, 88 / 74 at 24; 4096 rows: 33 / 31 at
+// 32 (2^25 elements), 39 / 35 at 48. 8 KV heads, 8192 rows, 32 query rows (2^25): 27 / 27 bf16, 35 / 31 int8; 512 rows:
+// 22 / 31 at 256 query rows, 61 / 49 at 1024. int8, 16 KV heads, 32768 rows: 93 / 96 at 16 query rows, 127 / 97 at 24.
 constexpr int kManyFrom = 17;
 constexpr long long kManyElements = 1ll << 25;
 
