@@ -876,10 +876,12 @@ constexpr int kJoinWarps = 8;
 template <int D, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) join(const AttnParams p) {
   constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
-  wait_before();
   const long long row = W == 1 ? blockIdx.x * 4ll + threadIdx.x / 32 : blockIdx.x, rows = (long long)p.batch * p.q_heads;
   const int lane = threadIdx.x % 32, sub = lane / LANES, piece = lane % LANES, warp = W == 1 ? 0 : threadIdx.x / 32;
-  if (W == 1 && row >= rows) return;
+  if (W == 1 && row >= rows) {
+    wait_before();
+    return;
+  }
   const int b = (int)(row / p.q_heads), h = (int)(row % p.q_heads);
   const int len = min(max(p.own_lens[b], 0), p.max_own);
   const int shared = b * p.group + h % p.group < p.wide_rows ? p.wide_slots : p.narrow_slots;
@@ -888,6 +890,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) join(const AttnParams p
     const int i = j * W + warp;
     return (long long)(i < shared ? i : i - shared + p.prefix_slots) * rows + row;
   };
+  wait_before();  // the lengths are inputs, what follows is not
   float top = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < parts; i0 += 32) {
