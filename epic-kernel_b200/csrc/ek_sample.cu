@@ -123,10 +123,13 @@ __device__ __forceinline__ float value_of(unsigned key) {
 // 0.0109 leaves an error below 0.0109^6 / 720 = 2.4e-15. The middle one is a
 // table. Both roundings to whole numbers are additions of 1.5 * 2^52.
 // An infinite maximum (then only infinite logits are weighed) counts as the largest finite number.
+// Logits below `low` (and NaN) weigh 0: their weight is less than half a unit, and further down n div 32 is not the
+// exponent of a number any more.
 struct Weight {
   double top, c;       // c = 32 log2(e) / T
   const double* table; // 2^(j / 32), shared memory
   int bits;
+  float low;
 
   __device__ __forceinline__ u64 operator()(float l) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
@@ -144,7 +147,7 @@ struct Weight {
     p *= table[n & 31];
     p = __hiloint2double(__double2hiint(p) + ((n >> 5) + bits) * (1 << 20), __double2loint(p));
     const double whole = p + 4503599627370496.0;  // 2^52: the low bits are the rounded p
-    return (u64)__double_as_longlong(whole) & 0xfffffffffffffull;
+    return l >= low ? (u64)__double_as_longlong(whole) & 0xfffffffffffffull : 0;
   }
 };
 
@@ -436,9 +439,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     }
     return;
   }
-  const Weight weight{(double)fminf(top, 3.402823466e38f), sh.c, sh.table, p.weight_bits};
   // below `low` a weight rounds to 0 and the token can never be drawn
   low = fmaxf(low, __double2float_ru((double)top - (double)temp * (0.6931471805599453 * (p.weight_bits + 1))));
+  const Weight weight{(double)fminf(top, 3.402823466e38f), sh.c, sh.table, p.weight_bits, low};
   const float u01 = p.uniforms[b];
   // the draw among a weight of `total`: the first token whose running weight exceeds this
   auto target = [&](u64 total) {
@@ -449,13 +452,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   auto share = [&](u64 total) { return max((u64)ceil((double)fmaxf(top_p, 0.f) * (double)total), 1ull); };
 
   // ---- cuts: keys above `cut` stay, and the first `ties` (by index) of those equal to it
-  unsigned cut = key_of<T>(low);
+  // (the first value of the logits' type at or above a border: a key of bf16 is cut off downwards for positive logits)
+  auto first_key = [&](float l) { return key_of<T>(sizeof(T) == 2 ? __bfloat162float(__float2bfloat16_ru(l)) : l); };
+  unsigned cut = first_key(low);
   u64 ties = ~0ull;
-  if (min_p > 0.f) {
-    float l = __double2float_ru((double)top + sh.min_offset);
-    if (sizeof(T) == 2) l = __bfloat162float(__float2bfloat16_ru(l));  // the next bf16 at or above
-    cut = max(cut, key_of<T>(fminf(l, top)));
-  }
+  if (min_p > 0.f) cut = max(cut, first_key(fminf(__double2float_ru((double)top + sh.min_offset), top)));
 
   // Finishes the row from the n <= kList listed tokens, which are all that may stay. `goal`: the weight for top-p, 0 if
   // it follows from the list.
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   if (table && !use_p && !(min_p > 0.f)) {  // min-p leaves too few weights
     for (int i = tid; i < kValues; i += kThreads) {
       const float l = value_at(i);
-      weight_at[i] = l >= low && l <= top ? weight(l) : 0;
+      weight_at[i] = l <= top ? weight(l) : 0;
     }
     __syncthreads();
     by_value = true;
@@ -893,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
         for_each_by_warp([&](int i, const float (&l)[kBatch]) {
           u64 w[kBatch];
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u) w[u] = weight(fmaxf(l[u], low));
+          for (int u = 0; u < kBatch; ++u) w[u] = weight(l[u]);
           unsigned hits = 0;
 #pragma unroll
           for (int u = 0; u < kBatch; ++u) {
@@ -1040,7 +1041,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
       if (!any) return;
       u64 w[kBatch];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) w[u] = weight(fmaxf(l[u], cut_value));
+      for (int u = 0; u < kBatch; ++u) w[u] = weight(l[u]);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) above += l[u] > cut_value ? w[u] : 0;
     });
