@@ -45,7 +45,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxCluster = 8;
-constexpr int kMaxElements = 65536;    // per block: a bin's 16-bit limbs add up below 2^32
+constexpr int kMaxElements = 65536;    // of a slice held in shared memory
 constexpr int kMaxBytes = 176 * 1024;  // of logits per block
 constexpr int kBatch = 4;
 constexpr int kList = 512;   // tokens that one block ranks
@@ -59,6 +59,14 @@ constexpr int kValues = 4096;
 constexpr int kTableBytes = kValues * (sizeof(unsigned) + sizeof(unsigned long long));  // counts, weights
 constexpr int kMaxVocab = kMaxCluster * kMaxBytes / 4;
 using u64 = unsigned long long;
+
+// Weights (up to 2^46) are added up in 32-bit limbs, the last with what is left: 16 bits each when a block sees a slice,
+// 13 when it sees a whole row, so that no sum of equal weights reaches 2^32.
+template <bool RESIDENT>
+struct Limbs {
+  static constexpr int N = RESIDENT ? 3 : 4, BITS = RESIDENT ? 16 : 13, MOST = RESIDENT ? kMaxElements : kMaxVocab;
+  static_assert(((1ull << BITS) - 1) * MOST < 1ull << 32 && (1ull << (46 - BITS * (N - 1))) * MOST < 1ull << 32, "limbs");
+};
 
 struct SampleParams {
   const void* logits;
@@ -151,10 +159,10 @@ struct Weight {
   }
 };
 
-template <int kThreads>
+template <int kThreads, int kLimbs>
 struct Shared {
   static constexpr int kWarps = kThreads / 32, kBins = kThreads;
-  unsigned hist[2][3][kBins];  // counts, or the three 16-bit limbs of weights
+  unsigned hist[2][kLimbs][kBins];  // counts, or the limbs of weights
   double table[32];
   double c, min_offset;        // 32 log2(e) / T; T ln(min_p)
   u64 scan[kWarps];
@@ -185,8 +193,8 @@ __device__ __forceinline__ u64 quotient_up(u64 a, u64 b) {
 }
 
 // Inclusive scan over the block's threads.
-template <int kThreads>
-__device__ u64 block_scan(u64 v, Shared<kThreads>& sh) {
+template <int kThreads, int kLimbs>
+__device__ u64 block_scan(u64 v, Shared<kThreads, kLimbs>& sh) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
@@ -234,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   extern __shared__ uint4 dynamic[];
   T* slice = reinterpret_cast<T*>(dynamic);
   u64* raw_list = reinterpret_cast<u64*>(dynamic);  // without a resident slice
-  __shared__ Shared<kThreads> sh;
+  using L = Limbs<RESIDENT>;
+  __shared__ Shared<kThreads, L::N> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = RESIDENT ? cluster.num_blocks() : 1, rank = RESIDENT ? cluster.block_rank() : 0;
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
   if (warp == 1) sh.table[lane] = exp2((double)lane / 32.0);
   if (warp == 2 && lane == 0) sh.c = 46.166241308446828 / (double)temp;
   if (warp == 3 && lane == 0) sh.min_offset = min_p > 0.f ? (double)temp * log((double)fminf(min_p, 1.f)) : 0.0;
-  for (int i = tid; i < 3 * kBins; i += kThreads) sh.hist[0][0][i] = 0;
+  for (int i = tid; i < L::N * kBins; i += kThreads) sh.hist[0][0][i] = 0;
 #pragma unroll
   for (int m = 16; m; m >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
@@ -561,6 +570,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
       if (before <= t && t < before + w) p.tokens[b] = (long long)(unsigned)own;
     }
   };
+  auto add_weight = [&](int buffer, int bin, u64 w) {
+#pragma unroll
+    for (int e = 0; e < L::N; ++e)
+      atomicAdd(&sh.hist[buffer][e][bin], (unsigned)(w >> (L::BITS * e)) & (e + 1 < L::N ? (1u << L::BITS) - 1 : ~0u));
+  };
   if (online && sh.listed <= kRaw) {
     // All kept tokens are listed. Their weights by ranges of the index, 512 of them; the range that holds the draw
     // is small enough to compare its tokens with each other.
@@ -571,12 +585,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
       if (key < cut) continue;  // ruled out by the final maximum
       const int at = (int)((unsigned)own / wide);
       const u64 w = weight(value_of<T>(key));
-      atomicAdd(&sh.hist[0][0][at], (unsigned)w & 0xffffu);
-      atomicAdd(&sh.hist[0][1][at], (unsigned)(w >> 16) & 0xffffu);
-      atomicAdd(&sh.hist[0][2][at], (unsigned)(w >> 32));
+      add_weight(0, at, w);
     }
     __syncthreads();
-    const u64 mine = sh.hist[0][0][tid] + ((u64)sh.hist[0][1][tid] << 16) + ((u64)sh.hist[0][2][tid] << 32);
+    u64 mine = 0;
+#pragma unroll
+    for (int e = 0; e < L::N; ++e) mine += (u64)sh.hist[0][e][tid] << (L::BITS * e);
     const u64 sum = block_scan(mine, sh);
     if (tid == kThreads - 1) sh.found_before = sum;
     __syncthreads();
@@ -617,24 +631,30 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     const float margin = (top - low) * 0x1p-18f + fmaxf(fabsf(top), fabsf(low)) * 0x1p-20f;
     return top - ((float)bin + half) / bins_per - copysignf(margin, half);
   };
-  // The cluster's sum of bin `tid` of the current histogram (one count, or three limbs); call after sync(). Turns
+  // The cluster's sum of bin `tid` of the current histogram (one count, or the limbs); call after sync(). Turns
   // to the other buffer, which is free: its last readers were past it before that barrier.
   auto collect = [&](bool limbs) {
-    unsigned h[3][RESIDENT ? kMaxCluster : 1];
     constexpr int R = RESIDENT ? kMaxCluster : 1;
+    unsigned h[L::N][R];
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (r < C) {
         const unsigned* other = peer(&sh.hist[buffer][0][0], r);
         h[0][r] = other[tid];
-        if (limbs) h[1][r] = other[kBins + tid], h[2][r] = other[2 * kBins + tid];
+#pragma unroll
+        for (int e = 1; e < L::N; ++e)
+          if (limbs) h[e][r] = other[e * kBins + tid];
       }
     u64 sum = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (r < C) sum += limbs ? h[0][r] + ((u64)h[1][r] << 16) + ((u64)h[2][r] << 32) : (u64)h[0][r];
+      if (r < C) {
+        sum += h[0][r];
+#pragma unroll
+        for (int e = 1; e < L::N; ++e) sum += limbs ? (u64)h[e][r] << (L::BITS * e) : 0;
+      }
     buffer ^= 1;
-    for (int i = tid; i < 3 * kBins; i += kThreads) sh.hist[buffer][0][i] = 0;
+    for (int i = tid; i < L::N * kBins; i += kThreads) sh.hist[buffer][0][i] = 0;
     return sum;
   };
   // All blocks' lists together in the first block's: their number, or -1 (nothing moved) if they are too many.
@@ -879,10 +899,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
         if (stage == 0) {
           atomicAdd(&sh.hist[buffer][0][at], 1u);
         } else {
-          const u64 w = weight(l);
-          atomicAdd(&sh.hist[buffer][0][at], (unsigned)w & 0xffffu);
-          atomicAdd(&sh.hist[buffer][1][at], (unsigned)(w >> 16) & 0xffffu);
-          atomicAdd(&sh.hist[buffer][2][at], (unsigned)(w >> 32));
+          add_weight(buffer, at, weight(l));
         }
       };
       if (weigh && stage == 0) {
@@ -1189,7 +1206,7 @@ cudaError_t launch(SampleParams& p, int batch, cudaStream_t st) {
     cluster *= 2;
   // Beyond 148 rows two blocks of 512 with the table share an SM while the row leaves room (155 rows of 19592: 33 us,
   // 42 on 1 x 1024; 32000: 61 and 51).
-  const int block_bytes = slice(1) * size + kTableBytes + (int)sizeof(Shared<512>) + 1024;
+  const int block_bytes = slice(1) * size + kTableBytes + (int)sizeof(Shared<512, 3>) + 1024;
   const bool pairs = by_value && batch > 148 && 2 * block_bytes <= 228 * 1024;
   if (pairs) {
     cluster = 1;
@@ -1240,7 +1257,7 @@ extern "C" int ek_sample(const EkSampleArgs* a, void* stream) {
   p.top_p_all = a->top_p_all;
   p.min_p_all = a->min_p_all;
   p.vocab = a->vocab;
-  // every sum stays below 2^62, and a weight below 2^48 (three limbs)
+  // every sum stays below 2^62, and a weight is at most 2^46
   int bits = 62;
   for (long long n = 1; n < a->vocab; n *= 2) --bits;
   p.weight_bits = bits < 46 ? bits : 46;
