@@ -592,7 +592,9 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     };
     float next_ks = 0.f, next_vs = 0.f;
     if (I8) next_ks = key_scale(0, 0), next_vs = key_scale(0, 1);
-    for (int use = 0; use < mine; ++use) {
+    // A warp whose wait runs out still comes to the next tile's barrier, where the warpgroup leaves together (with bf16
+    // rows there is none, and it leaves alone).
+    for (int use = 0; use < mine && (I8 || ok); ++use) {
       const int tile = tile0 + (wide ? use : 2 * use + w);
       const int keys = min(128, p.a.prefix_len - tile * 128);
       const float* ks = nullptr;
@@ -603,17 +605,18 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
           if (w == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
           else asm volatile("bar.sync 2, 128;" ::: "memory");
         };
-        sync();  // the scales of the tile before are done with
+        auto agree = [&](bool x) { return w == 0 ? ek::barrier_all<1, 128>(x) : ek::barrier_all<2, 128>(x); };
+        if (!(ok = agree(ok))) break;  // else the scales of the tile before are done with
         sc[t] = next_ks * scale, sc[128 + t] = next_vs;
         sync();
         ks = sc, vs = sc + 128;
         next_ks = key_scale(use + 1, 0), next_vs = key_scale(use + 1, 1);
       }
-      if (!(ok = spin(s_full + w, use & 1))) break;
+      if (!(ok = spin(s_full + w, use & 1))) continue;
       ek::tcgen05_after_sync();
       if (idle) {
         arrive(s_empty);
-        if (use > 0 && !(ok = spin(p_empty + w, (use - 1) & 1))) break;
+        if (use > 0 && !(ok = spin(p_empty + w, (use - 1) & 1))) continue;
       } else {
         uint32_t x[4][32];
 #pragma unroll
@@ -651,7 +654,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         const float grown = ek::max3_nan(m, high, high);
         if (use == 0) m = grown;
         // O and P are free once the products of the tile before are done
-        if (use > 0 && !(ok = spin(p_empty + w, (use - 1) & 1))) break;
+        if (use > 0 && !(ok = spin(p_empty + w, (use - 1) & 1))) continue;
         ek::tcgen05_after_sync();
         const bool far = grown > m + 8.f || grown != grown;
         if (__any_sync(~0u, far)) {

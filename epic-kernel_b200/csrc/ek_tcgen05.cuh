@@ -218,6 +218,19 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
+// ---------------------------------------------------------------- barrier with a vote
+// The THREADS threads of named barrier ID wait for one another; whether `x` holds in all of them.
+template <int ID, int THREADS>
+__device__ __forceinline__ bool barrier_all(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x), "n"(ID), "n"(THREADS)
+      : "memory");
+  return r != 0;
+}
+
 // ---------------------------------------------------------------- bounded wait
 // Waits for phase `parity` of `bar`. False once *abort is set, by this wait
 // after about two seconds or by another one.
