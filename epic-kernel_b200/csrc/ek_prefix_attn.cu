@@ -208,10 +208,9 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_consta
       }
       __syncwarp();
     }
-    if (n < steps) {  // gave up: let the copies in flight land
-      int quiet = 0;
-      for (int i = max(0, n - C::STAGES); i < n; ++i) ek::mbar_wait_bounded(full + i % C::STAGES, (i / C::STAGES) & 1, &quiet);
-    }
+    // The last copy of each stage lands before the stages hold O, also where a warp that gave up did not wait for it.
+    int quiet = 0;
+    for (int i = max(0, n - C::STAGES); i < n; ++i) ek::mbar_wait_bounded(full + i % C::STAGES, (i / C::STAGES) & 1, &quiet);
   } else {
     // q of row lane/4 as B fragments
     uint32_t q[KT][2];
@@ -702,8 +701,10 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     }
     if (ok && mine > 0) ok = wait(p_empty + w, (mine - 1) & 1);
     ek::tcgen05_after_sync();
-    if (!ok) m = NAN, l = NAN;  // a wait ran out: the result is NaN and the status is set
-    asm volatile("bar.sync 3, 256;" ::: "memory");  // all products of both warpgroups are done: Q, K and V are free
+    // All products of both warpgroups are done: Q, K and V are free, unless a wait ran out. Then all rows are NaN, and
+    // the status is set.
+    ok = ek::barrier_all<3, 256>(ok);
+    if (!ok) m = NAN, l = NAN;
     if (!idle) {
       const int b = row / p.a.group, h = head * p.a.group + row % p.a.group;
       const long long total_rows = (long long)p.a.batch * p.a.q_heads;
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         to = smem + (I8 ? C::OFF_RAW : is_v ? C::OFF_V : C::OFF_K) + at % stages * BYTES;
       };
       bool is_v;
-      int n = 0, tile, round;
+      int n = 0, tile, round, k_tiles = 0, v_tiles = 0;
       uint64_t *f, *e;
       uint8_t* to;
       for (; n < items; ++n) {
@@ -793,23 +794,15 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
             map.load(to + blk * 16384, blk * 64, head, key, 0, f);
         }
         __syncwarp();
+        k_tiles += !is_v, v_tiles += is_v;
       }
-      if (n < items) {  // gave up: let the copies in flight land, the last of each buffer
-        int quiet = 0;
-        for (int i = max(0, n - 2 * (C::KS + C::VS)); i < n; ++i) {
-          slot(i, is_v, tile, f, e, round, to);
-          bool last = true;
-          for (int j = i + 1; j < n; ++j) {
-            bool v2;
-            int t2, r2;
-            uint64_t *f2, *e2;
-            uint8_t* to2;
-            slot(j, v2, t2, f2, e2, r2, to2);
-            last = last && f2 != f;
-          }
-          if (last) ek::mbar_wait_bounded(f, round & 1, &quiet);
-        }
-      }
+      // The last copy of each buffer lands before the block ends, also where a warp that gave up did not wait for it.
+      int quiet = 0;
+      auto land = [&](uint64_t* f, int stages, int count) {
+        for (int i = max(0, count - stages); i < count; ++i) ek::mbar_wait_bounded(f + i % stages, (i / stages) & 1, &quiet);
+      };
+      if (I8) land(raw_full, RS, n);
+      else land(k_full, C::KS, k_tiles), land(v_full, C::VS, v_tiles);
     } else if (warp == C::SCORES || warp == C::VALUES) {
       // Two warps issue the products, so that neither's waits hold up the other's: the queue of issued products is
       // short, and a thread that issues is in step with the tensor core.

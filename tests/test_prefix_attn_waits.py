@@ -103,3 +103,36 @@ def test_softmax_warps_meet_at_their_barriers(tiles, idle):
         warps = [(0, warp(operations, condition, tiles[0], p)) for p in first]
         warps += [(1, warp(operations, condition, tiles[1], first[0] if tiles[1] > 1 else None)) for _ in range(WARPS)]
         assert run(warps), f"warps that give up at {first} leave others at a barrier"
+
+
+def loader_part(kernel, begin):
+    text = SOURCE[SOURCE.index(kernel + "(const __grid_constant__") :]
+    text = text[text.index(begin) :]
+    return text[: text.index("} else ")]
+
+
+def in_flight_at_the_end(steps, stages, fails_at, only_if_gave_up):
+    """Copies that may still be landing when a block's threads meet after its consumers gave up waiting for copy
+    `fails_at`: the loader issues while a buffer is free and waits for the last copy of each buffer, always or only if
+    it could not issue them all."""
+    issued = min(steps, fails_at + stages)
+    waited = range(max(0, issued - stages), issued) if issued < steps or not only_if_gave_up else ()
+    return [n for n in range(fails_at, issued) if n not in waited]
+
+
+@pytest.mark.parametrize("kernel,begin", [("few_rows", "if (warp == kWarps) {"), ("many_rows", "if (warp == C::LOADER) {")])
+def test_no_copy_is_in_flight_when_the_shared_memory_is_used_again(kernel, begin):
+    part = loader_part(kernel, begin)
+    assert part.count("&quiet") >= 1, "the loader waits for its copies, whatever the state of the block"
+    drain = part[: part.index("int quiet")]
+    only_if_gave_up = re.search(r"if \(n < (steps|items)\) \{[^}]*$", drain) is not None
+    for steps, stages in itertools.product(range(1, 9), range(1, 5)):
+        for fails_at in range(steps):
+            assert not in_flight_at_the_end(steps, stages, fails_at, only_if_gave_up), (steps, stages, fails_at)
+
+
+def test_rows_are_staged_only_if_no_softmax_warp_gave_up():
+    """O goes to global memory through the memory of K and V tiles, which hold late copies if a wait has run out."""
+    kernel = SOURCE[SOURCE.index("many_rows(const __grid_constant__") :]
+    end = kernel[kernel.index("wait(p_empty + w, (mine - 1) & 1)") : kernel.index("bulk_store(")]
+    assert re.search(r"ok = ek::barrier_all<3, 256>\(ok\);.*if \(!ok\) m = NAN, l = NAN;.*if \(mine > 0 && ok\)", end, re.S)
