@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_consta
         }
         if (I8) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[i] = s[i] == 0.f ? 0.f : s[i] * vs[i / 2];
+          for (int i = 0; i < 4; ++i) s[i] *= vs[i / 2];  // (0 past the end)
           load_scales(t + C::KEYS);
         }
         // probabilities are rounded to bf16 for the product: half a step is 2^-8 of each, as for V itself
