@@ -61,6 +61,8 @@ const Tensor& need(PyObject* o, const char* name, at::ScalarType type, int64_t d
   if (t.is_neg() || t.is_conj()) refuse(std::string(name) + ": has a pending negation or conjugation");
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse(std::string(name) + ": requires grad, but this operator has no backward pass (use torch.no_grad)");
+  if (t._fw_grad(0).defined())
+    refuse(std::string(name) + ": carries a tangent, but this operator has no forward derivative (use unpack_dual)");
   return t;
 }
 

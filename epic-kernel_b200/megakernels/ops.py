@@ -15,8 +15,9 @@ they were made on need torch's usual `record_stream`.
 
 Errors: a bad shape, dtype, stride or setting raises ValueError before
 anything is launched; a CUDA failure raises RuntimeError. There is no CPU path:
-CPU tensors raise ValueError. No operator has a backward pass: inputs that
-require grad raise ValueError while grad mode is on.
+CPU tensors raise ValueError. No operator has derivatives: tensors that require
+grad raise ValueError while grad mode is on, dual tensors of forward-mode
+differentiation always.
 """
 
 import ctypes
