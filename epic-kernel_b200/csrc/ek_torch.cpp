@@ -93,6 +93,11 @@ void no_overlap(const Tensor& t, const char* name) {
   }
 }
 
+// Counts a write, as torch's in-place operations do: autograd checks the tensors that it saved.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // K and V are written by different blocks.
 void apart(const Tensor& k, const Tensor& v, const char* what) {
   if (k.numel() && k.data_ptr() == v.data_ptr()) refuse(std::string(what) + ": K and V are the same memory");
@@ -185,6 +190,8 @@ void kv_copy(bool write, const Cache& c, const Tensor& k, const Tensor& v, py::h
   if (a.kv_heads == 0 || a.batch == 0 || a.length == 0) return;
   a.device = c.kc->device().index();
   check((write ? api.kv_write : api.kv_read)(&a, stream_of(k)), write ? "ek_kv_write" : "ek_kv_read");
+  if (write) written(*c.kc), written(*c.ks), written(*c.vc), written(*c.vs);
+  else written(k), written(v);
 }
 
 void kv_write(const py::tuple& cache, py::handle ko, py::handle vo, py::handle start) {
@@ -283,6 +290,7 @@ py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& ow
   Tensor workspace = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte));
   a.workspace = workspace.data_ptr();
   check(api.attention(&a, stream_of(q)), "ek_prefix_attention");
+  written(out);
   py::object result = out_o.is_none() ? py::cast(out) : py::reinterpret_borrow<py::object>(out_o);
   if (return_lse) return py::make_tuple(result, lse);
   return result;
@@ -355,6 +363,7 @@ py::object sample(py::handle logits_o, py::handle uniforms_o, py::handle tempera
   a.batch = fit32(batch, "batch"), a.vocab = (int)vocab;
   a.device = logits.device().index();
   check(api.sample(&a, stream_of(logits)), "ek_sample");
+  written(out);
   return out_o.is_none() ? py::cast(out) : py::reinterpret_borrow<py::object>(out_o);
 }
 
