@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -98,9 +99,64 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// K and V are written by different blocks.
-void apart(const Tensor& k, const Tensor& v, const char* what) {
-  if (k.numel() && k.data_ptr() == v.data_ptr()) refuse(std::string(what) + ": K and V are the same memory");
+// The bytes of a tensor: start + sum of index * step over its dimensions, neighbouring ones joined.
+struct Bytes {
+  int64_t start = 0, span = 0;  // addresses start .. start + span - 1; none if span is 0
+  int dims = 0;
+  int64_t n[9], step[9];
+
+  explicit Bytes(const Tensor& t) {
+    if (t.numel() == 0) return;
+    start = (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
+    span = t.element_size();
+    n[0] = span, step[0] = 1, dims = 1;
+    for (int64_t i = t.dim() - 1; i >= 0; --i) {
+      const int64_t size = t.size(i), at = t.stride(i) * (int64_t)t.element_size();
+      if (size == 1 || at == 0) continue;
+      span += (size - 1) * at;
+      if (at == n[dims - 1] * step[dims - 1]) n[dims - 1] *= size;
+      else n[dims] = size, step[dims] = at, ++dims;
+    }
+  }
+};
+
+// Whether a sum of d[i] * step[i], lo[i] <= d[i] <= hi[i], steps falling, can give `target`. Gives up with true (the
+// call is refused) once `budget` is spent, which rows of ordinary layouts never do.
+bool reachable(int64_t target, int dims, const int64_t* step, const int64_t* lo, const int64_t* hi, int& budget) {
+  if (dims == 0) return target == 0;
+  if (--budget < 0) return true;
+  int64_t low = 0, high = 0;  // what the smaller steps can give
+  for (int i = 1; i < dims; ++i) low += lo[i] * step[i], high += hi[i] * step[i];
+  auto down = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+  const int64_t first = std::max(lo[0], -down(high - target, step[0])), last = std::min(hi[0], down(target - low, step[0]));
+  for (int64_t d = first; d <= last; ++d)
+    if (reachable(target - d * step[0], dims - 1, step + 1, lo + 1, hi + 1, budget)) return true;
+  return false;
+}
+
+// Whether two tensors have a byte in common. Interleaved ones (K and V of a fused projection) have none.
+bool share_memory(const Bytes& a, const Bytes& b) {
+  if (!a.span || !b.span || a.start + a.span <= b.start || b.start + b.span <= a.start) return false;
+  int64_t step[18], lo[18], hi[18];
+  int dims = 0;
+  auto add = [&](int64_t s, int64_t from, int64_t to) {  // sorted by falling step, equal steps together
+    int i = 0;
+    while (i < dims && step[i] > s) ++i;
+    if (i == dims || step[i] != s) {
+      for (int j = dims++; j > i; --j) step[j] = step[j - 1], lo[j] = lo[j - 1], hi[j] = hi[j - 1];
+      step[i] = s, lo[i] = hi[i] = 0;
+    }
+    lo[i] += from, hi[i] += to;
+  };
+  for (int i = 0; i < a.dims; ++i) add(a.step[i], 0, a.n[i] - 1);
+  for (int i = 0; i < b.dims; ++i) add(b.step[i], 1 - b.n[i], 0);
+  int budget = 10000;
+  return reachable(b.start - a.start, dims, step, lo, hi, budget);
+}
+
+// Different blocks write `a` and read or write `b`, in any order.
+void apart(const Bytes& a, const Bytes& b, const char* what) {
+  if (share_memory(a, b)) refuse(std::string(what) + " are, in part, the same memory");
 }
 
 int64_t step(const Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
@@ -158,17 +214,37 @@ Cache take_cache(const py::tuple& t, const char* name, const Tensor* like = null
 
 void check_cache(const py::tuple& t) { take_cache(t, "cache"); }
 
-void kv_copy(bool write, const Cache& c, const Tensor& k, const Tensor& v, py::handle start) {
-  if (k.sizes() != v.sizes() || k.size(0) != c.kc->size(0) || k.sizes().slice(2) != c.kc->sizes().slice(2))
-    refuse("k " + shape_of(k) + " / v " + shape_of(v) + ": expected [batch, rows, kv_heads, head_dim] as in the cache " +
-           shape_of(*c.kc));
+// What the blocks of a copy write may not meet anything else of the call.
+void check_memory(bool write, const Cache& c, const Tensor& k, const Tensor& v, py::handle start) {
   if (write) {
     no_overlap(*c.kc, "k_codes"), no_overlap(*c.ks, "k_scales");
     no_overlap(*c.vc, "v_codes"), no_overlap(*c.vs, "v_scales");
-    apart(*c.kc, *c.vc, "cache codes"), apart(*c.ks, *c.vs, "cache scales");
   } else {
-    no_overlap(k, "out[0]"), no_overlap(v, "out[1]"), apart(k, v, "out");
+    no_overlap(k, "out[0]"), no_overlap(v, "out[1]");
   }
+  const Bytes values[2] = {Bytes(k), Bytes(v)}, cache[4] = {Bytes(*c.kc), Bytes(*c.ks), Bytes(*c.vc), Bytes(*c.vs)};
+  for (const Bytes& x : values)
+    for (const Bytes& y : cache) apart(x, y, write ? "rows and cache" : "out and cache");
+  if (write) {
+    for (int i = 1; i < 4; ++i)
+      for (int j = 0; j < i; ++j) apart(cache[i], cache[j], "tensors of the cache");
+  } else {
+    apart(values[0], values[1], "out: K and V");
+  }
+  if (THPVariable_Check(start.ptr())) {
+    const Bytes at(THPVariable_Unpack(start.ptr()));
+    if (write)
+      for (const Bytes& y : cache) apart(at, y, "start and cache");
+    else
+      for (const Bytes& x : values) apart(at, x, "start and out");
+  }
+}
+
+// `fresh`: k and v are new outputs, which nothing else shares.
+void kv_copy(bool write, bool fresh, const Cache& c, const Tensor& k, const Tensor& v, py::handle start) {
+  if (k.sizes() != v.sizes() || k.size(0) != c.kc->size(0) || k.sizes().slice(2) != c.kc->sizes().slice(2))
+    refuse("k " + shape_of(k) + " / v " + shape_of(v) + ": expected [batch, rows, kv_heads, head_dim] as in the cache " +
+           shape_of(*c.kc));
   EkKvCopyArgs a = {};
   a.k_values = describe(k, nullptr), a.v_values = describe(v, nullptr);
   a.k_cache = describe(*c.kc, c.ks), a.v_cache = describe(*c.vc, c.vs);
@@ -187,6 +263,7 @@ void kv_copy(bool write, const Cache& c, const Tensor& k, const Tensor& v, py::h
              std::to_string(a.capacity) + " rows");
     a.start_all = at;
   }
+  if (!fresh) check_memory(write, c, k, v, start);
   if (a.kv_heads == 0 || a.batch == 0 || a.length == 0) return;
   a.device = c.kc->device().index();
   check((write ? api.kv_write : api.kv_read)(&a, stream_of(k)), write ? "ek_kv_write" : "ek_kv_read");
@@ -198,7 +275,7 @@ void kv_write(const py::tuple& cache, py::handle ko, py::handle vo, py::handle s
   const Cache c = take_cache(cache, "cache");
   const Tensor& k = rows16(need(ko.ptr(), "k", at::kBFloat16, 4, c.kc), "k");
   const Tensor& v = rows16(need(vo.ptr(), "v", at::kBFloat16, 4, c.kc), "v");
-  kv_copy(true, c, k, v, start);
+  kv_copy(true, false, c, k, v, start);
 }
 
 py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::handle out) {
@@ -207,7 +284,7 @@ py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::
   if (out.is_none()) {
     const Tensor both = at::empty({2, c.kc->size(0), length, c.kc->size(2), c.kc->size(3)}, c.ks->options());
     const Tensor k = both.select(0, 0), v = both.select(0, 1);
-    kv_copy(false, c, k, v, start);
+    kv_copy(false, true, c, k, v, start);
     return py::make_tuple(k, v);
   }
   const py::sequence pair = py::reinterpret_borrow<py::sequence>(out);
@@ -216,7 +293,7 @@ py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::
   const Tensor& k = rows16(need(ko.ptr(), "out[0]", at::kBFloat16, 4, c.kc), "out[0]");
   const Tensor& v = rows16(need(vo.ptr(), "out[1]", at::kBFloat16, 4, c.kc), "out[1]");
   if (k.size(1) != length) refuse("out: " + std::to_string(k.size(1)) + " rows, expected " + std::to_string(length));
-  kv_copy(false, c, k, v, start);
+  kv_copy(false, false, c, k, v, start);
   return py::make_tuple(ko, vo);
 }
 
@@ -272,6 +349,8 @@ py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& ow
     out = rows16(need(out_o.ptr(), "out", at::kBFloat16, 3, &q), "out");
     no_overlap(out, "out");
     if (out.sizes() != q.sizes()) refuse("out: " + shape_of(out) + ", expected " + shape_of(q));
+    // (q, K and V have been read when the first result is written)
+    apart(Bytes(out), Bytes(lens), "out and own_lens");
   }
   Tensor lse;
   if (return_lse) lse = at::empty({batch, q_heads}, q.options().dtype(at::kFloat));
@@ -356,6 +435,10 @@ py::object sample(py::handle logits_o, py::handle uniforms_o, py::handle tempera
     out = need(out_o.ptr(), "out", at::kLong, 1, &logits);
     if (out.size(0) != batch || !out.is_contiguous())
       refuse("out: expected a contiguous int64 tensor of " + std::to_string(batch) + " tokens");
+    const Bytes at(out);
+    apart(at, Bytes(logits), "out and logits");
+    for (py::handle o : {uniforms_o, temperature, top_k, top_p, min_p})
+      if (THPVariable_Check(o.ptr())) apart(at, Bytes(THPVariable_Unpack(o.ptr())), "out and another input");
   }
   a.logits = logits.data_ptr(), a.uniforms = uniforms.data_ptr<float>(), a.tokens = out.data_ptr<int64_t>();
   a.row_stride = batch > 1 ? logits.stride(0) : 0;

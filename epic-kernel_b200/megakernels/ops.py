@@ -14,7 +14,9 @@ be captured into a CUDA graph. Tensors used on a stream other than the one that
 they were made on need torch's usual `record_stream`.
 
 Errors: a bad shape, dtype, stride or setting raises ValueError before
-anything is launched; a CUDA failure raises RuntimeError. There is no CPU path:
+anything is launched, and so does an output or cache in whose memory another
+argument lies (only results of `shared_prefix_attention` may replace q, K or
+V); a CUDA failure raises RuntimeError. There is no CPU path:
 CPU tensors raise ValueError. No operator has derivatives: tensors that require
 grad raise ValueError while grad mode is on, dual tensors of forward-mode
 differentiation always.
