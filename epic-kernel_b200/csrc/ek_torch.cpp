@@ -14,7 +14,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <optional>
 #include <string>
 
 #include "../../include/ek.h"
@@ -190,6 +189,26 @@ void head_dim_ok(int64_t d) {
   if (d != 64 && d != 128) refuse("head_dim " + std::to_string(d) + " (supported: 64, 128)");
 }
 
+double number(py::handle o, const char* name) {
+  const double x = PyFloat_AsDouble(o.ptr());
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(std::string(name) + ": expected a number");
+  }
+  return x;
+}
+
+int64_t whole_number(py::handle o, const char* name) {
+  PyObject* index = PyNumber_Index(o.ptr());
+  const long long x = index ? PyLong_AsLongLong(index) : -1;
+  Py_XDECREF(index);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(std::string(name) + ": expected a whole number of 64 bits");
+  }
+  return x;
+}
+
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // (codes, scales) of K and V: an 8-bit cache.
@@ -257,9 +276,9 @@ void kv_copy(bool write, bool fresh, const Cache& c, const Tensor& k, const Tens
       refuse("start: expected a contiguous int32 tensor of " + std::to_string(a.batch) + " positions");
     a.start = s.data_ptr<int32_t>();
   } else {
-    const int64_t at = py::cast<int64_t>(start);
+    const int64_t at = whole_number(start, "start");
     if (at < 0 || at > a.capacity - (int64_t)a.length)
-      refuse("rows " + std::to_string(at) + " .. " + std::to_string(at + a.length - 1) + " outside the cache of " +
+      refuse("start: " + std::to_string(a.length) + " rows from " + std::to_string(at) + " on lie outside the cache of " +
              std::to_string(a.capacity) + " rows");
     a.start_all = at;
   }
@@ -278,9 +297,11 @@ void kv_write(const py::tuple& cache, py::handle ko, py::handle vo, py::handle s
   kv_copy(true, false, c, k, v, start);
 }
 
-py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::handle out) {
+py::tuple kv_read(const py::tuple& cache, py::handle start, py::handle length_o, py::handle out) {
   const Cache c = take_cache(cache, "cache");
-  if (length < 0) refuse("length " + std::to_string(length));
+  const int64_t length = whole_number(length_o, "length");
+  if (length < 0 || (length > c.kc->size(1) && !THPVariable_Check(start.ptr())))  // (before anything is allocated)
+    refuse("length " + std::to_string(length) + ": outside the cache of " + std::to_string(c.kc->size(1)) + " rows");
   if (out.is_none()) {
     const Tensor both = at::empty({2, c.kc->size(0), length, c.kc->size(2), c.kc->size(3)}, c.ks->options());
     const Tensor k = both.select(0, 0), v = both.select(0, 1);
@@ -288,7 +309,7 @@ py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::
     return py::make_tuple(k, v);
   }
   const py::sequence pair = py::reinterpret_borrow<py::sequence>(out);
-  if (pair.size() != 2) refuse("out: expected a (k, v) pair");
+  if (!PySequence_Check(out.ptr()) || THPVariable_Check(out.ptr()) || pair.size() != 2) refuse("out: expected a (k, v) pair");
   const py::object ko = pair[0], vo = pair[1];
   const Tensor& k = rows16(need(ko.ptr(), "out[0]", at::kBFloat16, 4, c.kc), "out[0]");
   const Tensor& v = rows16(need(vo.ptr(), "out[1]", at::kBFloat16, 4, c.kc), "out[1]");
@@ -298,7 +319,7 @@ py::tuple kv_read(const py::tuple& cache, py::handle start, int64_t length, py::
 }
 
 py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& own, py::handle lens_o,
-                     std::optional<double> scale, std::optional<int64_t> max_own_len, py::handle out_o,
+                     py::handle scale, py::handle max_own_len, py::handle out_o,
                      bool return_lse) {
   const Tensor& q = rows16(need(qo.ptr(), "q", at::kBFloat16, 3), "q");
   const int64_t batch = q.size(0), q_heads = q.size(1), head_dim = q.size(2);
@@ -337,10 +358,10 @@ py::object attention(py::handle qo, const py::tuple& prefix, const py::tuple& ow
   const Tensor& lens = need(lens_o.ptr(), "own_lens", at::kInt, 1, &q);
   if (lens.size(0) != batch || !lens.is_contiguous())
     refuse("own_lens: expected a contiguous int32 tensor of " + std::to_string(batch) + " lengths");
-  const int64_t bound = max_own_len.value_or(rows);
+  const int64_t bound = max_own_len.is_none() ? rows : whole_number(max_own_len, "max_own_len");
   if (bound < 0 || bound > rows)
     refuse("max_own_len " + std::to_string(bound) + " outside the " + std::to_string(rows) + " own rows");
-  const double s = scale.value_or(1.0 / std::sqrt((double)head_dim));
+  const double s = scale.is_none() ? 1.0 / std::sqrt((double)head_dim) : number(scale, "scale");
   if (!std::isfinite((float)s)) refuse("scale: must be finite");
   Tensor out;
   if (out_o.is_none()) {
@@ -383,15 +404,6 @@ const V* per_row(py::handle o, const char* name, at::ScalarType type, const Tens
   if (t.size(0) != logits.size(0) || !t.is_contiguous())
     refuse(std::string(name) + ": expected a contiguous tensor of " + std::to_string(logits.size(0)) + " values");
   return t.data_ptr<V>();
-}
-
-double number(py::handle o, const char* name) {
-  const double x = PyFloat_AsDouble(o.ptr());
-  if (PyErr_Occurred()) {
-    PyErr_Clear();
-    refuse(std::string(name) + ": expected a number or a tensor");
-  }
-  return x;
 }
 
 py::object sample(py::handle logits_o, py::handle uniforms_o, py::handle temperature, py::handle top_k,
