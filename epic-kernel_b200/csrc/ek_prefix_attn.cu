@@ -36,17 +36,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int g_attention_status;  // 1: a wait inside a kernel ran out
 
-struct Store {
-  const char* k;
-  const char* v;
-  const __nv_bfloat16* ks;
-  const __nv_bfloat16* vs;
-  long long k_batch, k_row, k_head, v_batch, v_row, v_head;  // bytes
-  long long ks_batch, ks_row, ks_head, vs_batch, vs_row, vs_head;  // elements
+struct Scales {  // of 8-bit rows, which come by tensor maps themselves
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  long long k_batch, k_row, k_head, v_batch, v_row, v_head;  // elements
 };
 
 struct AttnParams {
-  Store prefix, own;
+  Scales prefix, own;
   const __nv_bfloat16* q;
   long long q_batch, q_head;
   __nv_bfloat16* out;
@@ -229,16 +226,16 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_consta
         }
       }
     }
-    const Store& store = shared ? p.prefix : p.own;
-    const __nv_bfloat16* ksb = store.ks + seq * store.ks_batch + head * store.ks_head;
-    const __nv_bfloat16* vsb = store.vs + seq * store.vs_batch + head * store.vs_head;
+    const Scales& scales = shared ? p.prefix : p.own;
+    const __nv_bfloat16* ksb = scales.k + seq * scales.k_batch + head * scales.k_head;
+    const __nv_bfloat16* vsb = scales.v + seq * scales.v_batch + head * scales.v_head;
     float ks[2], vs[2];  // scales of keys j and j + 8 of the step
     auto load_scales = [&](int t) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bool in = t + j + 8 * i < t1;
-        ks[i] = in ? __bfloat162float(ksb[(t + j + 8 * i) * store.ks_row]) : 0.f;
-        vs[i] = in ? __bfloat162float(vsb[(t + j + 8 * i) * store.vs_row]) : 0.f;
+        ks[i] = in ? __bfloat162float(ksb[(t + j + 8 * i) * scales.k_row]) : 0.f;
+        vs[i] = in ? __bfloat162float(vsb[(t + j + 8 * i) * scales.v_row]) : 0.f;
       }
     };
     if (I8) load_scales(t0 + warp * 16);
@@ -586,8 +583,8 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
     auto key_scale = [&](int use, int kv) {
       const int key = (tile0 + (wide ? use : 2 * use + w)) * 128 + t;
       if (use >= mine || key >= p.a.prefix_len) return kv ? 0.f : 1.f;  // masked scores stay -inf
-      const Store& s = p.a.prefix;
-      return __bfloat162float(kv ? s.vs[key * s.vs_row + head * s.vs_head] : s.ks[key * s.ks_row + head * s.ks_head]);
+      const Scales& s = p.a.prefix;
+      return __bfloat162float(kv ? s.v[key * s.v_row + head * s.v_head] : s.k[key * s.k_row + head * s.k_head]);
     };
     float next_ks = 0.f, next_vs = 0.f;
     if (I8) next_ks = key_scale(0, 0), next_vs = key_scale(0, 1);
@@ -1068,8 +1065,8 @@ int encode_rows(RowMap& m, const EkKvTensor& t, int batch, int rows, int heads, 
   return EK_SUCCESS;
 }
 
-// Fills one side of `s`; checks alignment and kind when there are rows.
-int take_store(const EkKvTensor& k, const EkKvTensor& v, int rows, bool i8, const char* name, Store& s) {
+// Checks alignment and kind of K and V when there are rows, and takes their scales.
+int take_rows(const EkKvTensor& k, const EkKvTensor& v, int rows, bool i8, const char* name, Scales& s) {
   using ek::fail;
   if (rows > 0) {
     const int unit = i8 ? 16 : 8;
@@ -1080,13 +1077,9 @@ int take_store(const EkKvTensor& k, const EkKvTensor& v, int rows, bool i8, cons
       if ((t->scales != nullptr) != i8) return fail(EK_E_INVALID, "prefix and own rows must be of one kind");
     }
   }
-  const int size = i8 ? 1 : 2;
-  s.k = static_cast<const char*>(k.data), s.v = static_cast<const char*>(v.data);
-  s.ks = static_cast<const __nv_bfloat16*>(k.scales), s.vs = static_cast<const __nv_bfloat16*>(v.scales);
-  s.k_batch = k.stride_batch * size, s.k_row = k.stride_row * size, s.k_head = k.stride_head * size;
-  s.v_batch = v.stride_batch * size, s.v_row = v.stride_row * size, s.v_head = v.stride_head * size;
-  s.ks_batch = k.scale_stride_batch, s.ks_row = k.scale_stride_row, s.ks_head = k.scale_stride_head;
-  s.vs_batch = v.scale_stride_batch, s.vs_row = v.scale_stride_row, s.vs_head = v.scale_stride_head;
+  s.k = static_cast<const __nv_bfloat16*>(k.scales), s.v = static_cast<const __nv_bfloat16*>(v.scales);
+  s.k_batch = k.scale_stride_batch, s.k_row = k.scale_stride_row, s.k_head = k.scale_stride_head;
+  s.v_batch = v.scale_stride_batch, s.v_row = v.scale_stride_row, s.v_head = v.scale_stride_head;
   return EK_SUCCESS;
 }
 
@@ -1164,8 +1157,8 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
   const bool i8 = (a->prefix_len > 0 ? a->prefix_k.scales : a->own_k.scales) != nullptr;
   FewParams few;
   AttnParams& p = few.a;
-  if ((rc = take_store(a->prefix_k, a->prefix_v, a->prefix_len, i8, "prefix", p.prefix))) return rc;
-  if ((rc = take_store(a->own_k, a->own_v, a->max_own_len > 0 ? a->own_capacity : 0, i8, "own", p.own))) return rc;
+  if ((rc = take_rows(a->prefix_k, a->prefix_v, a->prefix_len, i8, "prefix", p.prefix))) return rc;
+  if ((rc = take_rows(a->own_k, a->own_v, a->max_own_len > 0 ? a->own_capacity : 0, i8, "own", p.own))) return rc;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.q_batch = a->q_stride_batch, p.q_head = a->q_stride_head;
   p.out = static_cast<__nv_bfloat16*>(a->out);
