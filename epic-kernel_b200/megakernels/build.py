@@ -10,6 +10,7 @@ import argparse
 import os
 import shutil
 import subprocess
+import warnings
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent.parent
@@ -62,45 +63,74 @@ def binding_command(out: Path) -> list[str]:
             f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
 
 
-def stale() -> bool:
-    if not OUT.exists() or not BINDING.exists():
+def binding_problem() -> str | None:
+    """What keeps the tensor binding from being built here, or None. libek.so needs nvcc only."""
+    try:
+        gxx_path()
+        import torch
+        from torch.utils import cpp_extension  # noqa: F401
+    except (RuntimeError, ImportError) as e:
+        return str(e)
+    return None if torch.version.cuda else "torch is built without CUDA"
+
+
+def _stale(target: Path, kinds: tuple[str, ...]) -> bool:
+    if not target.exists():
         return True
-    t = min(OUT.stat().st_mtime, BINDING.stat().st_mtime)
-    deps = [f for kind in ("*.cu", "*.cuh", "*.h", "*.cpp") for f in CSRC.glob(kind)]
+    deps = [f for kind in kinds for f in CSRC.glob(kind)]
     deps.append(PKG_ROOT.parent / "include" / "ek.h")
-    return any(d.stat().st_mtime > t for d in deps if d.exists())
+    return any(d.stat().st_mtime > target.stat().st_mtime for d in deps if d.exists())
+
+
+def engine_stale() -> bool:
+    return _stale(OUT, ("*.cu", "*.cuh", "*.h"))
+
+
+def binding_stale() -> bool:
+    return _stale(BINDING, ("*.cpp",))
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not stale():
+    """Builds what is older than its sources. libek.so comes first: what only the binding needs may be missing (a
+    warning says so), and a binding that does not compile raises with the new libek.so in place."""
+    engine, binding = force or engine_stale(), force or binding_stale()
+    if not engine and not binding:
         return OUT
     from concurrent.futures import ThreadPoolExecutor
-
-    nvcc = nvcc_path()
-    objdir = PKG_ROOT / "_build"
-    objdir.mkdir(exist_ok=True)
-    jobs = []
-    for name, macros in VARIANTS:
-        defs = [f"-D{k}={v}" for k, v in macros.items()] + [f"-DEK_NS={name}"]
-        jobs.append([nvcc, *COMPILE_FLAGS, *defs, "-c", "-o", str(objdir / f"ek_decode_{name}.o"),
-                     str(CSRC / "ek_decode.cu")])
-    for name in SOURCES:
-        jobs.append([nvcc, *COMPILE_FLAGS, "-c", "-o", str(objdir / f"{name}.o"), str(CSRC / f"{name}.cu")])
 
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, cwd=PKG_ROOT)
 
-    binding = BINDING.with_suffix(".so.tmp")
-    jobs.append(binding_command(binding))
-    with ThreadPoolExecutor(max_workers=len(jobs)) as ex:
-        list(ex.map(run, jobs))
-    binding.replace(BINDING)
-    tmp = OUT.with_suffix(".so.tmp")
-    objs = [str(objdir / f"ek_decode_{n}.o") for n, _ in VARIANTS] + [str(objdir / f"{n}.o") for n in SOURCES]
-    run([nvcc, *LINK_FLAGS, "-o", str(tmp), *objs])
-    tmp.replace(OUT)
+    def build_binding():
+        tmp = BINDING.with_suffix(".so.tmp")
+        run(binding_command(tmp))
+        tmp.replace(BINDING)
+
+    problem = binding_problem() if binding else None
+    with ThreadPoolExecutor(max_workers=len(VARIANTS) + len(SOURCES) + 1) as ex:
+        bound = ex.submit(build_binding) if binding and problem is None else None
+        if engine:
+            nvcc = nvcc_path()
+            objdir = PKG_ROOT / "_build"
+            objdir.mkdir(exist_ok=True)
+            jobs = []
+            for name, macros in VARIANTS:
+                defs = [f"-D{k}={v}" for k, v in macros.items()] + [f"-DEK_NS={name}"]
+                jobs.append([nvcc, *COMPILE_FLAGS, *defs, "-c", "-o", str(objdir / f"ek_decode_{name}.o"),
+                             str(CSRC / "ek_decode.cu")])
+            for name in SOURCES:
+                jobs.append([nvcc, *COMPILE_FLAGS, "-c", "-o", str(objdir / f"{name}.o"), str(CSRC / f"{name}.cu")])
+            list(ex.map(run, jobs))
+            tmp = OUT.with_suffix(".so.tmp")
+            objs = [str(objdir / f"ek_decode_{n}.o") for n, _ in VARIANTS] + [str(objdir / f"{n}.o") for n in SOURCES]
+            run([nvcc, *LINK_FLAGS, "-o", str(tmp), *objs])
+            tmp.replace(OUT)
+        if bound is not None:
+            bound.result()
+    if problem is not None:
+        warnings.warn(f"{BINDING.name} is not built: {problem}", RuntimeWarning, stacklevel=2)
     return OUT
 
 
