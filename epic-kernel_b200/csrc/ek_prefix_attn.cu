@@ -1118,7 +1118,8 @@ cudaError_t launch(const FewParams& p, const ManyParams* many, cudaStream_t st) 
       (e = start(few_rows<D, I8>, p, items, kWarps * 32 + 32, Few<D, I8>::SMEM, false, st)) != cudaSuccess)
     return e;
   if (many) {
-    // the warpgroups take more registers out of those that the block is launched with
+    // The warpgroups take more registers out of those that the block is launched with. The build compares the numbers;
+    // this keeps a library built in another way from waiting for good.
     cudaFuncAttributes attr;
     if ((e = cudaFuncGetAttributes(&attr, many_rows<D, I8>)) != cudaSuccess) return e;
     if (attr.numRegs != M::REGS) return cudaErrorLaunchOutOfResources;

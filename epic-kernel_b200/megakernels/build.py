@@ -10,6 +10,7 @@ import argparse
 import os
 import shutil
 import subprocess
+import sys
 import warnings
 from pathlib import Path
 
@@ -74,6 +75,29 @@ def binding_problem() -> str | None:
     return None if torch.version.cuda else "torch is built without CUDA"
 
 
+def expected_registers() -> dict[int, int]:
+    """Registers per thread that the warpgroups of `many_rows` share out among themselves, by kind (0: bf16, 1: int8).
+    With fewer at launch they would wait for good; the launch refuses that too."""
+    import re
+
+    m = re.search(r"int REGS = I8 \? (\d+) : (\d+)", (CSRC / "ek_prefix_attn.cu").read_text())
+    return {0: int(m.group(2)), 1: int(m.group(1))}
+
+
+def check_registers(log: str):
+    """Compares what the compiler allotted to each many_rows<D, I8> with the kernel's numbers."""
+    import re
+
+    found = re.findall(r"Compiling entry function '\S*many_rowsILi(\d+)ELb([01])E\S*'.*?Used (\d+) registers", log, re.S)
+    expected = expected_registers()
+    for d, i8, n in found:
+        if int(n) != expected[int(i8)]:
+            raise RuntimeError(f"ek_prefix_attn.cu: many_rows<{d}, {i8}> got {n} registers per thread from this compiler, "
+                               f"its warpgroups count on {expected[int(i8)]}")
+    if len(found) != 4:
+        raise RuntimeError(f"ek_prefix_attn.cu: the compiler reported registers of {len(found)} of 4 many_rows kernels")
+
+
 def _stale(target: Path, kinds: tuple[str, ...]) -> bool:
     if not target.exists():
         return True
@@ -101,7 +125,14 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True, cwd=PKG_ROOT)
+        if "-v" not in cmd:
+            subprocess.run(cmd, check=True, cwd=PKG_ROOT)
+            return
+        done = subprocess.run(cmd, cwd=PKG_ROOT, stderr=subprocess.PIPE, text=True)
+        if done.returncode:
+            print(done.stderr, file=sys.stderr, flush=True)
+            raise subprocess.CalledProcessError(done.returncode, cmd)
+        check_registers(done.stderr)
 
     def build_binding():
         tmp = BINDING.with_suffix(".so.tmp")
@@ -121,7 +152,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
                 jobs.append([nvcc, *COMPILE_FLAGS, *defs, "-c", "-o", str(objdir / f"ek_decode_{name}.o"),
                              str(CSRC / "ek_decode.cu")])
             for name in SOURCES:
-                jobs.append([nvcc, *COMPILE_FLAGS, "-c", "-o", str(objdir / f"{name}.o"), str(CSRC / f"{name}.cu")])
+                report = ["-Xptxas", "-v"] if name == "ek_prefix_attn" else []  # for check_registers
+                jobs.append([nvcc, *COMPILE_FLAGS, *report, "-c", "-o", str(objdir / f"{name}.o"), str(CSRC / f"{name}.cu")])
             list(ex.map(run, jobs))
             tmp = OUT.with_suffix(".so.tmp")
             objs = [str(objdir / f"ek_decode_{n}.o") for n, _ in VARIANTS] + [str(objdir / f"{n}.o") for n in SOURCES]

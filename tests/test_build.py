@@ -15,6 +15,7 @@ def tree(tmp_path, monkeypatch):
     csrc.mkdir(parents=True)
     for name in ("ek_capi.cu", "ek_torch.cpp", "ek_host.h"):
         (csrc / name).write_text("")
+    (csrc / "ek_prefix_attn.cu").write_text("int REGS = I8 ? 128 : 168;")
     for name, value in {"PKG_ROOT": tmp_path / "pkg", "CSRC": csrc, "OUT": tmp_path / "pkg" / "libek.so",
                         "BINDING": tmp_path / "pkg" / "_ekops.so"}.items():
         monkeypatch.setattr(b, name, value)
@@ -85,3 +86,22 @@ def test_a_binding_that_does_not_compile_is_an_error_after_the_engine(tree):
     with pytest.raises(subprocess.CalledProcessError):
         b.build()
     assert b.OUT.exists() and not b.BINDING.exists()
+
+
+def test_registers_of_the_tensor_core_kernel_are_checked(tree, monkeypatch):
+    """A compiler that allots others than the kernel's split of registers counts on fails the build."""
+    text = "constexpr int REGS = I8 ? 128 : 168, SOFTMAX_REGS = 200;"
+    (b.CSRC / "ek_prefix_attn.cu").write_text(text)
+    b.build()
+    assert any("-v" in c for c in compiled(tree, "ek_prefix_attn.cu"))
+    (b.CSRC / "ek_prefix_attn.cu").write_text(text.replace("168", "160"))
+    with pytest.raises(RuntimeError, match="many_rows.*168 registers.*160"):
+        b.build(force=True)
+    monkeypatch.setattr(b.subprocess, "run", lambda cmd, **kw: subprocess.CompletedProcess(cmd, 0, stdout="", stderr=""))
+    with pytest.raises(RuntimeError, match="many_rows"):
+        b.build(force=True)
+
+
+def test_registers_of_the_source_as_it_is():
+    """The numbers that the build compares with are found in the kernel's source."""
+    assert b.expected_registers() == {0: 168, 1: 128}
