@@ -18,6 +18,7 @@ the model's cache, to go on with the megakernel at batch 1.
 from dataclasses import dataclass
 
 import torch
+import torch.distributed as dist
 from torch import Tensor
 
 from megakernels import ops
@@ -30,7 +31,9 @@ from megakernels.scheduler import Schedule
 class SamplingParams:
     """How tokens are drawn from the logits (see `ops.sample_tokens`). `generator`
     is the torch generator of the random numbers, on the logits' device; None
-    uses torch's default one. temperature 0 takes the largest logit."""
+    uses torch's default one. temperature 0 takes the largest logit. With several
+    tensor-parallel ranks the first one's generator serves all; the other
+    settings must be the same on every rank."""
 
     temperature: float = 1.0
     top_k: int = 0
@@ -40,26 +43,38 @@ class SamplingParams:
 
 
 class _Sampler:
-    """Draws tokens with the random numbers of a generator, which are made for many steps at once."""
+    """Draws tokens with the random numbers of a generator, which are made for many steps at once.
+
+    globs: the globals of a tensor-parallel model. All its ranks must draw the same token, so they use the numbers of
+    the first rank's generator, exchanged on the host once per STEPS steps; all ranks take the same steps."""
 
     STEPS = 256
 
-    def __init__(self, params: SamplingParams, rows: int):
+    def __init__(self, params: SamplingParams, rows: int, globs=None):
         self.params = params
         self.rows = rows
+        self.globs = globs
         self.step = self.STEPS
+
+    def draw(self, device) -> Tensor:
+        """The next step's uniforms `[rows]`."""
+        if self.step == self.STEPS:
+            self.uniforms = torch.rand((self.STEPS, self.rows), generator=self.params.generator, device=device)
+            if getattr(self.globs, "tp_world", 1) > 1:
+                group = self.globs.tp_group
+                numbers = [self.uniforms.cpu()]
+                dist.broadcast_object_list(numbers, src=dist.get_global_rank(group, 0) if group else 0, group=group)
+                self.uniforms.copy_(numbers[0])
+            self.step = 0
+        self.step += 1
+        return self.uniforms[self.step - 1]
 
     def __call__(self, logits: Tensor, out: Tensor | None = None) -> Tensor:
         p = self.params
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("sampling cannot be captured: a replay would use the same random numbers again")
-        if self.step == self.STEPS:
-            self.uniforms = torch.rand((self.STEPS, self.rows), generator=p.generator, device=logits.device)
-            self.step = 0
-        u = self.uniforms[self.step]
-        self.step += 1
-        return ops.sample_tokens(logits, u, temperature=p.temperature, top_k=p.top_k, top_p=p.top_p, min_p=p.min_p,
-                                 out=out)
+        return ops.sample_tokens(logits, self.draw(logits.device), temperature=p.temperature, top_k=p.top_k,
+                                 top_p=p.top_p, min_p=p.min_p, out=out)
 
 
 class Generator:
@@ -92,7 +107,7 @@ class MK_Generator(Generator):
         self.barrier_fill_val = barrier_fill_val
         self.skip_mk = skip_mk
         self.skip_rest = skip_rest
-        self.sampler = _Sampler(sampling, 1) if sampling is not None else None
+        self.sampler = _Sampler(sampling, 1, schedule.globs) if sampling is not None else None
         self.fill()
 
     def _fused_step(self) -> bool:

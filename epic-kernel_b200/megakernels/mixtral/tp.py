@@ -63,6 +63,7 @@ def setup_tensor_parallel(globs, rank: int, world: int, group=None):
     ek.check(lib.ek_tp_connect(ctx.handle, handles), "ek_tp_connect")
     globs.logits = _bf16_view(logits_ptr.value, full_vocab, dev)
     globs.logits.zero_()
+    globs.tp_world, globs.tp_group = world, group  # for what the ranks must agree on (sampling)
     torch.cuda.synchronize(dev)
     if group is not None or dist.is_initialized():
         dist.barrier(group=group)
