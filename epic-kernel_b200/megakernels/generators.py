@@ -31,9 +31,11 @@ from megakernels.scheduler import Schedule
 class SamplingParams:
     """How tokens are drawn from the logits (see `ops.sample_tokens`). `generator`
     is the torch generator of the random numbers, on the logits' device; None
-    uses torch's default one. temperature 0 takes the largest logit. With several
+    uses torch's default one; seeding it anew takes effect at the next token.
+    temperature 0 takes the largest logit. With several
     tensor-parallel ranks the first one's generator serves all; the other
-    settings must be the same on every rank."""
+    settings must be the same on every rank, and a new seed waits for the next
+    block of numbers."""
 
     temperature: float = 1.0
     top_k: int = 0
@@ -56,9 +58,20 @@ class _Sampler:
         self.globs = globs
         self.step = self.STEPS
 
+    def _place(self, device):
+        """Where the generator stands: numbers left over are dropped when it was seeded or used since. Several ranks,
+        which must make new numbers at the same step, keep to the steps."""
+        g = self.params.generator
+        if device.type != "cuda" or getattr(self.globs, "tp_world", 1) > 1:
+            return None
+        if g is None:
+            g = torch.cuda.default_generators[torch.cuda.current_device() if device.index is None else device.index]
+        return g.initial_seed(), g.get_offset()
+
     def draw(self, device) -> Tensor:
         """The next step's uniforms `[rows]`."""
-        if self.step == self.STEPS:
+        device = torch.device(device)
+        if self.step == self.STEPS or self._place(device) != self.place:
             self.uniforms = torch.rand((self.STEPS, self.rows), generator=self.params.generator, device=device)
             if getattr(self.globs, "tp_world", 1) > 1:
                 group = self.globs.tp_group
@@ -66,6 +79,7 @@ class _Sampler:
                 dist.broadcast_object_list(numbers, src=dist.get_global_rank(group, 0) if group else 0, group=group)
                 self.uniforms.copy_(numbers[0])
             self.step = 0
+            self.place = self._place(device)
         self.step += 1
         return self.uniforms[self.step - 1]
 
