@@ -285,6 +285,14 @@ class ParallelGenerator(Generator):
         for i in range(ntok):
             src = ntok_already_generated + i - 1
             output_tokens[:, src + 1] = self.run(output_tokens[:, src])
+        self.check()
+
+    def check(self):
+        """Wait for the steps so far; RuntimeError if a wait inside their attention ran out. Logits, tokens and cached
+        rows since then are worthless. `generate` ends and `hand_over` begins with it; callers of `run` call it themselves."""
+        if ops.attention_status(self.model.device):
+            raise RuntimeError("ParallelGenerator: a wait inside the attention ran out; the tokens since the last check "
+                               "are not valid")
 
     def hand_over(self, index: int) -> int:
         """Copy the rows of sequence `index` behind the prompt in the model's
@@ -292,6 +300,7 @@ class ParallelGenerator(Generator):
         (prompt and new tokens)."""
         if not 0 <= index < self.num_sequences:
             raise ValueError(f"sequence {index} of {self.num_sequences}")
+        self.check()
         n, end = self.new_tokens, self.prompt_len + self.new_tokens
         k_cache, v_cache = self.model.stacked_kv_cache
         for l, own in enumerate(self.own):
