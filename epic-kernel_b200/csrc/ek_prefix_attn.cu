@@ -457,7 +457,10 @@ struct ManyParams {
   AttnParams a;
   int rows, wide_blocks, narrow_rows;  // rows of a KV head; blocks of 256; rows left for a narrow block
   int wide_splits, wide_tiles, narrow_splits, narrow_tiles;  // splits of the keys and 128-key tiles of each
-  int negate;                   // scale < 0: q is negated and |scale| used
+  // Masked scores are -inf times the scale, so that is kept positive. scale < 0: q is negated. scale = 0: q is 0
+  // (infinities and NaN are NaN, as 0 times their products).
+  uint32_t q_flip;              // bits of q to turn
+  int q_zero;
 };
 
 
@@ -564,7 +567,13 @@ __global__ void __launch_bounds__(Many<D, I8>::WARPS * 32, 1) many_rows(const __
         for (int u = 0; u < BATCH; ++u) {
           if (i + u * ROWS >= rows) continue;
           const int r = first + i + u * ROWS, t = r % 128;
-          if (p.negate) x[u].x ^= 0x80008000u, x[u].y ^= 0x80008000u, x[u].z ^= 0x80008000u, x[u].w ^= 0x80008000u;
+          if (p.q_zero || p.q_flip) {
+            auto turn = [&](uint32_t y) {
+              const uint32_t nan = __vcmpeq2(y & 0x7f807f80u, 0x7f807f80u) & 0x7fc07fc0u;
+              return p.q_zero ? nan : y ^ p.q_flip;
+            };
+            x[u] = make_uint4(turn(x[u].x), turn(x[u].y), turn(x[u].z), turn(x[u].w));
+          }
           *reinterpret_cast<uint4*>(smem + r / 128 * C::TILE + piece / 8 * 16384 + t * 128 + ((piece % 8 ^ (t & 7)) << 4)) = x[u];
         }
       }
@@ -1201,9 +1210,9 @@ extern "C" int ek_prefix_attention(const EkPrefixAttnArgs* a, void* stream) {
     m.wide_blocks = pl.wide_blocks, m.narrow_rows = pl.narrow_rows;
     m.wide_splits = pl.wide_splits, m.wide_tiles = pl.wide_tiles;
     m.narrow_splits = pl.narrow_splits, m.narrow_tiles = pl.narrow_tiles;
-    // masked scores are -inf times the scale, so it is kept positive; 1e-30 stands for 0
-    m.negate = p.scale_log2 < 0.f;
-    m.a.scale_log2 = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
+    m.q_flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+    m.q_zero = p.scale_log2 == 0.f;
+    m.a.scale_log2 = m.q_zero ? kLog2e : fabsf(p.scale_log2);
     p.prefix_tiles = 0;  // nothing of the prefix is left for few_rows
   } else if (a->prefix_len > 0 &&
              (rc = encode(few.prefix_k, few.prefix_v, a->prefix_k, a->prefix_v, 1, a->prefix_len, kBox, few_swizzle))) {
