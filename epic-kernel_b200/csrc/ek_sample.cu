@@ -312,10 +312,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_rows(const S
     }
   };
 
-  const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
+  const float given = p.temperature ? p.temperature[b] : p.temperature_all;
+  const bool flat = given == INFINITY;  // all weights are 1: as the largest finite temperature, but for min-p
+  const float temp = flat ? 3.402823466e38f : given;
   const int k = p.top_k ? p.top_k[b] : p.top_k_all;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
+  const float min_p = flat ? 0.f : p.min_p ? p.min_p[b] : p.min_p_all;
   const bool use_k = k > 0 && k < p.vocab, use_p = top_p < 1.f;
   // list the kept tokens while the row is read
   const bool online = !RESIDENT && min_p > 0.f && !use_k && !use_p && temp > 0.f;

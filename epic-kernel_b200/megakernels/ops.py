@@ -195,5 +195,8 @@ def sample_tokens(logits: Tensor, uniforms: Tensor, *, temperature: float | Tens
     Weights are summed in fixed point, so the same inputs give the same token in
     every launch. NaN logits count as -inf (never drawn); several logits of
     +inf share the weight; a row without any logit above -inf gives token 0.
-    Uniforms outside [0, 1) count as the nearest value inside."""
+    Uniforms outside [0, 1) count as the nearest value inside. Settings per row
+    are not checked: temperatures below 0 and NaN count as 0, +inf gives all
+    logits above -inf the weight 1; other settings outside their range count as
+    the nearest value inside, NaN as no filter."""
     return _native().sample(logits, uniforms, temperature, top_k, top_p, min_p, out, MAX_VOCAB)

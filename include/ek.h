@@ -368,8 +368,9 @@ typedef struct EkSampleArgs {
  * w_i >= min_p; the token is the first kept i, by index, whose running weight
  * exceeds uniform * (kept weight). Weights are summed in fixed point
  * (2^-42 of the largest or finer), so the result does not depend on the
- * order of the additions. temperature <= 0: the largest logit. NaN logits
- * count as -inf; a row without any logit above -inf gives 0. */
+ * order of the additions. temperature <= 0 or NaN: the largest logit; +inf:
+ * every w_i is 1. top_p < 0 and min_p > 1 count as 0 and 1, NaN as no filter.
+ * NaN logits count as -inf; a row without any logit above -inf gives 0. */
 int ek_sample(const EkSampleArgs* args, void* stream);
 
 /* Copy the device status record to `out` (synchronises with all work queued
