@@ -122,7 +122,8 @@ def kv_cache_write(cache: KVCacheInt8, k: Tensor, v: Tensor, start: int | Tensor
 
     Per (row, head): scale = max|x| / 127 rounded up to bf16 (at least 2^-126),
     code = x / scale rounded half away from zero, so a value is off by at most
-    half a scale. A head holding a NaN or an infinity reads back as NaN."""
+    half a scale. A head holding a NaN or an infinity reads back as NaN; the
+    largest finite bf16 value reads back as infinity (127 scales round to it)."""
     _native().kv_write(_cache_tensors(cache), k, v, start)
 
 
