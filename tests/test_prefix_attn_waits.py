@@ -19,7 +19,7 @@ def softmax_loop():
     body = kernel[start : kernel.index("wait(p_empty + w, (mine - 1) & 1)", start)]
     condition = re.match(r"for \(int use = 0; ([^;]*);", body).group(1)
     operations = []
-    pattern = (r"if \(!\(ok = agree<[^>]*>\(ok\)[^;]*\)\) break;|if \(!\(ok = agree\(ok\)\)\) (?:break);|^\s*sync\(\);|"
+    pattern = (r"if \(!\(ok = agree\(ok\)\)\) break;|^\s*sync\(\);|"
                r"if \((?:use > 0 && )?!\(ok = spin\((\w+) \+ w, [^;]*\)\)\) (break|continue);")
     for m in re.finditer(pattern, body, re.M):
         if "agree" in m.group(0):
