@@ -415,6 +415,9 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) few_rows(const __grid_consta
 // grows by more than 2^8; until then the old one stays in use, which changes
 // no ratio.
 //
+// P is rounded to bf16, V's type, by at most 2^-8 of each probability (times V's scale, with 8-bit rows), while the sums
+// keep it in fp32. The rest of P as a second operand would double the products with V, half of the tensor core's work.
+//
 // K and V tiles come by TMA (128-byte swizzle) into a ring, in the order in
 // which the products use them. 8-bit tiles land in a raw ring and four warps
 // widen them to bf16 in the swizzled layout; the scales of keys multiply
